@@ -16,6 +16,7 @@
 #include <string>
 #include <vector>
 
+#include "capi_shared.h"
 #include "ofh_kernels.h"
 #include "stream_key.h"
 
@@ -955,6 +956,44 @@ void f32_to_half_bits(const float* in, uint16_t* out, size_t n, int dtype) {
 }
 
 }  // namespace
+
+namespace ofh {
+
+int api_error(int code, const std::string& msg) { return set_error(code, msg); }
+
+int ScratchLease::acquire(size_t bytes, hipStream_t stream, bool& fits) {
+    fits = true;
+    stream_ = stream;
+    g_scratch_mu.lock();
+    locked_ = true;
+    const bool capturing = stream_capturing(stream);
+    if (capturing && capture_scratch_bytes_locked(stream) < bytes) {
+        fits = false;
+        return OFH_SUCCESS;
+    }
+    SharedScratch* shared = nullptr;
+    if (int rc = library_scratch_locked(bytes, stream, capturing, &ptr, &shared)) return rc;
+    shared_ = shared;
+    return OFH_SUCCESS;
+}
+
+int ScratchLease::release() {
+    SharedScratch* sh = static_cast<SharedScratch*>(shared_);
+    shared_ = nullptr;
+    const int rc = sh == nullptr ? (int)OFH_SUCCESS : shared_scratch_release(sh, stream_);
+    if (locked_) g_scratch_mu.unlock();
+    locked_ = false;
+    return rc;
+}
+
+// (an error path: the call's own error message stays)
+ScratchLease::~ScratchLease() {
+    SharedScratch* sh = static_cast<SharedScratch*>(shared_);
+    if (sh != nullptr && hipEventRecord(sh->last_use, stream_) == hipSuccess) sh->recorded = true;
+    if (locked_) g_scratch_mu.unlock();
+}
+
+}  // namespace ofh
 
 extern "C" {
 

@@ -25,6 +25,7 @@ OFH_ERROR_INVALID_ARGUMENT = 1
 OFH_ERROR_UNSUPPORTED = 2
 OFH_ERROR_HIP = 3
 OFH_ERROR_WORKSPACE_TOO_SMALL = 4
+OFH_ERROR_OUT_OF_PAGES = 5
 
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 BIAS_NONE, BIAS_ALIBI, BIAS_DENSE = 0, 1, 2
@@ -42,6 +43,26 @@ EXPORTED_SYMBOLS = (
     "ofh_attention_useful_flops",
     "ofh_qk_score_params_init",
     "ofh_qk_score_tile",
+    "ofh_window_params_init",
+    "ofh_window_attention_workspace_bytes",
+    "ofh_window_attention_fwd",
+    "ofh_paged_params_init",
+    "ofh_paged_attention_workspace_bytes",
+    "ofh_paged_attention_fwd",
+    "ofh_cache_write_params_init",
+    "ofh_cache_write",
+    "ofh_cache_copy_pages",
+    "ofh_page_pool_create",
+    "ofh_page_pool_destroy",
+    "ofh_page_pool_add",
+    "ofh_page_pool_extend",
+    "ofh_page_pool_fork",
+    "ofh_page_pool_truncate",
+    "ofh_page_pool_free",
+    "ofh_page_pool_compact",
+    "ofh_page_pool_table",
+    "ofh_page_pool_length",
+    "ofh_page_pool_info",
     "ofh_last_error",
     "ofh_abi_version",
 )
@@ -140,6 +161,90 @@ class QkScoreParams(ctypes.Structure):
     ]
 
 
+class WindowParams(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("batch", ctypes.c_size_t),
+        ("heads", ctypes.c_size_t),
+        ("kv_heads", ctypes.c_size_t),
+        ("query_tokens", ctypes.c_size_t),
+        ("key_tokens", ctypes.c_size_t),
+        ("head_dim", ctypes.c_size_t),
+        ("value_dim", ctypes.c_size_t),
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("q_strides", ctypes.c_int64 * 3),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("o_strides", ctypes.c_int64 * 3),
+        ("scale", ctypes.c_float),
+        ("softcap", ctypes.c_float),
+        ("alibi_slopes", ctypes.c_void_p),
+        ("window", ctypes.c_size_t),
+        ("sink_tokens", ctypes.c_size_t),
+        ("query_offset", ctypes.c_size_t),
+        ("lengths", ctypes.c_void_p),
+        ("max_key_splits", ctypes.c_int32),
+    ]
+
+
+class _FlatWindowParams(ctypes.Structure):
+    _fields_ = _flat_fields(WindowParams._fields_)
+
+
+class PagedParams(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("batch", ctypes.c_size_t),
+        ("heads", ctypes.c_size_t),
+        ("kv_heads", ctypes.c_size_t),
+        ("query_tokens", ctypes.c_size_t),
+        ("head_dim", ctypes.c_size_t),
+        ("value_dim", ctypes.c_size_t),
+        ("num_pages", ctypes.c_size_t),
+        ("page_size", ctypes.c_size_t),
+        ("max_pages", ctypes.c_size_t),
+        ("table_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("q_strides", ctypes.c_int64 * 3),
+        ("o_strides", ctypes.c_int64 * 3),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("scale", ctypes.c_float),
+        ("softcap", ctypes.c_float),
+        ("alibi_slopes", ctypes.c_void_p),
+        ("window", ctypes.c_size_t),
+        ("sink_tokens", ctypes.c_size_t),
+        ("max_key_splits", ctypes.c_int32),
+    ]
+
+
+class CacheWriteParams(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("batch", ctypes.c_size_t),
+        ("kv_heads", ctypes.c_size_t),
+        ("tokens", ctypes.c_size_t),
+        ("head_dim", ctypes.c_size_t),
+        ("value_dim", ctypes.c_size_t),
+        ("num_pages", ctypes.c_size_t),
+        ("page_size", ctypes.c_size_t),
+        ("max_pages", ctypes.c_size_t),
+        ("table_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("k_strides", ctypes.c_int64 * 3),
+        ("v_strides", ctypes.c_int64 * 3),
+        ("k_page_strides", ctypes.c_int64 * 3),
+        ("v_page_strides", ctypes.c_int64 * 3),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+    ]
+
+
 class OfhError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"[ofh status {code}] {message}")
@@ -180,6 +285,31 @@ def lib() -> ctypes.CDLL:
         L.ofh_qk_score_params_init.restype = None
         L.ofh_qk_score_tile.argtypes = [QP] + [ctypes.c_void_p] * 4
         L.ofh_qk_score_tile.restype = ctypes.c_int
+        vp, sz, i64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int64
+        i32s, i64s, szs = ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(i64), ctypes.POINTER(sz)
+        for fn, result, args in (
+                ("ofh_window_params_init", None, [vp]),
+                ("ofh_window_attention_workspace_bytes", ctypes.c_int, [vp, szs]),
+                ("ofh_window_attention_fwd", ctypes.c_int, [vp] * 6 + [sz, vp]),
+                ("ofh_paged_params_init", None, [vp]),
+                ("ofh_paged_attention_workspace_bytes", ctypes.c_int, [vp, szs]),
+                ("ofh_paged_attention_fwd", ctypes.c_int, [vp] * 6 + [sz, vp]),
+                ("ofh_cache_write_params_init", None, [vp]),
+                ("ofh_cache_write", ctypes.c_int, [vp] * 6),
+                ("ofh_cache_copy_pages", ctypes.c_int, [vp, sz, sz, sz, sz, vp, vp, sz, vp]),
+                ("ofh_page_pool_create", ctypes.c_int, [sz, sz, ctypes.POINTER(vp)]),
+                ("ofh_page_pool_destroy", ctypes.c_int, [vp]),
+                ("ofh_page_pool_add", ctypes.c_int, [vp, i64s]),
+                ("ofh_page_pool_extend", ctypes.c_int, [vp, i64s, szs, sz, i32s, i32s, szs]),
+                ("ofh_page_pool_fork", ctypes.c_int, [vp, i64, i64s]),
+                ("ofh_page_pool_truncate", ctypes.c_int, [vp, i64, sz]),
+                ("ofh_page_pool_free", ctypes.c_int, [vp, i64]),
+                ("ofh_page_pool_compact", ctypes.c_int, [vp, i32s, i32s, sz, szs]),
+                ("ofh_page_pool_table", ctypes.c_int, [vp, i64s, sz, i32s, sz, i32s]),
+                ("ofh_page_pool_length", ctypes.c_int, [vp, i64, szs]),
+                ("ofh_page_pool_info", ctypes.c_int, [vp, szs, szs])):
+            getattr(L, fn).restype = result
+            getattr(L, fn).argtypes = args
         L.ofh_last_error.restype = ctypes.c_char_p
         L.ofh_last_error.argtypes = []
         L.ofh_abi_version.restype = ctypes.c_int
@@ -466,6 +596,372 @@ def qk_score_tile(q, k, *, scale: float | None = None, bias=None, softcap: float
     check(lib().ofh_qk_score_tile(ctypes.byref(p), q.data_ptr(), k.data_ptr(), out.data_ptr(),
                                   stream))
     return out
+
+
+# ---------------------------------------------------------------------------
+# Serving: windowed attention of prompts, attention over a paged key-value
+# cache, writing and copying of its pages. onednn_flash_cache.PagedCache keeps
+# such a cache.
+
+def _launch_on(torch, device, stream, call):
+    """call(stream handle) with `device` current: the library launches on the
+    current device."""
+    if stream is None:
+        stream = _raw_stream(torch, device)
+    if device.index is None or device.index == torch.cuda.current_device():
+        rc = call(stream)
+    else:
+        with torch.cuda.device(device):
+            rc = call(stream)
+    if rc != OFH_SUCCESS:
+        check(rc)
+
+
+def _check_rows(torch, name, t, dims, dtype, device):
+    """t is a tensor of `dims` dimensions with contiguous rows (None: any dtype or device)."""
+    if not isinstance(t, torch.Tensor) or t.dim() != dims:
+        raise ValueError(f"{name} must be a rank-{dims} tensor")
+    if t.dtype not in _DTYPE_CODES:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}")
+    if 0 in t.shape:
+        raise ValueError(f"{name} must not be empty")
+    if (t.shape[-1] > 1 and t.stride(-1) != 1) or min(t.stride()) < 0:
+        raise ValueError(f"{name}: last axis must be contiguous and strides non-negative")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be a GPU tensor")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} must be on {device}")
+
+
+def _axis_strides(name, t):
+    """The strides of t's first three axes as the C ABI takes them: those of axes of
+    one element, which torch leaves open, as a row's length, and never all zero
+    (which would mean a contiguous tensor)."""
+    row = t.shape[3]
+    a, b, c = [stride if size > 1 else row for size, stride in zip(t.shape[:3], t.stride())]
+    if a == 0 and b == 0 and c == 0:
+        raise ValueError(f"{name} must not be one row broadcast over every axis")
+    return a, b, c
+
+
+def _check_written(name, t):
+    """No two elements of t may share memory: it is written."""
+    for size, stride in zip(t.shape, t.stride()):
+        if size > 1 and stride == 0:
+            raise ValueError(f"{name} must not be a broadcast tensor")
+
+
+def _check_ints(torch, name, t, shape, device):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be an int32 tensor of shape {shape}")
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        raise ValueError(f"{name}: last axis must be contiguous")
+    if t.device != device:
+        raise ValueError(f"{name} must be on {device}")
+
+
+def _check_slopes(torch, slopes, heads, device):
+    if not isinstance(slopes, torch.Tensor) or slopes.dtype != torch.float32 or tuple(slopes.shape) != (heads,) \
+            or not slopes.is_contiguous():
+        raise ValueError("alibi_slopes must be a contiguous float32 tensor of length H")
+    if slopes.device != device:
+        raise ValueError(f"alibi_slopes must be on {device}")
+
+
+def _check_counts(**values):
+    for name, x in values.items():
+        if isinstance(x, bool) or not isinstance(x, int) or x < 0:
+            raise ValueError(f"{name} must be a non-negative integer")
+
+
+def _check_out(torch, out, shape, dtype, device):
+    _check_rows(torch, "out", out, 4, None, device)
+    if tuple(out.shape) != shape:
+        raise ValueError(f"out must have shape {shape}")
+    if out.dtype not in (dtype, torch.float32):
+        raise ValueError("out must have the dtype of q or float32")
+    _check_written("out", out)
+
+
+def _scratch(torch, need, workspace, device):
+    """(address, bytes) of the workspace, and the tensor that holds it."""
+    if workspace is None:
+        if need == 0:
+            return None, 0, None
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.device != device:
+        raise ValueError(f"workspace must be a contiguous uint8 tensor on {device}")
+    return workspace.data_ptr(), workspace.numel(), workspace
+
+
+def _workspace_need(query, p) -> int:
+    need = ctypes.c_size_t()
+    rc = query(ctypes.addressof(p), ctypes.byref(need))
+    if rc != OFH_SUCCESS:
+        check(rc)
+    return need.value
+
+
+def window_attention(q, k, v, *, window: int = 0, sink_tokens: int = 0, scale: float | None = None,
+                     query_offset: int = 0, lengths=None, alibi_slopes=None, softcap: float = 0.0, out=None,
+                     out_dtype=None, workspace=None, stream=None, max_key_splits: int = 0):
+    """Causal attention of prompts with a sliding window and first tokens that
+    stay visible. q: [B,H,M,D], k: [B,Hkv,N,D], v: [B,Hkv,N,Dv] device tensors,
+    H a multiple of Hkv (query head h reads key-value head h / (H / Hkv)).
+
+    Query row i is at position p = query_offset + i and sees key j iff j <= p
+    and p - j < window (any, with window 0) or j < sink_tokens. lengths: int32
+    device [B], the tokens of each sequence of a padded batch: keys from there
+    on are not seen, query rows at those positions are written as 0. scale
+    defaults to 1 / sqrt(D); alibi_slopes: f32 device [H]. Rows that see nothing
+    are 0. Returns out, [B,H,M,Dv].
+
+    The workspace (partial rows of calls with few query rows) is taken from
+    torch's allocator unless given."""
+    torch = _torch()
+    _check_rows(torch, "q", q, 4, None, None)
+    dev = q.device
+    _check_rows(torch, "k", k, 4, q.dtype, dev)
+    _check_rows(torch, "v", v, 4, q.dtype, dev)
+    B, H, M, D = q.shape
+    Hkv, N, Dv = k.shape[1], k.shape[2], v.shape[3]
+    if k.shape[0] != B or k.shape[3] != D or v.shape[:3] != k.shape[:3] or H % Hkv != 0:
+        raise ValueError("k must be [B, Hkv, N, D] and v [B, Hkv, N, Dv] with H a multiple of Hkv")
+    _check_counts(window=window, sink_tokens=sink_tokens, query_offset=query_offset, max_key_splits=max_key_splits)
+    if lengths is not None:
+        _check_ints(torch, "lengths", lengths, (B,), dev)
+    if alibi_slopes is not None:
+        _check_slopes(torch, alibi_slopes, H, dev)
+    if out is None:
+        if out_dtype not in (None, q.dtype, torch.float32):
+            raise ValueError("out_dtype must be the dtype of q or float32")
+        out = torch.empty((B, H, M, Dv), dtype=q.dtype if out_dtype is None else out_dtype, device=dev)
+    else:
+        _check_out(torch, out, (B, H, M, Dv), q.dtype, dev)
+        if out_dtype is not None and out.dtype != out_dtype:
+            raise ValueError("out and out_dtype disagree")
+    p = _FlatWindowParams(
+        ctypes.sizeof(WindowParams), B, H, Hkv, M, N, D, Dv, _DTYPE_CODES[q.dtype], _DTYPE_CODES[out.dtype],
+        *_axis_strides("q", q), *_axis_strides("k", k), *_axis_strides("v", v), *_axis_strides("out", out),
+        (1.0 / math.sqrt(D)) if scale is None else scale, softcap,
+        None if alibi_slopes is None else alibi_slopes.data_ptr(), window, sink_tokens, query_offset,
+        None if lengths is None else lengths.data_ptr(), max_key_splits)
+    L = lib()
+    need = _workspace_need(L.ofh_window_attention_workspace_bytes, p) if workspace is None else 0
+    ws, ws_bytes, _held = _scratch(torch, need, workspace, dev)
+    _launch_on(torch, dev, stream, lambda s: L.ofh_window_attention_fwd(
+        ctypes.addressof(p), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ws, ws_bytes, s))
+    return out
+
+
+def _check_pool(torch, k_pages, v_pages, page_table, lengths, batch=None):
+    """The tensors of a paged cache: k_pages [P,Hkv,S,D], v_pages [P,Hkv,S,Dv],
+    page_table [B,max_pages] and lengths [B]. Returns the batch."""
+    _check_rows(torch, "k_pages", k_pages, 4, None, None)
+    dev = k_pages.device
+    _check_rows(torch, "v_pages", v_pages, 4, k_pages.dtype, dev)
+    if v_pages.shape[:3] != k_pages.shape[:3]:
+        raise ValueError("k_pages must be [P, Hkv, S, D] and v_pages [P, Hkv, S, Dv]")
+    if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2 or 0 in page_table.shape:
+        raise ValueError("page_table must be an int32 tensor [B, max_pages]")
+    _check_ints(torch, "page_table", page_table, tuple(page_table.shape), dev)
+    _check_ints(torch, "lengths", lengths, (page_table.shape[0],), dev)
+
+
+class PagedAttention:
+    """Attention of new tokens over a paged key-value cache, for a program that
+    keeps the cache's tensors and calls it step after step: their checks are made
+    once, here, and each call reads what they hold then.
+
+    k_pages: [P,Hkv,S,D], v_pages: [P,Hkv,S,Dv] (S a power of two, 16 or more);
+    page_table: int32 [B,max_pages], key j of sequence b being row j % S of page
+    page_table[b, j // S]; lengths: int32 [B], the tokens of each sequence with
+    the query_tokens new ones, whose keys are in the cache by then (cache_write).
+    Token t of a sequence is at position lengths[b] - query_tokens + t and sees
+    what window_attention lets it see. Entries of keys that no token sees are
+    not read; the keys of an entry outside the pool are not seen."""
+
+    def __init__(self, k_pages, v_pages, page_table, lengths, *, heads: int, query_tokens: int = 1, window: int = 0,
+                 sink_tokens: int = 0, scale: float | None = None, alibi_slopes=None, softcap: float = 0.0,
+                 out_dtype=None, max_key_splits: int = 0):
+        torch = _torch()
+        _check_pool(torch, k_pages, v_pages, page_table, lengths)
+        _check_counts(heads=heads, query_tokens=query_tokens, window=window, sink_tokens=sink_tokens,
+                      max_key_splits=max_key_splits)
+        P, Hkv, S, D = k_pages.shape
+        B, max_pages = page_table.shape
+        Dv = v_pages.shape[3]
+        if heads == 0 or heads % Hkv != 0 or query_tokens == 0:
+            raise ValueError("heads must be a positive multiple of the cache's heads, query_tokens positive")
+        if alibi_slopes is not None:
+            _check_slopes(torch, alibi_slopes, heads, k_pages.device)
+        if out_dtype not in (None, k_pages.dtype, torch.float32):
+            raise ValueError("out_dtype must be the dtype of the cache or float32")
+        self._torch = torch
+        self._held = (k_pages, v_pages, page_table, lengths, alibi_slopes)
+        self._device, self._dtype = k_pages.device, k_pages.dtype
+        self._out_dtype = k_pages.dtype if out_dtype is None else out_dtype
+        self._q_shape, self._out_shape = (B, heads, query_tokens, D), (B, heads, query_tokens, Dv)
+        p = PagedParams()
+        L = lib()
+        L.ofh_paged_params_init(ctypes.addressof(p))
+        p.batch, p.heads, p.kv_heads, p.query_tokens, p.head_dim, p.value_dim = B, heads, Hkv, query_tokens, D, Dv
+        p.num_pages, p.page_size, p.max_pages, p.table_stride = P, S, max_pages, page_table.stride(0) if B > 1 else 0
+        p.dtype = _DTYPE_CODES[self._dtype]
+        p.k_strides[:], p.v_strides[:] = _axis_strides("k_pages", k_pages), _axis_strides("v_pages", v_pages)
+        p.page_table, p.lengths = page_table.data_ptr(), lengths.data_ptr()
+        p.scale = (1.0 / math.sqrt(D)) if scale is None else scale
+        p.softcap = softcap
+        if alibi_slopes is not None:
+            p.alibi_slopes = alibi_slopes.data_ptr()
+        p.window, p.sink_tokens, p.max_key_splits = window, sink_tokens, max_key_splits
+        p.out_dtype = _DTYPE_CODES[self._out_dtype]
+        self._params = bytes(p)
+        self._need = _workspace_need(L.ofh_paged_attention_workspace_bytes, p)
+        self._fwd = L.ofh_paged_attention_fwd
+        self._ptrs = (k_pages.data_ptr(), v_pages.data_ptr())
+
+    @property
+    def workspace_bytes(self) -> int:
+        return self._need
+
+    def __call__(self, q, *, out=None, workspace=None, stream=None):
+        """q: [B,H,T,D] in the cache's dtype. Returns out, [B,H,T,Dv]."""
+        torch, dev = self._torch, self._device
+        if not (isinstance(q, torch.Tensor) and tuple(q.shape) == self._q_shape and q.dtype == self._dtype
+                and q.device == dev):
+            raise ValueError(f"q must be a {self._dtype} tensor of shape {self._q_shape} on {dev}")
+        qs = q.stride()
+        if (qs[3] != 1 and q.shape[3] > 1) or min(qs) < 0:
+            raise ValueError("q: last axis must be contiguous and strides non-negative")
+        p = PagedParams.from_buffer_copy(self._params)  # (its own: calls may run on several threads)
+        p.q_strides[:] = _axis_strides("q", q)
+        if out is None:
+            out = torch.empty(self._out_shape, dtype=self._out_dtype, device=dev)
+        else:
+            _check_out(torch, out, self._out_shape, self._dtype, dev)
+            p.out_dtype = _DTYPE_CODES[out.dtype]
+            p.o_strides[:] = _axis_strides("out", out)
+        ws, ws_bytes, _held = _scratch(torch, self._need, workspace, dev)
+        _launch_on(torch, dev, stream, lambda s: self._fwd(
+            ctypes.addressof(p), q.data_ptr(), *self._ptrs, out.data_ptr(), ws, ws_bytes, s))
+        return out
+
+
+def paged_attention(q, k_pages, v_pages, page_table, lengths, *, window: int = 0, sink_tokens: int = 0,
+                    scale: float | None = None, alibi_slopes=None, softcap: float = 0.0, out=None, out_dtype=None,
+                    workspace=None, stream=None, max_key_splits: int = 0):
+    """One call of PagedAttention: q [B,H,T,D], the T new tokens of each sequence."""
+    if q.dim() != 4:
+        raise ValueError("q must be a rank-4 tensor")
+    if out is not None and out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError("out and out_dtype disagree")
+    return PagedAttention(k_pages, v_pages, page_table, lengths, heads=q.shape[1], query_tokens=q.shape[2],
+                          window=window, sink_tokens=sink_tokens, scale=scale, alibi_slopes=alibi_slopes,
+                          softcap=softcap, out_dtype=out_dtype, max_key_splits=max_key_splits)(
+                              q, out=out, workspace=workspace, stream=stream)
+
+
+class CacheWriter:
+    """Writes new keys and values into the pages of a cache, for a program that
+    keeps the cache's tensors (as PagedAttention). Token t < counts[b] of
+    sequence b (every token without counts) goes to position lengths[b] -
+    counts[b] + t; tokens without a place in the table or the pool are not
+    written. Sequences that share a page must not write the same place of it
+    (PagedCache.extend gives each its own)."""
+
+    def __init__(self, k_pages, v_pages, page_table, lengths, *, counts=None):
+        torch = _torch()
+        _check_pool(torch, k_pages, v_pages, page_table, lengths)
+        _check_written("k_pages", k_pages)
+        _check_written("v_pages", v_pages)
+        P, Hkv, S, D = k_pages.shape
+        B, max_pages = page_table.shape
+        if counts is not None:
+            _check_ints(torch, "counts", counts, (B,), k_pages.device)
+        self._torch = torch
+        self._held = (k_pages, v_pages, page_table, lengths, counts)
+        self._device, self._dtype = k_pages.device, k_pages.dtype
+        self._row = (B, Hkv, D, v_pages.shape[3])
+        p = CacheWriteParams()
+        L = lib()
+        L.ofh_cache_write_params_init(ctypes.addressof(p))
+        p.batch, p.kv_heads, p.head_dim, p.value_dim = B, Hkv, D, v_pages.shape[3]
+        p.num_pages, p.page_size, p.max_pages, p.table_stride = P, S, max_pages, page_table.stride(0) if B > 1 else 0
+        p.dtype = _DTYPE_CODES[self._dtype]
+        p.k_page_strides[:] = _axis_strides("k_pages", k_pages)
+        p.v_page_strides[:] = _axis_strides("v_pages", v_pages)
+        p.page_table, p.lengths = page_table.data_ptr(), lengths.data_ptr()
+        if counts is not None:
+            p.counts = counts.data_ptr()
+        self._params = bytes(p)
+        self._write = L.ofh_cache_write
+        self._ptrs = (k_pages.data_ptr(), v_pages.data_ptr())
+
+    def __call__(self, k, v, *, stream=None) -> None:
+        """k: [B,Hkv,T,D], v: [B,Hkv,T,Dv], the (padded) new rows."""
+        torch, dev = self._torch, self._device
+        B, Hkv, D, Dv = self._row
+        _check_rows(torch, "k", k, 4, self._dtype, dev)
+        _check_rows(torch, "v", v, 4, self._dtype, dev)
+        T = k.shape[2]
+        if tuple(k.shape) != (B, Hkv, T, D) or tuple(v.shape) != (B, Hkv, T, Dv):
+            raise ValueError(f"k must be {(B, Hkv, 'T', D)} and v {(B, Hkv, 'T', Dv)}")
+        p = CacheWriteParams.from_buffer_copy(self._params)
+        p.tokens = T
+        p.k_strides[:], p.v_strides[:] = _axis_strides("k", k), _axis_strides("v", v)
+        _launch_on(torch, dev, stream, lambda s: self._write(
+            ctypes.addressof(p), k.data_ptr(), v.data_ptr(), *self._ptrs, s))
+
+
+def cache_write(k, v, k_pages, v_pages, page_table, lengths, *, counts=None, stream=None) -> None:
+    """One call of CacheWriter."""
+    CacheWriter(k_pages, v_pages, page_table, lengths, counts=counts)(k, v, stream=stream)
+
+
+def copy_pages(pools, src, dst, *, stream=None) -> None:
+    """Copies pages src[i] -> dst[i] of every pool. pools: device tensors
+    [P, ...] of one shape and dtype whose pages are contiguous; src, dst: page
+    numbers on the host (int32 CPU tensors, or sequences of integers), read
+    before the call returns. Raises for pages outside the pools, a page twice in
+    dst, or a page in both src and dst."""
+    torch = _torch()
+    pools = list(pools)
+    if not pools or not all(isinstance(t, torch.Tensor) for t in pools):
+        raise ValueError("pools must be tensors [P, ...]")
+    first = pools[0]
+    dev = first.device
+    if first.dim() < 2 or first.numel() == 0 or dev.type != "cuda":
+        raise ValueError("pools must be GPU tensors [P, ...]")
+    for t in pools:
+        if t.shape != first.shape or t.dtype != first.dtype or t.device != dev or t.stride() != first.stride():
+            raise ValueError("pools must share shape, dtype, strides and device")
+    if not first[0].is_contiguous():
+        raise ValueError("pools: pages must be contiguous")
+    size = first.element_size()
+    page = first[0].numel() * size
+    stride = first.stride(0) * size if first.shape[0] > 1 else page
+    if stride < page:
+        raise ValueError("pools: pages must not overlap")
+
+    def numbers(name, x):
+        x = torch.as_tensor(x) if isinstance(x, torch.Tensor) else torch.tensor(list(x), dtype=torch.int64)
+        if x.dim() != 1 or x.device.type != "cpu" or x.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{name} must be a row of integers on the host")
+        if x.dtype != torch.int32:
+            if x.numel() and (int(x.min()) < 0 or int(x.max()) >= first.shape[0]):
+                raise ValueError(f"{name}: copied pages must be within the pool")
+            x = x.to(torch.int32)
+        return x.contiguous()
+
+    src, dst = numbers("src", src), numbers("dst", dst)
+    if src.numel() != dst.numel():
+        raise ValueError("src and dst must have the same length")
+    addresses = (ctypes.c_void_p * len(pools))(*(t.data_ptr() for t in pools))
+    _launch_on(torch, dev, stream, lambda s: lib().ofh_cache_copy_pages(
+        addresses, len(pools), first.shape[0], page, stride, src.data_ptr(), dst.data_ptr(), src.numel(), s))
 
 
 # Tile heuristic and layout choice of the reference wrapper

@@ -46,7 +46,8 @@ typedef enum ofh_status {
     OFH_ERROR_INVALID_ARGUMENT = 1,
     OFH_ERROR_UNSUPPORTED = 2,
     OFH_ERROR_HIP = 3,
-    OFH_ERROR_WORKSPACE_TOO_SMALL = 4
+    OFH_ERROR_WORKSPACE_TOO_SMALL = 4,
+    OFH_ERROR_OUT_OF_PAGES = 5 /* ofh_page_pool_extend: the pool has too few free pages */
 } ofh_status;
 
 /* Element type of Q, K, V and O in device memory. */
@@ -273,6 +274,155 @@ void ofh_qk_score_params_init(ofh_qk_score_params* p);
  * (qk_score_tile.cpp:16-26). */
 int ofh_qk_score_tile(const ofh_qk_score_params* p, const void* q, const void* k, float* score,
                       void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Serving: windowed attention of prompts, attention over a paged key-value
+ * cache, and what keeps such a cache. No counterparts in the reference.
+ *
+ * Both attentions share one rule. Query head h reads key-value head
+ * h / (heads / kv_heads). A query at position p of a sequence of `length` keys
+ * sees key j iff
+ *     j < length, j <= p, and (window == 0 or p - j < window or j < sink_tokens).
+ * A seen score is s = scale q.k, plus alibi_slopes[h] (j - p) when slopes are
+ * given, then softcap tanh(s / softcap) when softcap > 0; the row is
+ * softmax(s) V over the seen keys, 0 when there are none. Keys that a row does
+ * not see do not reach it, whatever their K and V hold (NaN and infinities
+ * too). Sums and the softmax are fp32; probabilities are rounded to the input
+ * type for their product with V.
+ *
+ * fp32, bf16 and fp16; head_dim and value_dim up to 256, multiples of 8 (16
+ * bits) or 4 (fp32); pointers 16-byte aligned and every stride a multiple of
+ * 16 bytes. Strides are in elements, the last axis is contiguous. Calls are
+ * ordered on `stream` and compute on the current device. Outputs do not
+ * overlap inputs. Everything else is refused with a status before any launch.
+ */
+
+typedef struct ofh_window_params {
+    uint32_t struct_size; /* set by ofh_window_params_init */
+    size_t batch, heads, kv_heads, query_tokens, key_tokens, head_dim, value_dim;
+    int32_t dtype;        /* ofh_dtype of q, k and v */
+    int32_t out_dtype;    /* the input type or OFH_DTYPE_F32 */
+    /* Batch, head and token strides of Q[B,H,M,D], K[B,Hkv,N,D], V[B,Hkv,N,Dv]
+     * and O[B,H,M,Dv]; all zero: contiguous. */
+    int64_t q_strides[3], k_strides[3], v_strides[3], o_strides[3];
+    float scale;          /* default 1.0 */
+    float softcap;        /* 0: off */
+    const float* alibi_slopes; /* device [heads] or NULL */
+    size_t window;        /* keys that a query sees, itself included; 0: all before it */
+    size_t sink_tokens;   /* first keys that stay visible behind a window */
+    size_t query_offset;  /* position of query row 0 */
+    /* Device int32 [B] or NULL. lengths[b] (taken between 0 and key_tokens) is
+     * what sequence b of a padded batch has: keys from there on are not seen,
+     * and query rows at those positions are padding, written as 0. */
+    const int32_t* lengths;
+    int32_t max_key_splits; /* 0: the library chooses, 1: never split, n: at most n */
+} ofh_window_params;
+
+/* Defaults: fp32, scale 1, everything else zero. */
+void ofh_window_params_init(ofh_window_params* p);
+
+/* Scratch of a call: partial rows where few query rows share many keys, whose
+ * range is then split over workgroups. */
+int ofh_window_attention_workspace_bytes(const ofh_window_params* p, size_t* bytes);
+
+/* workspace NULL: the library's scratch of the stream (as ofh_attention_fwd;
+ * under graph capture a split that does not fit it is dropped). */
+int ofh_window_attention_fwd(const ofh_window_params* p, const void* q, const void* k, const void* v, void* out,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* Pages. A pool holds num_pages pages of page_size tokens (a power of two, 16
+ * or more): K [page, kv_head, token, head_dim] and V [.., value_dim] under any
+ * strides. Row b of the page table lists the pages of sequence b: key j is row
+ * j mod page_size of page table[b][j / page_size]. */
+typedef struct ofh_paged_params {
+    uint32_t struct_size; /* set by ofh_paged_params_init */
+    size_t batch, heads, kv_heads, query_tokens, head_dim, value_dim;
+    size_t num_pages, page_size;
+    size_t max_pages;     /* entries of a page table row */
+    int64_t table_stride; /* entries between rows; 0: max_pages */
+    int32_t dtype, out_dtype;
+    int64_t q_strides[3], o_strides[3]; /* batch, head, token; all zero: contiguous Q[B,H,T,D], O[B,H,T,Dv] */
+    int64_t k_strides[3], v_strides[3]; /* page, head, token; all zero: contiguous */
+    const int32_t* page_table; /* device */
+    /* Device [B]: tokens of each sequence, the new ones included (taken between
+     * 0 and max_pages page_size). Token t is at position lengths[b] -
+     * query_tokens + t; before the first position there is nothing to see. */
+    const int32_t* lengths;
+    float scale, softcap;
+    const float* alibi_slopes;
+    size_t window, sink_tokens;
+    int32_t max_key_splits;
+} ofh_paged_params;
+
+void ofh_paged_params_init(ofh_paged_params* p);
+int ofh_paged_attention_workspace_bytes(const ofh_paged_params* p, size_t* bytes);
+
+/* Table entries are read for the keys below lengths[b] that some row of the
+ * sequence sees; the keys of an entry outside [0, num_pages) are not seen. */
+int ofh_paged_attention_fwd(const ofh_paged_params* p, const void* q, const void* k_pages, const void* v_pages,
+                            void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* New rows into the pages: token t < counts[b] of sequence b goes to position
+ * lengths[b] - counts[b] + t. K[B,Hkv,T,D] and V[B,Hkv,T,Dv] of any alignment.
+ * Tokens whose position is negative or past the table's row, or whose page is
+ * outside the pool, are not written. Two tokens of one call that share a place
+ * (sequences that share a page past their common tokens) leave either. */
+typedef struct ofh_cache_write_params {
+    uint32_t struct_size; /* set by ofh_cache_write_params_init */
+    size_t batch, kv_heads, tokens, head_dim, value_dim;
+    size_t num_pages, page_size, max_pages;
+    int64_t table_stride;
+    int32_t dtype;
+    int64_t k_strides[3], v_strides[3];           /* batch, head, token; all zero: contiguous */
+    int64_t k_page_strides[3], v_page_strides[3]; /* page, head, token; all zero: contiguous */
+    const int32_t* page_table;
+    const int32_t* lengths; /* device [B], the new tokens included */
+    const int32_t* counts;  /* device [B], taken between 0 and tokens, or NULL: tokens */
+} ofh_cache_write_params;
+
+void ofh_cache_write_params_init(ofh_cache_write_params* p);
+int ofh_cache_write(const ofh_cache_write_params* p, const void* k, const void* v, void* k_pages, void* v_pages,
+                    void* stream);
+
+/* Copies pages src[i] -> dst[i] of every pool. A page is page_bytes contiguous
+ * bytes, page_stride_bytes from the next (0: page_bytes). `pools`, src and dst
+ * are host arrays, read before the call returns. Refused: pages outside
+ * [0, num_pages), a page twice in dst, or a page in both src and dst (its
+ * copies would have no order). */
+int ofh_cache_copy_pages(void* const* pools, size_t num_pools, size_t num_pages, size_t page_bytes,
+                         size_t page_stride_bytes, const int32_t* src, const int32_t* dst, size_t count,
+                         void* stream);
+
+/* Which sequence holds which pages: host bookkeeping, no device work. Pages
+ * are handed out lowest first and counted: a fork shares its parent's pages,
+ * and a shared page that is to be written is replaced by a copy. Every call
+ * either does all it says or nothing; calls on one pool from several threads
+ * are safe. Errors: INVALID_ARGUMENT for unknown sequences. */
+typedef struct ofh_page_pool ofh_page_pool;
+
+int ofh_page_pool_create(size_t num_pages, size_t page_size, ofh_page_pool** pool);
+int ofh_page_pool_destroy(ofh_page_pool* pool); /* NULL: nothing */
+/* A new sequence without tokens. */
+int ofh_page_pool_add(ofh_page_pool* pool, int64_t* sequence);
+/* Room for tokens[i] more tokens in sequences[i] (each sequence once). Where
+ * a partly filled last page is shared, (copy_src, copy_dst) get the pair to copy
+ * before the new tokens are written: at most `count` pairs. */
+int ofh_page_pool_extend(ofh_page_pool* pool, const int64_t* sequences, const size_t* tokens, size_t count,
+                         int32_t* copy_src, int32_t* copy_dst, size_t* copies);
+/* A new sequence with the same tokens. */
+int ofh_page_pool_fork(ofh_page_pool* pool, int64_t sequence, int64_t* child);
+/* Drops the tokens from `length` on (at most what the sequence has). */
+int ofh_page_pool_truncate(ofh_page_pool* pool, int64_t sequence, size_t length);
+int ofh_page_pool_free(ofh_page_pool* pool, int64_t sequence);
+/* Moves used pages to the lowest numbers, at most `capacity` of them, and
+ * returns what to copy; no page is in both copy_src and copy_dst. */
+int ofh_page_pool_compact(ofh_page_pool* pool, int32_t* copy_src, int32_t* copy_dst, size_t capacity,
+                          size_t* copies);
+/* Page table rows of max_pages entries (the rest -1) and lengths. */
+int ofh_page_pool_table(ofh_page_pool* pool, const int64_t* sequences, size_t count, int32_t* table,
+                        size_t max_pages, int32_t* lengths);
+int ofh_page_pool_length(ofh_page_pool* pool, int64_t sequence, size_t* length);
+int ofh_page_pool_info(ofh_page_pool* pool, size_t* pages_in_use, size_t* sequences);
 
 /* Thread-local text of the last error on this thread ("" if none). */
 const char* ofh_last_error(void);
