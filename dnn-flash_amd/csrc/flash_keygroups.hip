@@ -39,10 +39,7 @@ __global__ __launch_bounds__(kGroupThreads, 1) void flash_fwd_keygroups_kernel(F
     constexpr int R = 8 / KS;
     using W = Wave32<T, D, MOD, false, kGroupThreads, BN, KS>;
     using L = typename W::L;
-    constexpr int NDB = D / 32;
-    constexpr int kStateFloats = NDB * 16 + 4;        // O, m, l of a lane (padded to 16 bytes)
-    constexpr int kStateBytes = 64 * 4 * kStateFloats;
-    static_assert((8 - R) * kStateBytes <= 2 * L::STAGE, "the folded states fit the LDS stages");
+    static_assert((8 - R) * group_state_bytes(D) <= 2 * L::STAGE, "the folded states fit the LDS stages");
     __shared__ __attribute__((aligned(16))) unsigned char smem[2 * L::STAGE];
     int bh, qt;
     map_work((int)blockIdx.x, a.B * a.H, a.num_q_tiles, a.causal, bh, qt);
@@ -75,49 +72,8 @@ __global__ __launch_bounds__(kGroupThreads, 1) void flash_fwd_keygroups_kernel(F
         __syncthreads();
     }
 
-    // Fold the states of the slice's wavefronts into key group 0's.
-    const int lane = threadIdx.x & 63;
-    if (kg > 0) {
-        float* st = (float*)(smem + (wave - R) * kStateBytes);
-#pragma unroll
-        for (int db = 0; db < NDB; ++db)
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-                *(f32x4*)(st + 4 * (64 * (4 * db + c) + lane)) =
-                    f32x4{w.o[db][4 * c], w.o[db][4 * c + 1], w.o[db][4 * c + 2], w.o[db][4 * c + 3]};
-        *(f32x4*)(st + 4 * (64 * 4 * NDB + lane)) = f32x4{w.m_run, w.l_run, 0.f, 0.f};
-    }
-    __syncthreads();
-    if (kg == 0) {
-        f32x4 ml[KS];
-        float mg = w.m_run;
-#pragma unroll
-        for (int k = 1; k < KS; ++k) {
-            ml[k] = *(const f32x4*)(smem + ((k - 1) * R + slice) * kStateBytes + 16 * (64 * 4 * NDB + lane));
-            mg = fmaxf(mg, ml[k][0]);
-        }
-        const float mu = mg == kNegInf ? 0.0f : mg;
-        const float w0 = __builtin_amdgcn_exp2f(w.m_run - mu);  // 0 for a group without a valid key
-        w.l_run *= w0;
-        w.m_run = mg;
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) w.o[db] *= w0;
-#pragma unroll
-        for (int k = 1; k < KS; ++k) {
-            const float wk = __builtin_amdgcn_exp2f(ml[k][0] - mu);
-            w.l_run += wk * ml[k][1];
-            const unsigned char* st = smem + ((k - 1) * R + slice) * kStateBytes;
-#pragma unroll
-            for (int db = 0; db < NDB; ++db)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const f32x4 v = *(const f32x4*)(st + 16 * (64 * (4 * db + c) + lane));
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) w.o[db][4 * c + j] += wk * v[j];
-                }
-        }
-        w.store_output();
-    }
+    fold_groups<W, KS>(w, smem, wave, slice, kg);
+    if (kg == 0) w.store_output();
 }
 
 template <typename T, int D, int MOD>

@@ -869,6 +869,57 @@ struct Wave32 {
     }
 };
 
+// Wavefronts that share a slice of 32 rows and split its keys: the (m, l, O) of
+// key groups 1 .. KS - 1 are folded into group 0's through LDS (wavefront =
+// slice + R kg, R slices).
+constexpr int group_state_bytes(int D) { return 64 * 4 * (D / 32 * 16 + 4); }  // O, m, l of a lane (padded to 16 bytes)
+template <typename W, int KS, int R = 8 / KS>
+__device__ __forceinline__ void fold_groups(W& w, unsigned char* smem, int wave, int slice, int kg) {
+    constexpr int NDB = sizeof(w.o) / sizeof(w.o[0]);
+    constexpr int kStateBytes = group_state_bytes(32 * NDB);
+    const int lane = threadIdx.x & 63;
+    if (kg > 0) {
+        float* st = (float*)(smem + (wave - R) * kStateBytes);
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                *(f32x4*)(st + 4 * (64 * (4 * db + c) + lane)) =
+                    f32x4{w.o[db][4 * c], w.o[db][4 * c + 1], w.o[db][4 * c + 2], w.o[db][4 * c + 3]};
+        *(f32x4*)(st + 4 * (64 * 4 * NDB + lane)) = f32x4{w.m_run, w.l_run, 0.f, 0.f};
+    }
+    __syncthreads();
+    if (kg == 0) {
+        f32x4 ml[KS];
+        float mg = w.m_run;
+#pragma unroll
+        for (int k = 1; k < KS; ++k) {
+            ml[k] = *(const f32x4*)(smem + ((k - 1) * R + slice) * kStateBytes + 16 * (64 * 4 * NDB + lane));
+            mg = fmaxf(mg, ml[k][0]);
+        }
+        const float mu = mg == kNegInf ? 0.0f : mg;
+        const float w0 = __builtin_amdgcn_exp2f(w.m_run - mu);  // 0 for a group without a valid key
+        w.l_run *= w0;
+        w.m_run = mg;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) w.o[db] *= w0;
+#pragma unroll
+        for (int k = 1; k < KS; ++k) {
+            const float wk = __builtin_amdgcn_exp2f(ml[k][0] - mu);
+            w.l_run += wk * ml[k][1];
+            const unsigned char* st = smem + ((k - 1) * R + slice) * kStateBytes;
+#pragma unroll
+            for (int db = 0; db < NDB; ++db)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const f32x4 v = *(const f32x4*)(st + 16 * (64 * (4 * db + c) + lane));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w.o[db][4 * c + j] += wk * v[j];
+                }
+        }
+    }
+}
+
 // End of a query tile (or of its key split `split` of `active`): O, or the
 // partial rows followed by the merge in the split workgroup that arrives last.
 template <typename W, int NTHREADS, bool SPLIT>

@@ -182,7 +182,8 @@ int window_args(const ofh_window_params* p, bool check_ptrs, const void* q, cons
                               p->out_dtype, p->scale, p->softcap, p->window, p->sink_tokens, p->max_key_splits))
         return rc;
     if (p->key_tokens == 0) return invalid("attention dimensions must be non-zero");
-    if (p->key_tokens > (size_t)kMaxTokens || p->query_offset > (size_t)kMaxTokens)
+    // (positions of whole row tiles are 32-bit)
+    if (p->key_tokens > (size_t)kMaxTokens || p->query_offset + p->query_tokens > (size_t)kMaxTokens)
         return unsupported("attention dimensions exceed the 32-bit index range");
     int64_t qs[3], ks[3], vs[3], os[3];
     resolve_strides(qs, p->q_strides, p->heads, p->query_tokens, p->head_dim);
@@ -210,6 +211,81 @@ int window_args(const ofh_window_params* p, bool check_ptrs, const void* q, cons
     a.softcap = p->softcap;
     a.alibi = p->alibi_slopes;
     a.out_f32 = p->out_dtype == OFH_DTYPE_F32;
+    return OFH_SUCCESS;
+}
+
+// How a windowed call runs: the streaming kernel (0), or in 16 bits K and V
+// staged through LDS with 128 rows per workgroup (1), or 64 (2).
+//
+// 64 rows, whose keys two wavefront groups share, have half the chain and twice
+// the workgroups: faster while 128-row tiles leave CUs idle (us, 128 / 64 rows,
+// D128: B1 H32 N512 16.2 / 13.0, B1 H8 N2000 window 512 21.3 / 16.2, B2 H16 N700
+// 19.6 / 17.8), slower past that (480 tiles, B1 H40 N1500 window 256: 24.8 /
+// 28.6; 768, B2 H32 N1500: 53 / 68).
+//
+// The streaming kernel splits the keys over workgroups, so few rows against many
+// keys are its calls; but each of its tiles of 16 or 32 rows reads all its keys
+// itself. Measured (us, streaming / LDS, tiles): D128 N1500 B1 H8 M32 14.9 /
+// 26.8 (8), B8 H32/8 M4 23.7 / 28.1 (64), B4 H16 M32 32.1 / 28.0 (64), B8 H32/8
+// M16 46.0 / 28.0 (128); N6000 B1 H32/8 M32 38.7 / 88 (32), B4 H16 M63 73 / 86
+// (128), B8 H32/8 M32 110 / 89 (256); N300 B1 H32/8 M4 9.2 / 10.1 (8), B4 H16 M63
+// 13.1 / 10.8 (128); D256, where the LDS kernel has one workgroup per CU: B4 H16
+// M32 N6000 112 / 344 (128), B32 H32/4 M16 N6000 484 / 1317 (1024, four rounds),
+// B8 H32/8 M63 N6000 464 / 341 (1024, one round), B8 H32/8 M32 N300 28.5 / 24.0
+// (512).
+int window_groups(const ofh::StreamArgs& a, int dtype) {
+    if (dtype == OFH_DTYPE_F32) return 0;
+    // (a lane adds the offsets of up to 128 rows in 32 bits)
+    for (int64_t stride : {a.k_st, a.v_st})
+        if (stride > (kMaxOffset / 2 - 256) / 256) return 0;
+    const int dk = ofh::stream_kernel_dim(a.D, a.Dv);
+    const int64_t heads = (int64_t)a.B * a.H;
+    const int64_t wide = heads * ((a.T + ofh::window_rows(1) - 1) / ofh::window_rows(1));
+    const int groups = dk <= 128 && wide <= ofh::kComputeUnits ? 2 : 1;
+    const int64_t wgs = groups == 1 ? wide : heads * ((a.T + ofh::window_rows(2) - 1) / ofh::window_rows(2));
+    const int64_t slots = dk <= 128 ? 2 * ofh::kComputeUnits : ofh::kComputeUnits;
+    const int64_t rounds = (wgs + slots - 1) / slots;
+    const int rows = ofh::stream_tile_rows(dk, a.T * a.G);
+    const int64_t tiles = (int64_t)a.B * a.Hkv * (((int64_t)a.T * a.G + rows - 1) / rows);
+    int64_t keys = a.capacity;
+    if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + a.sinks + a.T);
+    const int64_t few = dk == 256 ? 400 : std::min<int64_t>(keys / 24, 160);
+    return tiles <= rounds * few ? 0 : groups;
+}
+
+int run_window(const ofh::StreamArgs& a, int dtype, int groups, hipStream_t stream) {
+    ofh::WindowArgs w{};
+    ofh::FwdArgs& f = w.f;
+    f.q = a.q;
+    f.k = a.k;
+    f.v = a.v;
+    f.o = a.o;
+    f.q_sb = a.q_sb; f.q_sh = a.q_sh; f.q_sm = a.q_st;
+    f.k_sb = a.k_sp; f.k_sh = a.k_sh; f.k_sn = a.k_st;
+    f.v_sb = a.v_sp; f.v_sh = a.v_sh; f.v_sn = a.v_st;
+    f.o_sb = a.o_sb; f.o_sh = a.o_sh; f.o_sm = a.o_st;
+    f.B = a.B;
+    f.H = a.H;
+    f.M = a.T;
+    f.N = a.capacity;
+    f.D = a.D;
+    f.Dv = a.Dv;
+    f.scale = a.scale;
+    f.scale_log2 = a.scale * 1.4426950408889634f;
+    f.softcap = a.softcap;
+    f.inv_softcap = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+    f.alibi = a.alibi;
+    f.out_f32 = a.out_f32;
+    const int rows = ofh::window_rows(groups);
+    f.num_q_tiles = (a.T + rows - 1) / rows;
+    w.G = a.G;
+    w.window = a.window;
+    w.sinks = a.sinks;
+    w.query_offset = (int)a.query_offset;
+    w.lengths = a.lengths;
+    w.key_splits = groups;
+    if (!ofh::grid_fits((int64_t)a.B * a.H * f.num_q_tiles, 256)) return unsupported("attention call exceeds the launch range");
+    OFH_HIP_CHECK(ofh::launch_window(w, dtype, stream));
     return OFH_SUCCESS;
 }
 
@@ -304,7 +380,7 @@ int ofh_window_attention_workspace_bytes(const ofh_window_params* p, size_t* byt
         if (bytes == nullptr) return invalid("bytes must be non-null");
         ofh::StreamArgs a;
         if (int rc = window_args(p, false, nullptr, nullptr, nullptr, nullptr, a)) return rc;
-        *bytes = plan_split(a, p->dtype, p->max_key_splits).bytes;
+        *bytes = window_groups(a, p->dtype) > 0 ? 0 : plan_split(a, p->dtype, p->max_key_splits).bytes;
         return OFH_SUCCESS;
     });
 }
@@ -314,6 +390,8 @@ int ofh_window_attention_fwd(const ofh_window_params* p, const void* q, const vo
     return guarded([&]() -> int {
         ofh::StreamArgs a;
         if (int rc = window_args(p, true, q, k, v, out, a)) return rc;
+        if (const int groups = window_groups(a, p->dtype))
+            return run_window(a, p->dtype, groups, static_cast<hipStream_t>(stream));
         return run_stream(a, p->dtype, plan_split(a, p->dtype, p->max_key_splits), workspace, workspace_bytes,
                           static_cast<hipStream_t>(stream));
     });

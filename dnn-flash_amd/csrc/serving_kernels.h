@@ -66,8 +66,10 @@ struct WindowArgs {
     int window, sinks;
     int query_offset;
     const int32_t* lengths;
-    int key_splits;  // wavefront groups that share a row slice's keys: 1, 2 or 4
+    int key_splits;  // wavefronts that share the keys of 32 rows: 1, or 2 up to kernel dim 128
 };
+// Query rows of a workgroup.
+inline int window_rows(int key_splits) { return 4 * kQueriesPerWave / key_splits; }
 hipError_t launch_window(const WindowArgs& a, int dtype, hipStream_t s);
 
 // New rows into pages.

@@ -32,8 +32,9 @@
 //
 // A key that no row of the tile sees has its V zeroed, so whatever a page holds
 // past a sequence's end does not reach the result. Where rows differ in what
-// they see (several new tokens) and such a step's V holds a NaN or an infinity,
-// the step's products are formed once per token.
+// they see (several new tokens), a NaN or an infinity in the V of a key leaves a
+// NaN in the O of rows that do not see it: a wavefront that ends with a NaN runs
+// again and forms the products of such steps once per token.
 
 #include "flash_wave32.h"
 #include "serving_kernels.h"
@@ -363,6 +364,8 @@ struct StreamWave {
         return acc;
     }
 
+    // SEEN: steps in which rows differ in what they see form their products once per token.
+    template <bool SEEN>
     __device__ __forceinline__ void compute(Step& s, int step, const Pages& pg) {
         int key0[S::NB];  // -1: the block's keys count for nothing
         bool mask = false;
@@ -383,22 +386,10 @@ struct StreamWave {
         }
         Operands vt;
         v_operands(s, vt);
-        bool redo = false;  // rows differ in what they see, and V holds a NaN or an infinity
         unsigned keep[MASKS] = {};
         if (mask) {
             key_masks(key0, hi_max, lo_min, keep);
             vt.apply(keep);
-            if (r.t0 != r.t1) {
-                // 0 V summed over the step is NaN for such a V, else 0
-                f32x4 probe = {0.f, 0.f, 0.f, 0.f};
-                const float none[S::NB * 4] = {};
-#pragma unroll
-                for (int j = 0; j < S::NO; ++j) probe = pv<false>(j, vt, none, u32x4{0u, 0u, 0u, 0u}, keep, probe);
-                bool bad = false;
-#pragma unroll
-                for (int t = 0; t < 4; ++t) bad = bad || !(probe[t] == 0.0f);
-                redo = __builtin_amdgcn_ballot_w64(bad) != 0;
-            }
         }
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
@@ -476,7 +467,7 @@ struct StreamWave {
                 for (int t = 0; t < 8; t += 2) l[i] = Dot2<T>::sum2(typename Dot2<T>::v2{pk[t], pk[t + 1]}, l[i]);
                 pb = __builtin_bit_cast(u32x4, pk);
             }
-            if (!redo) {
+            if (!SEEN || !mask) {
 #pragma unroll
                 for (int j = 0; j < S::NO; ++j) o[i][j] = pv<false>(j, vt, p, pb, keep, o[i][j]);
             } else {
@@ -495,36 +486,61 @@ struct StreamWave {
         }
     }
 
+    __device__ __forceinline__ bool nan_in_o() const {
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int c = 0; c < S::NO; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bad = bad || o[i][c][e] != o[i][c][e];
+        return __builtin_amdgcn_ballot_w64(bad) != 0;
+    }
+
     // This wavefront's steps: begin, begin + kWaves, ... below end.
     __device__ __forceinline__ void run(int begin, int end) {
         if (begin >= end) return;
-        if constexpr (DK > 128) {
-            Step s;
-            Pages p0 = pages(begin);
-            for (int step = begin; step < end; step += kWaves) {
-                load(s, step, p0);
-                const Pages p1 = pages(min(step + kWaves, end - 1));
-                compute(s, step, p0);
-                p0 = p1;
-            }
-            return;
-        }
         // loads past the last step repeat it: a branch around them would make
         // every wait one for all loads in flight
         auto clamp = [&](int step) { return min(step, end - 1); };
-        Step s0, s1;
-        Pages p0 = pages(begin), p1 = pages(clamp(begin + kWaves));
-        load(s0, begin, p0);
-        for (int step = begin; step < end; step += 2 * kWaves) {
-            load(s1, clamp(step + kWaves), p1);
-            const Pages p2 = pages(clamp(step + 2 * kWaves));
-            compute(s0, step, p0);
-            if (step + kWaves >= end) break;
-            load(s0, clamp(step + 2 * kWaves), p2);
-            const Pages p3 = pages(clamp(step + 3 * kWaves));
-            compute(s1, step + kWaves, p1);
-            p0 = p2;
-            p1 = p3;
+        if constexpr (DK <= 128) {
+            Step s0, s1;
+            Pages p0 = pages(begin), p1 = pages(clamp(begin + kWaves));
+            load(s0, begin, p0);
+            for (int step = begin; step < end; step += 2 * kWaves) {
+                load(s1, clamp(step + kWaves), p1);
+                const Pages p2 = pages(clamp(step + 2 * kWaves));
+                compute<false>(s0, step, p0);
+                if (step + kWaves >= end) break;
+                load(s0, clamp(step + 2 * kWaves), p2);
+                const Pages p3 = pages(clamp(step + 3 * kWaves));
+                compute<false>(s1, step + kWaves, p1);
+                p0 = p2;
+                p1 = p3;
+            }
+        } else {
+            run_plain<false>(begin, end);  // (two steps' K and V do not fit the registers)
+        }
+        if (r.t0 != r.t1 && nan_in_o()) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+#pragma unroll
+                for (int c = 0; c < S::NO; ++c) o[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+                m[i] = kNegInf;
+                l[i] = 0.0f;
+            }
+            run_plain<true>(begin, end);
+        }
+    }
+    template <bool SEEN>
+    __device__ __forceinline__ void run_plain(int begin, int end) {
+        Step s;
+        Pages p0 = pages(begin);
+        for (int step = begin; step < end; step += kWaves) {
+            load(s, step, p0);
+            const Pages p1 = pages(min(step + kWaves, end - 1));
+            compute<SEEN>(s, step, p0);
+            p0 = p1;
         }
     }
 };
