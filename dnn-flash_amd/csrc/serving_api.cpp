@@ -99,20 +99,31 @@ struct Split {
     size_t bytes;
 };
 
+// Measured (us, bf16 H32/8 D128 unless said, parts per tile): a workgroup per CU
+// fills the memory's rate, so more parts only add starts and rows to join: B8
+// N4000 4 parts 31.6, 16 36.0; D256 B4 H16/4 N20000 16 parts 65, 32 71; two per CU
+// pay off with long parts: f32 D128 B8 H16 N2000-8000 2 parts 140, 4 133, D64 B16
+// H16 N2000-8000 1 part 82, 2 75, but B32 N100-600 1 part 15.4, 2 20.1. Parts of a
+// step per wavefront (4): one sequence of 1001 keys 10.6, of 8 steps 11.8, of 16
+// 14.7; with less than four such parts in all the join costs more than they save:
+// B4 N300 split 11.6, unsplit 10.1.
 Split plan_split(const ofh::StreamArgs& a, int dtype, int max_key_splits) {
-    Split s;
+    Split s{};
     const int dk = ofh::stream_kernel_dim(a.D, a.Dv);
     s.tile_rows = ofh::stream_tile_rows(dk, a.T * a.G);
     s.row_tiles = (int)(((int64_t)a.T * a.G + s.tile_rows - 1) / s.tile_rows);
     s.units = (int64_t)a.B * a.Hkv * s.row_tiles;
-    // two steps of each wavefront: fewer are not worth joining
-    s.min_steps = 2 * ofh::kStreamThreads / 64;
+    s.splits = 1;
+    s.min_steps = ofh::kStreamThreads / 64;
     const int64_t tile_tokens = std::min<int64_t>(a.T, s.tile_rows / a.G + 2);
     int64_t keys = a.capacity;
     if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + a.sinks + tile_tokens + 2 * ofh::kStreamKeys);
-    const int64_t steps = (keys + ofh::stream_step_keys(dtype, dk) - 1) / ofh::stream_step_keys(dtype, dk);
-    int64_t n = std::min<int64_t>(steps / s.min_steps, (4 * ofh::kComputeUnits + s.units - 1) / s.units);
-    n = std::min<int64_t>(n, max_key_splits > 0 ? max_key_splits : 128);
+    const int step = ofh::stream_step_keys(dtype, dk);
+    const int64_t steps = (keys + step - 1) / step;
+    if (steps < 4 * s.min_steps) return s;
+    const int64_t one = (ofh::kComputeUnits + s.units - 1) / s.units, two = (2 * ofh::kComputeUnits + s.units - 1) / s.units;
+    int64_t n = dk <= 128 ? std::max(one, std::min<int64_t>(two, steps / 32)) : one;
+    n = std::min<int64_t>({n, steps / s.min_steps, max_key_splits > 0 ? max_key_splits : 128});
     s.splits = (int)std::max<int64_t>(1, n);
     const size_t rows = (size_t)s.units * s.splits * s.tile_rows;
     s.bytes = s.splits > 1 ? round256(rows * a.Dv * 4) + rows * 8 : 0;
@@ -124,15 +135,10 @@ void unsplit(Split& s) {
     s.bytes = 0;
 }
 
-int check_grid(const Split& s, const ofh::StreamArgs& a) {
-    if (!ofh::grid_fits(s.units * s.splits, ofh::kStreamThreads) ||
-        !ofh::grid_fits((int64_t)a.B * a.Hkv * a.T * a.G, ofh::kStreamThreads))
-        return unsupported("attention call exceeds the launch range");
-    return OFH_SUCCESS;
-}
-
 int run_stream(ofh::StreamArgs& a, int dtype, Split s, void* workspace, size_t workspace_bytes, hipStream_t stream) {
-    if (int rc = check_grid(s, a)) return rc;
+    if (!ofh::grid_fits(s.units * s.splits, ofh::kStreamThreads) ||
+        !ofh::grid_fits((int64_t)a.B * a.Hkv * a.T * a.G * ((a.Dv + 31) / 32), 64))
+        return unsupported("attention call exceeds the launch range");
     ofh::ScratchLease lease;
     if (s.bytes > 0 && workspace == nullptr) {
         bool fits = true;

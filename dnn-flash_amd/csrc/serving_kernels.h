@@ -41,11 +41,12 @@ struct StreamArgs {
     float scale, softcap;
     const float* alibi;  // [H] or null
     int out_f32;
-    // Row tiles per (sequence, key-value head) and workgroups per row tile.
-    int row_tiles, splits, min_steps;
-    float* part_o;   // [units][splits][rows of a tile][Dv], splits > 1
-    float* part_ml;  // [units][splits][rows of a tile][2]: max (log2 units), sum
-    unsigned* counters;  // arrival counters [units], zero between calls, or null: a second launch joins
+    int row_tiles;  // per (sequence, key-value head)
+    // Workgroups per tile. A tile shares its own steps among as many of them as
+    // get min_steps each; the others have nothing to do.
+    int splits, min_steps;
+    float* part_o;   // [tiles][splits][rows of a tile][Dv]
+    float* part_ml;  // [tiles][splits][rows of a tile][2]: max (log2 units), sum
 };
 
 constexpr int kStreamThreads = 256;

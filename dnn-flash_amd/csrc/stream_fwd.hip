@@ -14,15 +14,16 @@
 //  * the accumulator layout (lane n + 16 g holds keys 4g .. 4g + 3 of query row
 //    n) is the operand layout of P^T when a product's eight keys per lane group
 //    are 4g .. 4g + 3 of two 16-key blocks, so P stays where it is formed.
-// The next step's K and V are requested before this step's products. Blocks of
-// 16 keys never cross a page (page sizes are multiples of 16), so a block's
-// page is one scalar load, made two steps ahead.
+// Blocks of 16 keys never cross a page (page sizes are multiples of 16), so a
+// block's page is one scalar load, made a step ahead.
 //
 // A tile has 16 (or 32) rows of one (sequence, key-value head): the heads of a
 // group and the new tokens share what is read. The wavefronts of a workgroup
-// take the steps in turn and fold their (m, l, O) in LDS; `splits` workgroups
-// share a tile's steps evenly, by the sequence's own visible keys, and are
-// joined with O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.
+// take the steps in turn and fold their (m, l, O) in LDS. Where tiles are few,
+// `splits` workgroups share a tile's steps evenly and are joined with
+// O = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s. (On ragged batches finer
+// parts cost what their better balance gains, a start of 3-4 us each; shares
+// of the whole work, longest sequence first, were slower still.)
 //
 // The running max that probabilities are taken against is raised only when a
 // score exceeds it by more than 2^8, so a step without a raise (nearly all)
@@ -35,6 +36,8 @@
 // they see (several new tokens), a NaN or an infinity in the V of a key leaves a
 // NaN in the O of rows that do not see it: a wavefront that ends with a NaN runs
 // again and forms the products of such steps once per token.
+
+#include <algorithm>
 
 #include "flash_wave32.h"
 #include "serving_kernels.h"
@@ -131,20 +134,18 @@ __device__ __forceinline__ StreamRange stream_range(const StreamArgs& a, int b, 
     return r;
 }
 
-// Steps per split and splits that have any, of a tile of `steps` steps.
-__device__ __forceinline__ int stream_split(const StreamArgs& a, int steps, int& per) {
-    const int n = max(1, min(a.splits, steps / max(1, a.min_steps)));
-    per = max(1, (steps + n - 1) / n);
-    return max(1, (steps + per - 1) / per);
-}
+// A workgroup's share: part `part` of a tile.
+struct StreamPart {
+    int b, hk, rt, part;
+};
 
-// Workgroup -> (sequence and key-value head, row tile, split). Workgroups go to
-// the 8 XCDs in turn; where they can be dealt out evenly, the tiles and splits
-// of one key-value head run on one XCD and share its L2. Late tokens, whose
-// keys are most, run first.
-__device__ __forceinline__ void stream_work(const StreamArgs& a, int id, int& bh, int& rt, int& split) {
+// Workgroups go to the 8 XCDs in turn; where they can be dealt out evenly, the
+// tiles and parts of a key-value head run on one XCD and share its L2. Late
+// tokens, whose keys are most, run first.
+__device__ __forceinline__ StreamPart stream_part(const StreamArgs& a, int id) {
     const int n = a.B * a.Hkv, per = a.row_tiles * a.splits;
-    int rest;
+    StreamPart p;
+    int rest, bh;
     if ((n & 7) == 0) {
         const int j = id >> 3;
         bh = j / per * 8 + (id & 7);
@@ -153,8 +154,18 @@ __device__ __forceinline__ void stream_work(const StreamArgs& a, int id, int& bh
         bh = id / per;
         rest = id % per;
     }
-    split = rest % a.splits;
-    rt = a.row_tiles - 1 - rest / a.splits;
+    p.b = bh / a.Hkv;
+    p.hk = bh - p.b * a.Hkv;
+    p.part = rest % a.splits;
+    p.rt = a.row_tiles - 1 - rest / a.splits;
+    return p;
+}
+
+// Parts of a tile of `steps` steps, and the steps of each.
+__device__ __forceinline__ int stream_parts(const StreamArgs& a, int steps, int& per) {
+    const int n = max(1, min(a.splits, steps / a.min_steps));
+    per = max(1, (steps + n - 1) / n);
+    return max(1, (steps + per - 1) / per);
 }
 
 // O of a row, columns [c, c + W): normalised, in the output's type.
@@ -182,8 +193,10 @@ struct StreamWave {
     static constexpr int VD = VB / 4;         // dwords
     typedef unsigned int vraw __attribute__((ext_vector_type(VD)));
 
-    struct Step {  // K and V of a step as loaded
+    struct StepK {  // K and V of a step as loaded
         u32x4 k[S::NB][S::KF];
+    };
+    struct StepV {
         vraw v[S::NB * 4][S::VC];
     };
     struct Pages {  // pages of a step's blocks (contiguous K and V: unused)
@@ -204,13 +217,12 @@ struct StreamWave {
     const char* vbase;
     unsigned koff, voff[4];
 
-    __device__ __forceinline__ StreamWave(const StreamArgs& args, const StreamRange& range, int bh, int rt)
-        : a(args), r(range) {
+    __device__ __forceinline__ StreamWave(const StreamArgs& args, const StreamRange& range, const StreamPart& at)
+        : a(args), r(range), b(at.b), hk(at.hk) {
+        const int rt = at.rt;
         const int lane = threadIdx.x & 63;
         n = lane & 15;
         g = lane >> 4;
-        b = bh / a.Hkv;
-        hk = bh - b * a.Hkv;
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             const int row = min(rt * ROWS + 16 * i + n, a.T * a.G - 1);
@@ -272,47 +284,51 @@ struct StreamWave {
     }
     __device__ __forceinline__ bool page_ok(int id) const { return (unsigned)id < (unsigned)a.num_pages; }
 
-    __device__ __forceinline__ void load(Step& s, int step, const Pages& p) const {
+    // Address of the first row of a block, rows `stride` elements apart and pages
+    // `page_stride`; an entry outside the pool reads page 0, masked.
+    __device__ __forceinline__ const char* block_at(const char* base, int key, int page, int64_t page_stride,
+                                                    int64_t stride) const {
+        if (!PAGED) return base + (int64_t)key * stride * S::ES;
+        const int64_t id = page_ok(page) ? uniform(page) : 0;
+        return base + (id * page_stride + (int64_t)(key & ((1 << a.page_shift) - 1)) * stride) * S::ES;
+    }
+    // Contiguous rows past the end repeat the last one: the rows of the block.
+    __device__ __forceinline__ int last_row(int key) const {
+        return PAGED ? kStreamKeys - 1 : min(kStreamKeys - 1, a.capacity - 1 - key);
+    }
+    // (Columns past the head dim repeat the row's last chunk: K is cleared before
+    // its product, V fills columns that are never stored.)
+    __device__ __forceinline__ void load_k(StepK& s, int step, const Pages& p) const {
 #pragma unroll
         for (int j = 0; j < S::NB; ++j) {
-            const int key = first_key(step, j);
-            const char* kb = kbase;
-            const char* vb = vbase;
-            unsigned ko = koff, vo[4] = {voff[0], voff[1], voff[2], voff[3]};
-            if (PAGED) {
-                // an entry outside the pool reads page 0, masked
-                const int64_t page = page_ok(p.id[j]) ? uniform(p.id[j]) : 0;
-                const int64_t row = key & ((1 << a.page_shift) - 1);
-                kb += (page * a.k_sp + row * a.k_st) * S::ES;
-                vb += (page * a.v_sp + row * a.v_st) * S::ES;
-            } else {
-                kb += (int64_t)key * a.k_st * S::ES;
-                vb += (int64_t)key * a.v_st * S::ES;
-                if (key + kStreamKeys > a.capacity) {  // rows past the end repeat the last one
-                    const int last = a.capacity - 1 - key;
-                    ko = (unsigned)(min(n, last) * (int)a.k_st * S::ES);
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) vo[t] = (unsigned)(min(4 * g + t, last) * (int)a.v_st * S::ES);
-                }
-            }
-            // columns past the head dim repeat the row's last chunk: K is
-            // cleared below, V fills columns that are never stored
+            const int key = first_key(step, j), last = last_row(key);
+            const char* kb = block_at(kbase, key, p.id[j], a.k_sp, a.k_st);
+            const unsigned ko = last == kStreamKeys - 1 ? koff : (unsigned)(min(n, last) * (int)a.k_st * S::ES);
 #pragma unroll
             for (int c = 0; c < S::KF; ++c)
                 s.k[j][c] = *(const u32x4*)(kb + ko + (unsigned)(S::ES * min(S::KW * (4 * c + g), a.D - S::KW)));
+        }
+    }
+    __device__ __forceinline__ void load_v(StepV& s, int step, const Pages& p) const {
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+        for (int j = 0; j < S::NB; ++j) {
+            const int key = first_key(step, j), last = last_row(key);
+            const char* vb = block_at(vbase, key, p.id[j], a.v_sp, a.v_st);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const unsigned vo =
+                    last == kStreamKeys - 1 ? voff[t] : (unsigned)(min(4 * g + t, last) * (int)a.v_st * S::ES);
 #pragma unroll
                 for (int c = 0; c < S::VC; ++c)
-                    s.v[4 * j + t][c] =
-                        *(const vraw*)(vb + vo[t] + (unsigned)(S::ES * min(S::VW * (16 * c + n), a.Dv - S::VW)));
+                    s.v[4 * j + t][c] = *(const vraw*)(vb + vo + (unsigned)(S::ES * min(S::VW * (16 * c + n), a.Dv - S::VW)));
+            }
         }
     }
 
     // V operands of a step. 16 bits: product i of chunk c holds eight keys of
     // column 8m + i. fp32: the rows as they are, product (key, chunk, i).
     using Operands = typename S::template Operands<vraw>;
-    __device__ __forceinline__ void v_operands(const Step& s, Operands& vt) const {
+    __device__ __forceinline__ void v_operands(const StepV& s, Operands& vt) const {
         if constexpr (F32) {
 #pragma unroll
             for (int t = 0; t < S::NB * 4; ++t)
@@ -364,122 +380,154 @@ struct StreamWave {
         return acc;
     }
 
-    // SEEN: steps in which rows differ in what they see form their products once per token.
-    template <bool SEEN>
-    __device__ __forceinline__ void compute(Step& s, int step, const Pages& pg) {
-        int key0[S::NB];  // -1: the block's keys count for nothing
-        bool mask = false;
+    // S^T = K Q^T of row tile i.
+    __device__ __forceinline__ void scores(const StepK& s, int i, f32x4 (&sc)[S::NB]) const {
 #pragma unroll
         for (int j = 0; j < S::NB; ++j) {
-            key0[j] = first_key(step, j);
-            if (step * S::NB + j >= r.blocks || (PAGED && !page_ok(uniform(pg.id[j])))) key0[j] = -1;
-            mask = mask || key0[j] < 0 || key0[j] + kStreamKeys > hi_min ||
-                   (key0[j] < lo_max && key0[j] + kStreamKeys > a.sinks);
-        }
-        if (S::KW * 4 * S::KF > a.D) {  // K columns past the head dim
+            sc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < S::KF; ++c)
-                if (S::KW * (4 * c + g) >= a.D) {
+            for (int c = 0; c < S::KF; ++c) {
+                if constexpr (F32) {
 #pragma unroll
-                    for (int j = 0; j < S::NB; ++j) s.k[j][c] = u32x4{0u, 0u, 0u, 0u};
-                }
-        }
-        Operands vt;
-        v_operands(s, vt);
-        unsigned keep[MASKS] = {};
-        if (mask) {
-            key_masks(key0, hi_max, lo_min, keep);
-            vt.apply(keep);
-        }
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-            f32x4 sc[S::NB];
-#pragma unroll
-            for (int j = 0; j < S::NB; ++j) {
-                sc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < S::KF; ++c) {
-                    if constexpr (F32) {
-#pragma unroll
-                        for (int t = 0; t < 4; ++t)
-                            sc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                __builtin_bit_cast(float, (unsigned)s.k[j][c][t]),
-                                __builtin_bit_cast(float, (unsigned)q[i][c][t]), sc[j], 0, 0, 0);
-                    } else {
-                        sc[j] = S::mma(s.k[j][c], q[i][c], sc[j]);
-                    }
+                    for (int t = 0; t < 4; ++t)
+                        sc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, (unsigned)s.k[j][c][t]),
+                                                                     __builtin_bit_cast(float, (unsigned)q[i][c][t]),
+                                                                     sc[j], 0, 0, 0);
+                } else {
+                    sc[j] = S::mma(s.k[j][c], q[i][c], sc[j]);
                 }
             }
-            // scores in log2 units
-            float x[S::NB * 4];
-            const float to_log2 = a.scale * kLog2e;
+        }
+    }
+
+    // Scores of row tile i -> probabilities against the running max: p, and in 16
+    // bits their operand pb; m, l and O are brought to that max.
+    __device__ __forceinline__ void softmax(int i, const f32x4 (&sc)[S::NB], const int (&key0)[S::NB], bool mask,
+                                            float (&p)[S::NB * 4], u32x4& pb) {
+        // scores in log2 units
+        float x[S::NB * 4];
+        const float to_log2 = a.scale * kLog2e;
+#pragma unroll
+        for (int j = 0; j < S::NB; ++j)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) x[4 * j + t] = sc[j][t] * to_log2;
+        if (a.alibi != nullptr || a.softcap > 0.0f) {
 #pragma unroll
             for (int j = 0; j < S::NB; ++j)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) x[4 * j + t] = sc[j][t] * to_log2;
-            if (a.alibi != nullptr || a.softcap > 0.0f) {
+                for (int t = 0; t < 4; ++t) {
+                    float y = sc[j][t] * a.scale;
+                    if (a.alibi != nullptr) y = __builtin_fmaf(slope[i], (float)(key0[j] + 4 * g + t - pos[i]), y);
+                    if (a.softcap > 0.0f) {
+                        // cap tanh(y / cap) = cap (1 - 2 / (2^u + 1)), u = 2 log2(e) y / cap
+                        const float u = __builtin_amdgcn_exp2f(y * (2.0f * kLog2e / a.softcap));
+                        y = __builtin_fmaf(-2.0f * a.softcap, __builtin_amdgcn_rcpf(u + 1.0f), a.softcap);
+                    }
+                    x[4 * j + t] = y * kLog2e;
+                }
+        }
+        if (mask) {
 #pragma unroll
-                for (int j = 0; j < S::NB; ++j)
+            for (int j = 0; j < S::NB; ++j)
 #pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        float y = sc[j][t] * a.scale;
-                        if (a.alibi != nullptr) y = __builtin_fmaf(slope[i], (float)(key0[j] + 4 * g + t - pos[i]), y);
-                        if (a.softcap > 0.0f) {
-                            // cap tanh(y / cap) = cap (1 - 2 / (2^u + 1)), u = 2 log2(e) y / cap
-                            const float u = __builtin_amdgcn_exp2f(y * (2.0f * kLog2e / a.softcap));
-                            y = __builtin_fmaf(-2.0f * a.softcap, __builtin_amdgcn_rcpf(u + 1.0f), a.softcap);
-                        }
-                        x[4 * j + t] = y * kLog2e;
+                for (int t = 0; t < 4; ++t)
+                    if (!(key0[j] >= 0 && seen(key0[j] + 4 * g + t, hi[i], lo[i]))) x[4 * j + t] = kNegInf;
+        }
+        float top = x[0];
+#pragma unroll
+        for (int t = 1; t < S::NB * 4; ++t) top = fmaxf(top, x[t]);
+        if (__builtin_amdgcn_ballot_w64(top > m[i] + kRescaleSlack) != 0) {
+            top = max4(top);
+            const bool raise = top > m[i] + kRescaleSlack;
+            const float alpha = raise ? __builtin_amdgcn_exp2f(m[i] - top) : 1.0f;
+            m[i] = raise ? top : m[i];
+            l[i] *= alpha;
+#pragma unroll
+            for (int c = 0; c < S::NO; ++c) o[i][c] *= alpha;
+        }
+        const float mu = m[i] == kNegInf ? 0.0f : m[i];
+#pragma unroll
+        for (int t = 0; t < S::NB * 4; ++t) p[t] = __builtin_amdgcn_exp2f(x[t] - mu);
+        if constexpr (F32) {
+#pragma unroll
+            for (int t = 0; t < S::NB * 4; ++t) l[i] += p[t];
+        } else {
+            typename S::P pk;
+#pragma unroll
+            for (int t = 0; t < 8; ++t) pk[t] = (T)p[t];
+#pragma unroll
+            for (int t = 0; t < 8; t += 2) l[i] = Dot2<T>::sum2(typename Dot2<T>::v2{pk[t], pk[t + 1]}, l[i]);
+            pb = __builtin_bit_cast(u32x4, pk);
+        }
+    }
+
+    // The steps begin, begin + kWaves, ... below end. K's registers take the next
+    // step's rows once its products are formed, V's once its operands are: loads
+    // are in flight all the time without a second set of registers. Loads past
+    // the last step repeat it (a branch around them would make every wait one for
+    // all loads in flight).
+    // SEEN: steps in which rows differ in what they see form their products once per token.
+    template <bool SEEN>
+    __device__ __forceinline__ void run_steps(int begin, int end) {
+        StepK sk;
+        StepV sv;
+        Pages pg = pages(begin);
+        load_k(sk, begin, pg);
+        load_v(sv, begin, pg);
+        Pages pn = pages(min(begin + kWaves, end - 1));
+        for (int step = begin; step < end; step += kWaves) {
+            const int next = min(step + kWaves, end - 1);
+            int key0[S::NB];  // -1: the block's keys count for nothing
+            bool mask = false;
+#pragma unroll
+            for (int j = 0; j < S::NB; ++j) {
+                key0[j] = first_key(step, j);
+                if (step * S::NB + j >= r.blocks || (PAGED && !page_ok(uniform(pg.id[j])))) key0[j] = -1;
+                mask = mask || key0[j] < 0 || key0[j] + kStreamKeys > hi_min ||
+                       (key0[j] < lo_max && key0[j] + kStreamKeys > a.sinks);
+            }
+            if (S::KW * 4 * S::KF > a.D) {  // K columns past the head dim
+#pragma unroll
+                for (int c = 0; c < S::KF; ++c)
+                    if (S::KW * (4 * c + g) >= a.D) {
+#pragma unroll
+                        for (int j = 0; j < S::NB; ++j) sk.k[j][c] = u32x4{0u, 0u, 0u, 0u};
                     }
             }
+            f32x4 sc[RT][S::NB];
+#pragma unroll
+            for (int i = 0; i < RT; ++i) scores(sk, i, sc[i]);
+            load_k(sk, next, pn);
+            float p[RT][S::NB * 4];
+            u32x4 pb[RT];
+#pragma unroll
+            for (int i = 0; i < RT; ++i) softmax(i, sc[i], key0, mask, p[i], pb[i]);
+            Operands vt;
+            v_operands(sv, vt);
+            load_v(sv, next, pn);
+            pg = pn;
+            pn = pages(min(step + 2 * kWaves, end - 1));
+            unsigned keep[MASKS] = {};
             if (mask) {
-#pragma unroll
-                for (int j = 0; j < S::NB; ++j)
-#pragma unroll
-                    for (int t = 0; t < 4; ++t)
-                        if (!(key0[j] >= 0 && seen(key0[j] + 4 * g + t, hi[i], lo[i]))) x[4 * j + t] = kNegInf;
+                key_masks(key0, hi_max, lo_min, keep);
+                vt.apply(keep);
             }
-            float top = x[0];
 #pragma unroll
-            for (int t = 1; t < S::NB * 4; ++t) top = fmaxf(top, x[t]);
-            if (__builtin_amdgcn_ballot_w64(top > m[i] + kRescaleSlack) != 0) {
-                top = max4(top);
-                const bool raise = top > m[i] + kRescaleSlack;
-                const float alpha = raise ? __builtin_amdgcn_exp2f(m[i] - top) : 1.0f;
-                m[i] = raise ? top : m[i];
-                l[i] *= alpha;
+            for (int i = 0; i < RT; ++i) {
+                if (!SEEN || !mask) {
 #pragma unroll
-                for (int c = 0; c < S::NO; ++c) o[i][c] *= alpha;
-            }
-            const float mu = m[i] == kNegInf ? 0.0f : m[i];
-            float p[S::NB * 4];
-            u32x4 pb = {0u, 0u, 0u, 0u};
+                    for (int j = 0; j < S::NO; ++j) o[i][j] = pv<false>(j, vt, p[i], pb[i], keep, o[i][j]);
+                } else {
+                    for (int t = r.t0; t <= r.t1; ++t) {
+                        int h, w;
+                        limits(t, h, w);
+                        key_masks(key0, h, w, keep);
 #pragma unroll
-            for (int t = 0; t < S::NB * 4; ++t) p[t] = __builtin_amdgcn_exp2f(x[t] - mu);
-            if constexpr (F32) {
+                        for (int j = 0; j < S::NO; ++j) {
+                            const f32x4 acc = pv<true>(j, vt, p[i], pb[i], keep, o[i][j]);
 #pragma unroll
-                for (int t = 0; t < S::NB * 4; ++t) l[i] += p[t];
-            } else {
-                typename S::P pk;
-#pragma unroll
-                for (int t = 0; t < 8; ++t) pk[t] = (T)p[t];
-#pragma unroll
-                for (int t = 0; t < 8; t += 2) l[i] = Dot2<T>::sum2(typename Dot2<T>::v2{pk[t], pk[t + 1]}, l[i]);
-                pb = __builtin_bit_cast(u32x4, pk);
-            }
-            if (!SEEN || !mask) {
-#pragma unroll
-                for (int j = 0; j < S::NO; ++j) o[i][j] = pv<false>(j, vt, p, pb, keep, o[i][j]);
-            } else {
-                for (int t = r.t0; t <= r.t1; ++t) {
-                    int h, w;
-                    limits(t, h, w);
-                    key_masks(key0, h, w, keep);
-#pragma unroll
-                    for (int j = 0; j < S::NO; ++j) {
-                        const f32x4 acc = pv<true>(j, vt, p, pb, keep, o[i][j]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[i][j][e] = tok[i] == t ? acc[e] : o[i][j][e];
+                            for (int e = 0; e < 4; ++e) o[i][j][e] = tok[i] == t ? acc[e] : o[i][j][e];
+                        }
                     }
                 }
             }
@@ -500,27 +548,7 @@ struct StreamWave {
     // This wavefront's steps: begin, begin + kWaves, ... below end.
     __device__ __forceinline__ void run(int begin, int end) {
         if (begin >= end) return;
-        // loads past the last step repeat it: a branch around them would make
-        // every wait one for all loads in flight
-        auto clamp = [&](int step) { return min(step, end - 1); };
-        if constexpr (DK <= 128) {
-            Step s0, s1;
-            Pages p0 = pages(begin), p1 = pages(clamp(begin + kWaves));
-            load(s0, begin, p0);
-            for (int step = begin; step < end; step += 2 * kWaves) {
-                load(s1, clamp(step + kWaves), p1);
-                const Pages p2 = pages(clamp(step + 2 * kWaves));
-                compute<false>(s0, step, p0);
-                if (step + kWaves >= end) break;
-                load(s0, clamp(step + 2 * kWaves), p2);
-                const Pages p3 = pages(clamp(step + 3 * kWaves));
-                compute<false>(s1, step + kWaves, p1);
-                p0 = p2;
-                p1 = p3;
-            }
-        } else {
-            run_plain<false>(begin, end);  // (two steps' K and V do not fit the registers)
-        }
+        run_steps<false>(begin, end);
         if (r.t0 != r.t1 && nan_in_o()) {
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
@@ -529,38 +557,90 @@ struct StreamWave {
                 m[i] = kNegInf;
                 l[i] = 0.0f;
             }
-            run_plain<true>(begin, end);
-        }
-    }
-    template <bool SEEN>
-    __device__ __forceinline__ void run_plain(int begin, int end) {
-        Step s;
-        Pages p0 = pages(begin);
-        for (int step = begin; step < end; step += kWaves) {
-            load(s, step, p0);
-            const Pages p1 = pages(min(step + kWaves, end - 1));
-            compute<SEEN>(s, step, p0);
-            p0 = p1;
+            run_steps<true>(begin, end);
         }
     }
 };
 
-template <typename T, int DK, int RT, bool PAGED>
-__global__ __launch_bounds__(kStreamThreads, 1) void stream_fwd_kernel(StreamArgs a) {
+// Joins the parts of every row: O = sum_s w_s O_s / sum_s w_s l_s with w_s =
+// 2^(m_s - max m). A wavefront takes 32 columns of a row: lane c + 8 g has four
+// columns of parts g, g + 8, ..., four of them in flight, and the eight lane
+// groups are folded with lane exchanges, so the order of the sums depends on
+// the number of parts alone. It reads every slot, without the lengths that say
+// which were used (a part without steps leaves max -inf and sum 0): one memory
+// round trip instead of two. (Joining in the workgroup that ends last, with
+// coherent stores and loads, took 3 us longer than this launch.)
+template <typename T>
+__global__ __launch_bounds__(kStreamThreads) void stream_join_kernel(StreamArgs a, int tile_rows) {
+    constexpr int G = 4;
+    const int lane = threadIdx.x & 63, grp = lane >> 3;
+    const int chunks = a.Dv / 4, blocks = (chunks + 7) / 8, rows = a.T * a.G;
+    const int64_t item = (int64_t)blockIdx.x * (kStreamThreads / 64) + uniform(threadIdx.x >> 6);
+    const int64_t at = item / blocks;  // row of all heads
+    const int bh = (int)(at / rows), row = (int)(at - (int64_t)bh * rows);
+    if (bh >= a.B * a.Hkv) return;
+    const int c = 8 * (int)(item - at * blocks) + (lane & 7), cc = min(c, chunks - 1);
+    const int rt = row / tile_rows;
+    const int64_t first = ((int64_t)bh * a.row_tiles + rt) * a.splits * tile_rows + row - rt * tile_rows;
+    float m = kNegInf, l = 0.0f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s = grp; s < a.splits; s += 8 * G) {
+        float ms[G], ls[G];
+        f32x4 os[G];
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+            const int64_t p = first + (int64_t)(s + 8 * j < a.splits ? s + 8 * j : s) * tile_rows;
+            ms[j] = a.part_ml[2 * p];
+            ls[j] = a.part_ml[2 * p + 1];
+            os[j] = *(const f32x4*)(a.part_o + p * a.Dv + 4 * cc);
+        }
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+            if (s + 8 * j >= a.splits) ms[j] = kNegInf;
+            // (O of a part without steps was not written; a NaN sum stays)
+            const bool none = ms[j] == kNegInf && !(ls[j] != ls[j]);
+            lse_fold(m, l, acc, ms[j], none ? 0.0f : ls[j], none ? f32x4{0.f, 0.f, 0.f, 0.f} : os[j]);
+        }
+    }
+#pragma unroll
+    for (int d = 8; d < 64; d *= 2) {
+        const float m2 = __shfl_xor(m, d), l2 = __shfl_xor(l, d);
+        f32x4 o2;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o2[j] = __shfl_xor(acc[j], d);
+        lse_fold(m, l, acc, m2, l2, o2);
+    }
+    if (grp == 0 && c < chunks) {
+        const int t = row / a.G, h = bh % a.Hkv * a.G + row - t * a.G;
+        const float x[4] = {acc[0], acc[1], acc[2], acc[3]};
+        put_out<T, 4>(a, bh / a.Hkv * a.o_sb + h * a.o_sh + t * a.o_st + 4 * c, x, l > 0.0f ? 1.0f / l : 0.0f);
+    }
+}
+
+template <typename T, int DK, int RT, bool PAGED, bool SPLIT>
+__global__
+__launch_bounds__(kStreamThreads, DK > 128 || (RT == 2 && DK * sizeof(T) >= 256) ? 1 : 2)
+void stream_fwd_kernel(StreamArgs a) {
     using W = StreamWave<T, DK, RT, PAGED>;
     using S = typename W::S;
     constexpr int STATE = 64 * (4 * S::NO * RT + 2 * RT);  // floats of a wavefront's state
     __shared__ __attribute__((aligned(16))) float lds[(kWaves - 1) * STATE];
-    int bh, rt, split;
-    stream_work(a, blockIdx.x, bh, rt, split);
-    const StreamRange r = stream_range(a, bh / a.Hkv, rt, W::ROWS);
+    const StreamPart at = stream_part(a, blockIdx.x);
+    const StreamRange r = stream_range(a, at.b, at.rt, W::ROWS);
     const int steps = (r.blocks + S::NB - 1) / S::NB;
-    int per;
-    const int active = stream_split(a, steps, per);
-    if (split >= active) return;
+    const int64_t slot = (((int64_t)at.b * a.Hkv + at.hk) * a.row_tiles + at.rt) * a.splits + at.part;
+    int per = steps;
+    if (SPLIT && at.part >= stream_parts(a, steps, per)) {
+        // no steps: what the join reads of this part
+        if ((int)threadIdx.x < W::ROWS) {
+            a.part_ml[2 * (slot * W::ROWS + threadIdx.x)] = kNegInf;
+            a.part_ml[2 * (slot * W::ROWS + threadIdx.x) + 1] = 0.0f;
+        }
+        return;
+    }
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    W w(a, r, bh, rt);
-    w.run(split * per + wave, min(steps, (split + 1) * per));
+    W w(a, r, at);
+    w.run(at.part * per + wave, min(steps, (at.part + 1) * per));
 
     // fold the wavefronts' states into wavefront 0's
 #pragma unroll
@@ -606,12 +686,12 @@ __global__ __launch_bounds__(kStreamThreads, 1) void stream_fwd_kernel(StreamArg
             }
         }
         // row n, columns 16 VW c + VW (4 g + e) + 0 .. VW - 1
-        const int row = rt * W::ROWS + 16 * i + w.n;
+        const int row = at.rt * W::ROWS + 16 * i + w.n;
         if (row >= a.T * a.G) continue;
         const int t = row / a.G, h = w.hk * a.G + row - t * a.G;
         const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
         const int64_t off = w.b * a.o_sb + h * a.o_sh + t * a.o_st;
-        const int64_t prow = (((int64_t)bh * a.row_tiles + rt) * a.splits + split) * W::ROWS + 16 * i + w.n;
+        const int64_t prow = slot * W::ROWS + 16 * i + w.n;
 #pragma unroll
         for (int c = 0; c < S::VC; ++c)
 #pragma unroll
@@ -621,7 +701,7 @@ __global__ __launch_bounds__(kStreamThreads, 1) void stream_fwd_kernel(StreamArg
                 float x[S::VW];
 #pragma unroll
                 for (int k = 0; k < S::VW; ++k) x[k] = w.o[i][c * S::VW + k][e];
-                if (active == 1) {
+                if (!SPLIT) {
                     put_out<T, S::VW>(a, off + col, x, inv);
                 } else {
 #pragma unroll
@@ -629,63 +709,26 @@ __global__ __launch_bounds__(kStreamThreads, 1) void stream_fwd_kernel(StreamArg
                         *(f32x4*)(a.part_o + prow * a.Dv + col + k) = f32x4{x[k], x[k + 1], x[k + 2], x[k + 3]};
                 }
             }
-        if (active > 1 && w.g == 0) {
+        if (SPLIT && w.g == 0) {
             a.part_ml[2 * prow] = top;
             a.part_ml[2 * prow + 1] = sum;
         }
     }
 }
-
-// Joins the splits of a row: a workgroup per row, groups of Dv / 4 threads
-// taking the splits in turn.
-template <typename T>
-__global__ __launch_bounds__(kStreamThreads) void stream_join_kernel(StreamArgs a, int rows, int step_keys) {
-    __shared__ float red[6 * kStreamThreads];
-    const int per_head = a.T * a.G;
-    const int bh = (int)(blockIdx.x / per_head), row = (int)(blockIdx.x % per_head);
-    const int rt = row / rows;
-    const StreamRange r = stream_range(a, bh / a.Hkv, rt, rows);
-    const int steps = (r.blocks * kStreamKeys + step_keys - 1) / step_keys;
-    int per;
-    const int active = stream_split(a, steps, per);
-    if (active == 1) return;  // written by its workgroup
-    const int chunks = a.Dv / 4, c = (int)threadIdx.x % chunks, grp = (int)threadIdx.x / chunks;
-    const int groups = min(active, kStreamThreads / chunks);
-    const int64_t first = ((int64_t)bh * a.row_tiles + rt) * a.splits * rows + row - rt * rows;
-    float m = kNegInf, l = 0.0f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    if (grp < groups)
-        for (int s = grp; s < active; s += groups) {
-            const int64_t p = first + (int64_t)s * rows;
-            lse_fold(m, l, acc, a.part_ml[2 * p], a.part_ml[2 * p + 1], *(const f32x4*)(a.part_o + p * a.Dv + 4 * c));
-        }
-    if (grp > 0 && grp < groups) {
-        float* e = red + 6 * threadIdx.x;
-        e[0] = m;
-        e[1] = l;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) e[2 + j] = acc[j];
-    }
-    __syncthreads();
-    if (grp != 0) return;
-    for (int k = 1; k < groups; ++k) {
-        const float* e = red + 6 * (k * chunks + c);
-        lse_fold(m, l, acc, e[0], e[1], f32x4{e[2], e[3], e[4], e[5]});
-    }
-    const int t = row / a.G, h = bh % a.Hkv * a.G + row - t * a.G;
-    const float x[4] = {acc[0], acc[1], acc[2], acc[3]};
-    put_out<T, 4>(a, bh / a.Hkv * a.o_sb + h * a.o_sh + t * a.o_st + 4 * c, x, l > 0.0f ? 1.0f / l : 0.0f);
-}
-
 template <typename T, int DK, int RT>
 hipError_t launch_stream_rt(const StreamArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)a.B * a.Hkv * a.row_tiles * a.splits)), block(kStreamThreads);
-    if (a.paged) hipLaunchKernelGGL((stream_fwd_kernel<T, DK, RT, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((stream_fwd_kernel<T, DK, RT, false>), grid, block, 0, s, a);
+    if (a.splits > 1) {
+        if (a.paged) hipLaunchKernelGGL((stream_fwd_kernel<T, DK, RT, true, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((stream_fwd_kernel<T, DK, RT, false, true>), grid, block, 0, s, a);
+    } else {
+        if (a.paged) hipLaunchKernelGGL((stream_fwd_kernel<T, DK, RT, true, false>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((stream_fwd_kernel<T, DK, RT, false, false>), grid, block, 0, s, a);
+    }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
-    hipLaunchKernelGGL((stream_join_kernel<T>), dim3((unsigned)((int64_t)a.B * a.Hkv * a.T * a.G)), block, 0, s, a,
-                       16 * RT, kStreamKeys * StreamTile<T, DK>::NB);
+    const int64_t items = (int64_t)a.B * a.Hkv * a.T * a.G * ((a.Dv + 31) / 32);
+    hipLaunchKernelGGL((stream_join_kernel<T>), dim3((unsigned)((items + kWaves - 1) / kWaves)), block, 0, s, a, 16 * RT);
     return hipGetLastError();
 }
 
