@@ -110,7 +110,7 @@ struct Split {
 Split plan_split(const ofh::StreamArgs& a, int dtype, int max_key_splits) {
     Split s{};
     const int dk = ofh::stream_kernel_dim(a.D, a.Dv);
-    s.tile_rows = ofh::stream_tile_rows(dk, a.T * a.G);
+    s.tile_rows = ofh::stream_tile_rows(dtype, dk, a.T * a.G);
     s.row_tiles = (int)(((int64_t)a.T * a.G + s.tile_rows - 1) / s.tile_rows);
     s.units = (int64_t)a.B * a.Hkv * s.row_tiles;
     s.splits = 1;
@@ -251,7 +251,7 @@ int window_groups(const ofh::StreamArgs& a, int dtype) {
     const int64_t wgs = groups == 1 ? wide : heads * ((a.T + ofh::window_rows(2) - 1) / ofh::window_rows(2));
     const int64_t slots = dk <= 128 ? 2 * ofh::kComputeUnits : ofh::kComputeUnits;
     const int64_t rounds = (wgs + slots - 1) / slots;
-    const int rows = ofh::stream_tile_rows(dk, a.T * a.G);
+    const int rows = ofh::stream_tile_rows(dtype, dk, a.T * a.G);
     const int64_t tiles = (int64_t)a.B * a.Hkv * (((int64_t)a.T * a.G + rows - 1) / rows);
     int64_t keys = a.capacity;
     if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + a.sinks + a.T);

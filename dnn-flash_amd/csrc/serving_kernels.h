@@ -55,7 +55,7 @@ constexpr int kStreamKeys = 16;  // keys of a block, the unit in which K and V a
 // Head dim that a stream kernel is built for: 64, 128 or 256 (0: none).
 int stream_kernel_dim(int D, int Dv);
 // Rows of a tile: 16 or 32.
-int stream_tile_rows(int kernel_dim, int rows);
+int stream_tile_rows(int dtype, int kernel_dim, int rows);
 // Keys of a wavefront's step.
 int stream_step_keys(int dtype, int kernel_dim);
 hipError_t launch_stream(const StreamArgs& a, int dtype, hipStream_t s);

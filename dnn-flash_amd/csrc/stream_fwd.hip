@@ -142,8 +142,8 @@ struct StreamPart {
 // Workgroups go to the 8 XCDs in turn; where they can be dealt out evenly, the
 // tiles and parts of a key-value head run on one XCD and share its L2. Late
 // tokens, whose keys are most, run first.
-__device__ __forceinline__ StreamPart stream_part(const StreamArgs& a, int id) {
-    const int n = a.B * a.Hkv, per = a.row_tiles * a.splits;
+__device__ __forceinline__ StreamPart stream_part(const StreamArgs& a, int id, int row_tiles) {
+    const int n = a.B * a.Hkv, per = row_tiles * a.splits;
     StreamPart p;
     int rest, bh;
     if ((n & 7) == 0) {
@@ -157,7 +157,7 @@ __device__ __forceinline__ StreamPart stream_part(const StreamArgs& a, int id) {
     p.b = bh / a.Hkv;
     p.hk = bh - p.b * a.Hkv;
     p.part = rest % a.splits;
-    p.rt = a.row_tiles - 1 - rest / a.splits;
+    p.rt = row_tiles - 1 - rest / a.splits;
     return p;
 }
 
@@ -184,7 +184,11 @@ __device__ __forceinline__ void put_out(const StreamArgs& a, int64_t off, const 
     }
 }
 
-template <typename T, int DK, int RT, bool PAGED>
+// How the wavefronts of a workgroup share: a tile's steps among them (kTile), of
+// which the workgroup has a part (kPart), or a tile each (kOwn).
+enum StreamMode { kTile, kPart, kOwn };
+
+template <typename T, int DK, int RT, bool PAGED, int STRIDE>
 struct StreamWave {
     using S = StreamTile<T, DK>;
     static constexpr int ROWS = 16 * RT;
@@ -461,7 +465,7 @@ struct StreamWave {
         }
     }
 
-    // The steps begin, begin + kWaves, ... below end. K's registers take the next
+    // The steps begin, begin + STRIDE, ... below end. K's registers take the next
     // step's rows once its products are formed, V's once its operands are: loads
     // are in flight all the time without a second set of registers. Loads past
     // the last step repeat it (a branch around them would make every wait one for
@@ -474,9 +478,9 @@ struct StreamWave {
         Pages pg = pages(begin);
         load_k(sk, begin, pg);
         load_v(sv, begin, pg);
-        Pages pn = pages(min(begin + kWaves, end - 1));
-        for (int step = begin; step < end; step += kWaves) {
-            const int next = min(step + kWaves, end - 1);
+        Pages pn = pages(min(begin + STRIDE, end - 1));
+        for (int step = begin; step < end; step += STRIDE) {
+            const int next = min(step + STRIDE, end - 1);
             int key0[S::NB];  // -1: the block's keys count for nothing
             bool mask = false;
 #pragma unroll
@@ -506,7 +510,7 @@ struct StreamWave {
             v_operands(sv, vt);
             load_v(sv, next, pn);
             pg = pn;
-            pn = pages(min(step + 2 * kWaves, end - 1));
+            pn = pages(min(step + 2 * STRIDE, end - 1));
             unsigned keep[MASKS] = {};
             if (mask) {
                 key_masks(key0, hi_max, lo_min, keep);
@@ -545,7 +549,7 @@ struct StreamWave {
         return __builtin_amdgcn_ballot_w64(bad) != 0;
     }
 
-    // This wavefront's steps: begin, begin + kWaves, ... below end.
+    // This wavefront's steps: begin, begin + STRIDE, ... below end.
     __device__ __forceinline__ void run(int begin, int end) {
         if (begin >= end) return;
         run_steps<false>(begin, end);
@@ -617,15 +621,21 @@ __global__ __launch_bounds__(kStreamThreads) void stream_join_kernel(StreamArgs 
     }
 }
 
-template <typename T, int DK, int RT, bool PAGED, bool SPLIT>
+template <typename T, int DK, int RT, bool PAGED, int MODE>
 __global__
 __launch_bounds__(kStreamThreads, DK > 128 || (RT == 2 && DK * sizeof(T) >= 256) ? 1 : 2)
 void stream_fwd_kernel(StreamArgs a) {
-    using W = StreamWave<T, DK, RT, PAGED>;
+    using W = StreamWave<T, DK, RT, PAGED, MODE == kOwn ? 1 : kWaves>;
+    constexpr bool SPLIT = MODE == kPart;
     using S = typename W::S;
     constexpr int STATE = 64 * (4 * S::NO * RT + 2 * RT);  // floats of a wavefront's state
-    __shared__ __attribute__((aligned(16))) float lds[(kWaves - 1) * STATE];
-    const StreamPart at = stream_part(a, blockIdx.x);
+    __shared__ __attribute__((aligned(16))) float lds[MODE == kOwn ? 1 : (kWaves - 1) * STATE];
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    StreamPart at = stream_part(a, blockIdx.x, MODE == kOwn ? (a.row_tiles + kWaves - 1) / kWaves : a.row_tiles);
+    if (MODE == kOwn) {
+        at.rt = at.rt * kWaves + wave;
+        if (at.rt >= a.row_tiles) return;
+    }
     const StreamRange r = stream_range(a, at.b, at.rt, W::ROWS);
     const int steps = (r.blocks + S::NB - 1) / S::NB;
     const int64_t slot = (((int64_t)at.b * a.Hkv + at.hk) * a.row_tiles + at.rt) * a.splits + at.part;
@@ -638,14 +648,13 @@ void stream_fwd_kernel(StreamArgs a) {
         }
         return;
     }
-    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     W w(a, r, at);
-    w.run(at.part * per + wave, min(steps, (at.part + 1) * per));
+    w.run(at.part * per + (MODE == kOwn ? 0 : wave), min(steps, (at.part + 1) * per));
 
     // fold the wavefronts' states into wavefront 0's
 #pragma unroll
     for (int i = 0; i < RT; ++i) w.l[i] = sum4(w.l[i]);
-    if (wave > 0) {
+    if (MODE != kOwn && wave > 0) {
         float* st = lds + (wave - 1) * STATE;
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
@@ -655,14 +664,17 @@ void stream_fwd_kernel(StreamArgs a) {
             st[64 * 4 * S::NO * RT + 64 * (2 * i + 1) + lane] = w.l[i];
         }
     }
-    __syncthreads();
-    if (wave != 0) return;
+    if (MODE != kOwn) {
+        __syncthreads();
+        if (wave != 0) return;
+    }
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
+        float top = w.m[i], sum = w.l[i];
+        if constexpr (MODE != kOwn) {
         float ms[kWaves], ls[kWaves];
         ms[0] = w.m[i];
         ls[0] = w.l[i];
-        float top = w.m[i];
 #pragma unroll
         for (int k = 1; k < kWaves; ++k) {
             const float* st = lds + (k - 1) * STATE + 64 * 4 * S::NO * RT;
@@ -672,7 +684,7 @@ void stream_fwd_kernel(StreamArgs a) {
         }
         const float mu = top == kNegInf ? 0.0f : top;
         const float keep = __builtin_amdgcn_exp2f(w.m[i] - mu);
-        float sum = ls[0] * keep;
+        sum = ls[0] * keep;
 #pragma unroll
         for (int c = 0; c < S::NO; ++c) w.o[i][c] *= keep;
 #pragma unroll
@@ -684,6 +696,7 @@ void stream_fwd_kernel(StreamArgs a) {
                 const f32x4 v = *(const f32x4*)(lds + (k - 1) * STATE + 4 * (64 * (i * S::NO + c) + lane));
                 w.o[i][c] += f * v;
             }
+        }
         }
         // row n, columns 16 VW c + VW (4 g + e) + 0 .. VW - 1
         const int row = at.rt * W::ROWS + 16 * i + w.n;
@@ -715,27 +728,40 @@ void stream_fwd_kernel(StreamArgs a) {
         }
     }
 }
+template <typename T, int DK, int RT, int MODE>
+hipError_t launch_stream_mode(const StreamArgs& a, hipStream_t s) {
+    const int per_head = MODE == kOwn ? (a.row_tiles + kWaves - 1) / kWaves : a.row_tiles * a.splits;
+    const dim3 grid((unsigned)((int64_t)a.B * a.Hkv * per_head)), block(kStreamThreads);
+    if (a.paged) hipLaunchKernelGGL((stream_fwd_kernel<T, DK, RT, true, MODE>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((stream_fwd_kernel<T, DK, RT, false, MODE>), grid, block, 0, s, a);
+    return hipGetLastError();
+}
+
 template <typename T, int DK, int RT>
 hipError_t launch_stream_rt(const StreamArgs& a, hipStream_t s) {
-    const dim3 grid((unsigned)((int64_t)a.B * a.Hkv * a.row_tiles * a.splits)), block(kStreamThreads);
-    if (a.splits > 1) {
-        if (a.paged) hipLaunchKernelGGL((stream_fwd_kernel<T, DK, RT, true, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((stream_fwd_kernel<T, DK, RT, false, true>), grid, block, 0, s, a);
-    } else {
-        if (a.paged) hipLaunchKernelGGL((stream_fwd_kernel<T, DK, RT, true, false>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((stream_fwd_kernel<T, DK, RT, false, false>), grid, block, 0, s, a);
+    if (a.splits == 1) {
+        // Enough tiles for every SIMD's wavefront to have one: nothing to fold.
+        // Without a window the last tiles, whose keys are most, would end alone
+        // (us, a workgroup per tile / a wavefront per tile: f32 D64 B2 H8 N2047
+        // window 512 82 / 64, B4 H16 N4096 window 1024 860 / 734; causal B2 H8
+        // N2048 120 / 177; D128 B1 H8 N2000 window 256, 504 tiles, 43 / 60).
+        if constexpr (RT == 2 || DK == 256 || sizeof(T) == 4)
+            if (a.window > 0 && a.row_tiles >= kWaves && (int64_t)a.B * a.Hkv * a.row_tiles >= 4 * kComputeUnits)
+                return launch_stream_mode<T, DK, RT, kOwn>(a, s);
+        return launch_stream_mode<T, DK, RT, kTile>(a, s);
     }
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.splits == 1) return e;
+    hipError_t e = launch_stream_mode<T, DK, RT, kPart>(a, s);
+    if (e != hipSuccess) return e;
     const int64_t items = (int64_t)a.B * a.Hkv * a.T * a.G * ((a.Dv + 31) / 32);
-    hipLaunchKernelGGL((stream_join_kernel<T>), dim3((unsigned)((items + kWaves - 1) / kWaves)), block, 0, s, a, 16 * RT);
+    hipLaunchKernelGGL((stream_join_kernel<T>), dim3((unsigned)((items + kWaves - 1) / kWaves)), dim3(kStreamThreads), 0,
+                       s, a, 16 * RT);
     return hipGetLastError();
 }
 
 template <typename T>
 hipError_t launch_stream_type(const StreamArgs& a, hipStream_t s) {
     const int dk = stream_kernel_dim(a.D, a.Dv);
-    const bool wide = stream_tile_rows(dk, a.T * a.G) == 32;
+    const bool wide = stream_tile_rows(sizeof(T) == 4 ? DT_F32 : DT_BF16, dk, a.T * a.G) == 32;
     switch (dk) {
         case 64: return wide ? launch_stream_rt<T, 64, 2>(a, s) : launch_stream_rt<T, 64, 1>(a, s);
         case 128: return wide ? launch_stream_rt<T, 128, 2>(a, s) : launch_stream_rt<T, 128, 1>(a, s);
@@ -751,9 +777,14 @@ int stream_kernel_dim(int D, int Dv) {
     return d <= 64 ? 64 : d <= 128 ? 128 : d <= 256 ? 256 : 0;
 }
 
-// 32 rows halve the reads of a tile; at kernel dim 256 their accumulators and
-// two steps of K and V exceed the registers.
-int stream_tile_rows(int kernel_dim, int rows) { return kernel_dim <= 128 && rows > 16 ? 32 : 16; }
+// 32 rows halve what tiles read: bf16 B16 H64/8 D128, 4 tokens, N500-8000 86 us
+// against 109 with 16; f32 187 against 219. At kernel dim 256 their accumulators
+// exceed the registers, and many fp32 rows (prompts) are bound by the products,
+// which two wavefronts of 16 rows per SIMD overlap better: D64 B4 H16 N4096 window
+// 1024 735 us, with 16 rows 671.
+int stream_tile_rows(int dtype, int kernel_dim, int rows) {
+    return kernel_dim > 128 || rows <= 16 || (dtype == DT_F32 && rows > 256) ? 16 : 32;
+}
 
 int stream_step_keys(int dtype, int kernel_dim) { return dtype == DT_F32 && kernel_dim > 64 ? kStreamKeys : 2 * kStreamKeys; }
 

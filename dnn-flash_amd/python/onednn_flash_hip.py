@@ -603,18 +603,18 @@ def qk_score_tile(q, k, *, scale: float | None = None, bias=None, softcap: float
 # cache, writing and copying of its pages. onednn_flash_cache.PagedCache keeps
 # such a cache.
 
-def _launch_on(torch, device, stream, call):
-    """call(stream handle) with `device` current: the library launches on the
-    current device."""
+def _launch(torch, device, stream, entry, *args):
+    """entry(*args, stream handle) with `device` current: the library launches on
+    the current device."""
+    index = device.index
     if stream is None:
-        stream = _raw_stream(torch, device)
-    if device.index is None or device.index == torch.cuda.current_device():
-        rc = call(stream)
+        stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        rc = entry(*args, stream)
     else:
         with torch.cuda.device(device):
-            rc = call(stream)
-    if rc != OFH_SUCCESS:
-        check(rc)
+            rc = entry(*args, stream)
+    return rc
 
 
 def _check_rows(torch, name, t, dims, dtype, device):
@@ -639,11 +639,26 @@ def _axis_strides(name, t):
     """The strides of t's first three axes as the C ABI takes them: those of axes of
     one element, which torch leaves open, as a row's length, and never all zero
     (which would mean a contiguous tensor)."""
-    row = t.shape[3]
-    a, b, c = [stride if size > 1 else row for size, stride in zip(t.shape[:3], t.stride())]
+    s0, s1, s2, row = t.shape
+    a, b, c, _ = t.stride()
+    if s0 == 1:
+        a = row
+    if s1 == 1:
+        b = row
+    if s2 == 1:
+        c = row
     if a == 0 and b == 0 and c == 0:
         raise ValueError(f"{name} must not be one row broadcast over every axis")
     return a, b, c
+
+
+def _is_rows(torch, t, dtype, device):
+    """What _check_rows asks of a 4-axis tensor, in one pass: true only where it
+    would find nothing to report."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device:
+        return False
+    shape, stride = t.shape, t.stride()
+    return len(shape) == 4 and 0 not in shape and min(stride) >= 0 and (stride[3] == 1 or shape[3] == 1)
 
 
 def _check_written(name, t):
@@ -672,7 +687,7 @@ def _check_slopes(torch, slopes, heads, device):
 
 def _check_counts(**values):
     for name, x in values.items():
-        if isinstance(x, bool) or not isinstance(x, int) or x < 0:
+        if type(x) is not int or x < 0:
             raise ValueError(f"{name} must be a non-negative integer")
 
 
@@ -685,15 +700,10 @@ def _check_out(torch, out, shape, dtype, device):
     _check_written("out", out)
 
 
-def _scratch(torch, need, workspace, device):
-    """(address, bytes) of the workspace, and the tensor that holds it."""
-    if workspace is None:
-        if need == 0:
-            return None, 0, None
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous() or workspace.device != device:
+def _check_workspace(torch, workspace, device):
+    if not isinstance(workspace, torch.Tensor) or workspace.dtype != torch.uint8 or not workspace.is_contiguous() \
+            or workspace.device != device:
         raise ValueError(f"workspace must be a contiguous uint8 tensor on {device}")
-    return workspace.data_ptr(), workspace.numel(), workspace
 
 
 def _workspace_need(query, p) -> int:
@@ -721,13 +731,17 @@ def window_attention(q, k, v, *, window: int = 0, sink_tokens: int = 0, scale: f
     The workspace (partial rows of calls with few query rows) is taken from
     torch's allocator unless given."""
     torch = _torch()
-    _check_rows(torch, "q", q, 4, None, None)
-    dev = q.device
-    _check_rows(torch, "k", k, 4, q.dtype, dev)
-    _check_rows(torch, "v", v, 4, q.dtype, dev)
+    if not (isinstance(q, torch.Tensor) and q.dtype in _DTYPE_CODES and q.device.type == "cuda"
+            and _is_rows(torch, q, q.dtype, q.device) and _is_rows(torch, k, q.dtype, q.device)
+            and _is_rows(torch, v, q.dtype, q.device)):
+        _check_rows(torch, "q", q, 4, None, None)
+        _check_rows(torch, "k", k, 4, q.dtype, q.device)
+        _check_rows(torch, "v", v, 4, q.dtype, q.device)
+    dev, dtype = q.device, q.dtype
     B, H, M, D = q.shape
-    Hkv, N, Dv = k.shape[1], k.shape[2], v.shape[3]
-    if k.shape[0] != B or k.shape[3] != D or v.shape[:3] != k.shape[:3] or H % Hkv != 0:
+    _, Hkv, N, _ = k.shape
+    Dv = v.shape[3]
+    if k.shape != (B, Hkv, N, D) or v.shape != (B, Hkv, N, Dv) or H % Hkv != 0:
         raise ValueError("k must be [B, Hkv, N, D] and v [B, Hkv, N, Dv] with H a multiple of Hkv")
     _check_counts(window=window, sink_tokens=sink_tokens, query_offset=query_offset, max_key_splits=max_key_splits)
     if lengths is not None:
@@ -735,24 +749,35 @@ def window_attention(q, k, v, *, window: int = 0, sink_tokens: int = 0, scale: f
     if alibi_slopes is not None:
         _check_slopes(torch, alibi_slopes, H, dev)
     if out is None:
-        if out_dtype not in (None, q.dtype, torch.float32):
+        if out_dtype not in (None, dtype, torch.float32):
             raise ValueError("out_dtype must be the dtype of q or float32")
-        out = torch.empty((B, H, M, Dv), dtype=q.dtype if out_dtype is None else out_dtype, device=dev)
+        out = torch.empty((B, H, M, Dv), dtype=dtype if out_dtype is None else out_dtype, device=dev)
+        o_strides = (0, 0, 0)  # contiguous
     else:
-        _check_out(torch, out, (B, H, M, Dv), q.dtype, dev)
+        _check_out(torch, out, (B, H, M, Dv), dtype, dev)
         if out_dtype is not None and out.dtype != out_dtype:
             raise ValueError("out and out_dtype disagree")
+        o_strides = _axis_strides("out", out)
     p = _FlatWindowParams(
-        ctypes.sizeof(WindowParams), B, H, Hkv, M, N, D, Dv, _DTYPE_CODES[q.dtype], _DTYPE_CODES[out.dtype],
-        *_axis_strides("q", q), *_axis_strides("k", k), *_axis_strides("v", v), *_axis_strides("out", out),
+        ctypes.sizeof(WindowParams), B, H, Hkv, M, N, D, Dv, _DTYPE_CODES[dtype], _DTYPE_CODES[out.dtype],
+        *_axis_strides("q", q), *_axis_strides("k", k), *_axis_strides("v", v), *o_strides,
         (1.0 / math.sqrt(D)) if scale is None else scale, softcap,
         None if alibi_slopes is None else alibi_slopes.data_ptr(), window, sink_tokens, query_offset,
         None if lengths is None else lengths.data_ptr(), max_key_splits)
     L = lib()
-    need = _workspace_need(L.ofh_window_attention_workspace_bytes, p) if workspace is None else 0
-    ws, ws_bytes, _held = _scratch(torch, need, workspace, dev)
-    _launch_on(torch, dev, stream, lambda s: L.ofh_window_attention_fwd(
-        ctypes.addressof(p), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ws, ws_bytes, s))
+    args = (ctypes.addressof(p), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr())
+    if workspace is not None:
+        _check_workspace(torch, workspace, dev)
+        rc = _launch(torch, dev, stream, L.ofh_window_attention_fwd, *args, workspace.data_ptr(), workspace.numel())
+    else:
+        # most calls need none: first with an empty one, which a call that does refuses
+        rc = _launch(torch, dev, stream, L.ofh_window_attention_fwd, *args, out.data_ptr(), 0)
+        if rc == OFH_ERROR_WORKSPACE_TOO_SMALL:
+            need = _workspace_need(L.ofh_window_attention_workspace_bytes, p)
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+            rc = _launch(torch, dev, stream, L.ofh_window_attention_fwd, *args, workspace.data_ptr(), need)
+    if rc != OFH_SUCCESS:
+        check(rc)
     return out
 
 
@@ -830,23 +855,27 @@ class PagedAttention:
     def __call__(self, q, *, out=None, workspace=None, stream=None):
         """q: [B,H,T,D] in the cache's dtype. Returns out, [B,H,T,Dv]."""
         torch, dev = self._torch, self._device
-        if not (isinstance(q, torch.Tensor) and tuple(q.shape) == self._q_shape and q.dtype == self._dtype
-                and q.device == dev):
-            raise ValueError(f"q must be a {self._dtype} tensor of shape {self._q_shape} on {dev}")
-        qs = q.stride()
-        if (qs[3] != 1 and q.shape[3] > 1) or min(qs) < 0:
-            raise ValueError("q: last axis must be contiguous and strides non-negative")
+        if not (_is_rows(torch, q, self._dtype, dev) and q.shape == self._q_shape):
+            raise ValueError(f"q must be a {self._dtype} tensor of shape {self._q_shape} on {dev}, its last axis "
+                             "contiguous and strides non-negative")
         p = PagedParams.from_buffer_copy(self._params)  # (its own: calls may run on several threads)
-        p.q_strides[:] = _axis_strides("q", q)
+        if not q.is_contiguous():
+            p.q_strides[:] = _axis_strides("q", q)
         if out is None:
             out = torch.empty(self._out_shape, dtype=self._out_dtype, device=dev)
         else:
             _check_out(torch, out, self._out_shape, self._dtype, dev)
             p.out_dtype = _DTYPE_CODES[out.dtype]
             p.o_strides[:] = _axis_strides("out", out)
-        ws, ws_bytes, _held = _scratch(torch, self._need, workspace, dev)
-        _launch_on(torch, dev, stream, lambda s: self._fwd(
-            ctypes.addressof(p), q.data_ptr(), *self._ptrs, out.data_ptr(), ws, ws_bytes, s))
+        if workspace is not None:
+            _check_workspace(torch, workspace, dev)
+        elif self._need:
+            workspace = torch.empty(self._need, dtype=torch.uint8, device=dev)
+        ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
+        rc = _launch(torch, dev, stream, self._fwd, ctypes.addressof(p), q.data_ptr(), *self._ptrs, out.data_ptr(), ws,
+                     ws_bytes)
+        if rc != OFH_SUCCESS:
+            check(rc)
         return out
 
 
@@ -904,16 +933,21 @@ class CacheWriter:
         """k: [B,Hkv,T,D], v: [B,Hkv,T,Dv], the (padded) new rows."""
         torch, dev = self._torch, self._device
         B, Hkv, D, Dv = self._row
-        _check_rows(torch, "k", k, 4, self._dtype, dev)
-        _check_rows(torch, "v", v, 4, self._dtype, dev)
+        if not (_is_rows(torch, k, self._dtype, dev) and _is_rows(torch, v, self._dtype, dev)):
+            _check_rows(torch, "k", k, 4, self._dtype, dev)
+            _check_rows(torch, "v", v, 4, self._dtype, dev)
         T = k.shape[2]
-        if tuple(k.shape) != (B, Hkv, T, D) or tuple(v.shape) != (B, Hkv, T, Dv):
+        if k.shape != (B, Hkv, T, D) or v.shape != (B, Hkv, T, Dv):
             raise ValueError(f"k must be {(B, Hkv, 'T', D)} and v {(B, Hkv, 'T', Dv)}")
         p = CacheWriteParams.from_buffer_copy(self._params)
         p.tokens = T
-        p.k_strides[:], p.v_strides[:] = _axis_strides("k", k), _axis_strides("v", v)
-        _launch_on(torch, dev, stream, lambda s: self._write(
-            ctypes.addressof(p), k.data_ptr(), v.data_ptr(), *self._ptrs, s))
+        if not k.is_contiguous():
+            p.k_strides[:] = _axis_strides("k", k)
+        if not v.is_contiguous():
+            p.v_strides[:] = _axis_strides("v", v)
+        rc = _launch(torch, dev, stream, self._write, ctypes.addressof(p), k.data_ptr(), v.data_ptr(), *self._ptrs)
+        if rc != OFH_SUCCESS:
+            check(rc)
 
 
 def cache_write(k, v, k_pages, v_pages, page_table, lengths, *, counts=None, stream=None) -> None:
@@ -932,36 +966,41 @@ def copy_pages(pools, src, dst, *, stream=None) -> None:
     if not pools or not all(isinstance(t, torch.Tensor) for t in pools):
         raise ValueError("pools must be tensors [P, ...]")
     first = pools[0]
-    dev = first.device
-    if first.dim() < 2 or first.numel() == 0 or dev.type != "cuda":
+    shape, strides, dtype, dev = first.shape, first.stride(), first.dtype, first.device
+    if len(shape) < 2 or 0 in shape or dev.type != "cuda":
         raise ValueError("pools must be GPU tensors [P, ...]")
     for t in pools:
-        if t.shape != first.shape or t.dtype != first.dtype or t.device != dev or t.stride() != first.stride():
+        if t.shape != shape or t.dtype != dtype or t.device != dev or t.stride() != strides:
             raise ValueError("pools must share shape, dtype, strides and device")
-    if not first[0].is_contiguous():
-        raise ValueError("pools: pages must be contiguous")
-    size = first.element_size()
-    page = first[0].numel() * size
-    stride = first.stride(0) * size if first.shape[0] > 1 else page
-    if stride < page:
+    page = 1
+    for size, stride in zip(reversed(shape[1:]), reversed(strides[1:])):
+        if size > 1 and stride != page:
+            raise ValueError("pools: pages must be contiguous")
+        page *= size
+    between = strides[0] if shape[0] > 1 else page
+    if between < page:
         raise ValueError("pools: pages must not overlap")
 
     def numbers(name, x):
-        x = torch.as_tensor(x) if isinstance(x, torch.Tensor) else torch.tensor(list(x), dtype=torch.int64)
+        if not isinstance(x, torch.Tensor):
+            x = torch.tensor(list(x), dtype=torch.int64)
         if x.dim() != 1 or x.device.type != "cpu" or x.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{name} must be a row of integers on the host")
-        if x.dtype != torch.int32:
-            if x.numel() and (int(x.min()) < 0 or int(x.max()) >= first.shape[0]):
+        if x.dtype == torch.int64:
+            if x.numel() and (int(x.min()) < 0 or int(x.max()) >= shape[0]):
                 raise ValueError(f"{name}: copied pages must be within the pool")
             x = x.to(torch.int32)
-        return x.contiguous()
+        return x if x.is_contiguous() else x.contiguous()
 
     src, dst = numbers("src", src), numbers("dst", dst)
-    if src.numel() != dst.numel():
+    count, size = src.numel(), first.element_size()
+    if count != dst.numel():
         raise ValueError("src and dst must have the same length")
-    addresses = (ctypes.c_void_p * len(pools))(*(t.data_ptr() for t in pools))
-    _launch_on(torch, dev, stream, lambda s: lib().ofh_cache_copy_pages(
-        addresses, len(pools), first.shape[0], page, stride, src.data_ptr(), dst.data_ptr(), src.numel(), s))
+    addresses = (ctypes.c_void_p * len(pools))(*[t.data_ptr() for t in pools])
+    rc = _launch(torch, dev, stream, lib().ofh_cache_copy_pages, addresses, len(pools), shape[0], page * size,
+                 between * size, src.data_ptr(), dst.data_ptr(), count)
+    if rc != OFH_SUCCESS:
+        check(rc)
 
 
 # Tile heuristic and layout choice of the reference wrapper
