@@ -484,8 +484,9 @@ int ofh_cache_write(const ofh_cache_write_params* p, const void* k, const void* 
         a.elem = elem_size(p->dtype);
         a.k_bytes = (int)p->head_dim * a.elem;
         a.v_bytes = (int)p->value_dim * a.elem;
-        // (below 2^60 by the bounds above and their product's)
-        if ((double)p->batch * (double)p->tokens * (double)p->kv_heads * (double)(a.k_bytes + a.v_bytes) / 2 >= 4294967040.0)
+        // workgroups of a token, with chunks of an element, times tokens
+        const double blocks = std::floor((double)p->kv_heads * (double)(p->head_dim + p->value_dim) * (a.elem / 2) / 256.0) + 1.0;
+        if ((double)p->batch * (double)p->tokens * blocks * 256.0 >= 4294967040.0)
             return unsupported("cache write exceeds the launch range");
         OFH_HIP_CHECK(ofh::launch_cache_write(a, static_cast<hipStream_t>(stream)));
         return OFH_SUCCESS;
@@ -501,7 +502,7 @@ int ofh_cache_copy_pages(void* const* pools, size_t num_pools, size_t num_pages,
             return invalid("pools, src and dst must be non-null");
         const size_t stride = page_stride_bytes != 0 ? page_stride_bytes : page_bytes;
         if (stride < page_bytes) return invalid("pages must not overlap");
-        if (num_pages > (size_t)kMaxOffset || stride > ((size_t)1 << 36))
+        if (num_pages > (size_t)kMaxOffset || stride > ((size_t)1 << 34))
             return unsupported("pages exceed the index range");
         if (page_bytes % 2 != 0 || stride % 2 != 0) return unsupported("pages must be whole 2-byte elements");
         for (size_t i = 0; i < num_pools; ++i) {
@@ -519,21 +520,41 @@ int ofh_cache_copy_pages(void* const* pools, size_t num_pools, size_t num_pages,
             role[(size_t)dst[i]] |= 2;
             if (role[(size_t)dst[i]] & 1) return invalid("a page is both copied from and copied to");
         }
-        // pages past 64 MiB: a launch holds fewer pairs and pools
-        const size_t pairs = stride > ((size_t)64 << 20) ? 1 : ofh::kCopyPairs;
-        const size_t most = stride > ((size_t)64 << 20) ? 1 : stride > ((size_t)1 << 20) ? 4 : ofh::kCopyPools;
-        for (size_t i = 0; i < count; i += pairs)
-            for (size_t j = 0; j < num_pools; j += most) {
-                ofh::CopyPagesArgs a{};
-                a.num_pairs = (int)std::min<size_t>(pairs, count - i);
-                a.num_pools = (int)std::min<size_t>(most, num_pools - j);
-                std::copy(src + i, src + i + a.num_pairs, a.src);
-                std::copy(dst + i, dst + i + a.num_pairs, a.dst);
-                for (int t = 0; t < a.num_pools; ++t) a.pools[t] = static_cast<char*>(pools[j + t]);
-                a.page_stride = (int64_t)stride;
-                a.page_bytes = (int64_t)page_bytes;
+        // A launch has at most 2^32 work items of which 2-byte chunks move 8
+        // bytes each: fewer pairs and pools of pages past 16 MiB, one of both past 2 GiB.
+        const bool wide = num_pages > ((size_t)1 << 16);
+        const size_t most_pools = page_bytes > ((size_t)1 << 31) ? 1 : page_bytes > ((size_t)1 << 24) ? 8 : ofh::kCopyWords / 4;
+        const size_t most_pairs = page_bytes > ((size_t)1 << 24) ? 1 : (size_t)1 << 31;
+        for (size_t j = 0; j < num_pools; j += most_pools) {
+            ofh::CopyPagesArgs a{};
+            a.num_pools = (int)std::min(most_pools, num_pools - j);
+            a.wide = wide ? 1 : 0;
+            a.page_stride = (int64_t)stride;
+            a.page_bytes = (int64_t)page_bytes;
+            for (int t = 0; t < a.num_pools; ++t) {
+                const uint64_t at = reinterpret_cast<uintptr_t>(pools[j + t]);
+                a.words[2 * t] = (uint32_t)at;
+                a.words[2 * t + 1] = (uint32_t)(at >> 32);
+            }
+            uint32_t* pairs = a.words + 2 * a.num_pools;
+            // (a launch of small pages stays within 2^32 work items too)
+            const size_t items = (page_bytes / 8 + 256) * (size_t)a.num_pools;
+            const size_t fit = std::min(most_pairs, std::max<size_t>(1, (((size_t)1 << 32) - 1) / items));
+            const size_t room = std::min(fit, (size_t)(ofh::kCopyWords - 2 * a.num_pools) / (wide ? 2 : 1));
+            for (size_t i = 0; i < count; i += room) {
+                a.num_pairs = (int)std::min(room, count - i);
+                for (int t = 0; t < a.num_pairs; ++t) {
+                    const uint32_t from = (uint32_t)src[i + t], to = (uint32_t)dst[i + t];
+                    if (wide) {
+                        pairs[2 * t] = from;
+                        pairs[2 * t + 1] = to;
+                    } else {
+                        pairs[t] = from | to << 16;
+                    }
+                }
                 OFH_HIP_CHECK(ofh::launch_copy_pages(a, static_cast<hipStream_t>(stream)));
             }
+        }
         return OFH_SUCCESS;
     });
 }

@@ -94,15 +94,15 @@ struct CacheWriteArgs {
 };
 hipError_t launch_cache_write(const CacheWriteArgs& a, hipStream_t s);
 
-// Whole pages src -> dst in several pools of one geometry.
-constexpr int kCopyPairs = 320;
-constexpr int kCopyPools = 128;
+// Whole pages src -> dst in several pools of one geometry. The words of a
+// launch (its arguments hold 4 KB) are the pools' addresses, low word first, then
+// the pairs: a word each, dst above src, or with `wide` (pages past 2^16) two.
+constexpr int kCopyWords = 976;
 struct CopyPagesArgs {
-    char* pools[kCopyPools];
-    int32_t src[kCopyPairs], dst[kCopyPairs];
+    uint32_t words[kCopyWords];
     int64_t page_stride;  // bytes
     int64_t page_bytes;
-    int num_pools, num_pairs;
+    int num_pools, num_pairs, wide;
 };
 hipError_t launch_copy_pages(const CopyPagesArgs& a, hipStream_t s);
 
