@@ -104,6 +104,24 @@ struct WindowWave : Wave32<T, D, MOD_PLAIN, false, WindowTiles<D, KS>::THREADS, 
     __device__ __forceinline__ void softmax_window(int k0, bool mask) {
         float mx = kNegInf;
         const bool raw = !GENERAL && !mask && a.scale_log2 >= 0.0f;  // s holds dot products
+        // At D = 64 the softmax's arithmetic bounds a step: p is taken against the
+        // running max first. A row sum of at most 2^kRescaleSlack proves that the
+        // tile's max would have raised nothing; else the tile is redone with it.
+        if (D <= 64 && raw && __builtin_amdgcn_ballot_w64(m_run == kNegInf) == 0) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int c = 0; c < BN / 16; ++c) {
+#pragma unroll
+                for (int t = 0; t < 8; ++t)
+                    pf[c][t] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[c >> 1][8 * (c & 1) + t], a.scale_log2, -m_run));
+#pragma unroll
+                for (int t = 0; t < 8; t += 2) sum = Dot2<T>::sum2(typename Dot2<T>::v2{pf[c][t], pf[c][t + 1]}, sum);
+            }
+            if (__builtin_amdgcn_ballot_w64(!(sum <= kSumBound)) == 0) {
+                l_run += sum;
+                return;
+            }
+        }
         if (raw) {
 #pragma unroll
             for (int sb = 0; sb < BN / 32; ++sb)
