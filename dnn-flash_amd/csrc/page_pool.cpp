@@ -9,7 +9,6 @@
 #include <limits>
 #include <map>
 #include <mutex>
-#include <new>
 #include <string>
 #include <vector>
 
@@ -50,6 +49,15 @@ int unknown(int64_t sequence) {
     return api_error(OFH_ERROR_INVALID_ARGUMENT, "unknown sequence " + std::to_string(sequence));
 }
 
+// (Where not even the message finds memory, the last one stays.)
+int out_of_memory() {
+    try {
+        return api_error(OFH_ERROR_HIP, "page pool: out of host memory");
+    } catch (...) {
+        return OFH_ERROR_HIP;
+    }
+}
+
 // Runs `body` under the pool's lock; no exception leaves the C ABI.
 template <typename F>
 int guarded(ofh_page_pool* pool, F&& body) {
@@ -57,10 +65,8 @@ int guarded(ofh_page_pool* pool, F&& body) {
     try {
         std::lock_guard<std::mutex> lock(pool->mu);
         return body();
-    } catch (const std::bad_alloc&) {
-        return api_error(OFH_ERROR_HIP, "page pool: out of host memory");
     } catch (...) {
-        return api_error(OFH_ERROR_HIP, "page pool: host error");
+        return out_of_memory();
     }
 }
 
@@ -85,7 +91,7 @@ int ofh_page_pool_create(size_t num_pages, size_t page_size, ofh_page_pool** poo
         for (size_t i = 0; i < num_pages; ++i) p->free[i] = (int32_t)i;  // ascending: a min-heap
     } catch (...) {
         delete p;
-        return api_error(OFH_ERROR_HIP, "page pool: out of host memory");
+        return out_of_memory();
     }
     *pool = p;
     return OFH_SUCCESS;

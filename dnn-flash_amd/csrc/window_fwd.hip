@@ -93,6 +93,17 @@ struct WindowWave : Wave32<T, D, MOD_PLAIN, false, WindowTiles<D, KS>::THREADS, 
         w = wa.window > 0 ? p + 1 - wa.window : 0;
     }
 
+    // K columns of a staged tile past the head dim -> 0: the copies repeat the row's
+    // last chunk there, and an infinity in it times Q's zeros would be a NaN.
+    __device__ __forceinline__ void zero_pad(int stage) {
+        const int lane = threadIdx.x & 63, pos = (64 * this->wave + lane) % L::CPR;
+        if (8 * (pos ^ L::kswz(this->dma_row0)) < a.D) return;
+        constexpr int NW = Tiles::THREADS / 64;
+#pragma unroll
+        for (int u = 0; u < Base::CPT; ++u)
+            *(u32x4*)(smem + stage + 1024 * (this->wave + NW * u) + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
+    }
+
     __device__ __forceinline__ bool sees(int k0) const { return k0 < hi_max && (k0 + BN > lo_min || k0 < sinks); }
     __device__ __forceinline__ bool partly(int k0) const {
         return k0 + BN > hi_min || (k0 < lo_max && k0 + BN > sinks);
@@ -324,6 +335,7 @@ void window_fwd_kernel(WindowArgs wa) {
         w.copy_tile(tile(0), 0);
         wait_vm_loads();
         w.zero_tail(tile(0), 0);
+        if (a.D < D) w.zero_pad(0);
         __syncthreads();
         for (int st = 0; st < steps; ++st) {
             const int stage = (st & 1) * L::STAGE, next = ((st + 1) & 1) * L::STAGE;
@@ -334,7 +346,10 @@ void window_fwd_kernel(WindowArgs wa) {
                 if (w.sees(k0)) w.template step<GENERAL, decltype(seen)::value>(stage, sub, k0);
             }
             wait_vm_loads();
-            if (st + 1 < steps) w.zero_tail(tile(st + 1), next);
+            if (st + 1 < steps) {
+                w.zero_tail(tile(st + 1), next);
+                if (a.D < D) w.zero_pad(next);
+            }
             __syncthreads();
         }
     };

@@ -146,6 +146,8 @@ class PagedCache:
     def extend(self, sequences, tokens) -> "CacheBatch":
         """Room for tokens[i] new tokens in sequences[i], whose K and V the
         batch's write brings."""
+        if not sequences:
+            raise ValueError("a batch needs a sequence")
         self._copy(*self.pool.extend(sequences, tokens))
         return CacheBatch(self, sequences, tokens)
 

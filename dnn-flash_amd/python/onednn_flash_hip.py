@@ -706,6 +706,15 @@ def _check_workspace(torch, workspace, device):
         raise ValueError(f"workspace must be a contiguous uint8 tensor on {device}")
 
 
+def _new_workspace(torch, need, device, stream):
+    """Scratch of one call on `stream` (a handle; None: the current stream). It is
+    freed when the call returns, so it belongs to the stream that uses it."""
+    if stream is None:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+        return torch.empty(need, dtype=torch.uint8, device=device)
+
+
 def _workspace_need(query, p) -> int:
     need = ctypes.c_size_t()
     rc = query(ctypes.addressof(p), ctypes.byref(need))
@@ -774,7 +783,7 @@ def window_attention(q, k, v, *, window: int = 0, sink_tokens: int = 0, scale: f
         rc = _launch(torch, dev, stream, L.ofh_window_attention_fwd, *args, out.data_ptr(), 0)
         if rc == OFH_ERROR_WORKSPACE_TOO_SMALL:
             need = _workspace_need(L.ofh_window_attention_workspace_bytes, p)
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+            workspace = _new_workspace(torch, need, dev, stream)
             rc = _launch(torch, dev, stream, L.ofh_window_attention_fwd, *args, workspace.data_ptr(), need)
     if rc != OFH_SUCCESS:
         check(rc)
@@ -792,6 +801,8 @@ def _check_pool(torch, k_pages, v_pages, page_table, lengths, batch=None):
     if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2 or 0 in page_table.shape:
         raise ValueError("page_table must be an int32 tensor [B, max_pages]")
     _check_ints(torch, "page_table", page_table, tuple(page_table.shape), dev)
+    if page_table.shape[0] > 1 and page_table.stride(0) == 0:  # (a stride of 0 means contiguous rows)
+        raise ValueError("page_table must not be a broadcast tensor")
     _check_ints(torch, "lengths", lengths, (page_table.shape[0],), dev)
 
 
@@ -870,7 +881,7 @@ class PagedAttention:
         if workspace is not None:
             _check_workspace(torch, workspace, dev)
         elif self._need:
-            workspace = torch.empty(self._need, dtype=torch.uint8, device=dev)
+            workspace = _new_workspace(torch, self._need, dev, stream)
         ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
         rc = _launch(torch, dev, stream, self._fwd, ctypes.addressof(p), q.data_ptr(), *self._ptrs, out.data_ptr(), ws,
                      ws_bytes)

@@ -309,7 +309,7 @@ typedef struct ofh_window_params {
     float softcap;        /* 0: off */
     const float* alibi_slopes; /* device [heads] or NULL */
     size_t window;        /* keys that a query sees, itself included; 0: all before it */
-    size_t sink_tokens;   /* first keys that stay visible behind a window */
+    size_t sink_tokens;   /* first keys that stay visible behind a window (0 without one) */
     size_t query_offset;  /* position of query row 0 */
     /* Device int32 [B] or NULL. lengths[b] (taken between 0 and key_tokens) is
      * what sequence b of a padded batch has: keys from there on are not seen,

@@ -101,6 +101,27 @@ def test_window_head_dims(ofh, dt, D, Dv):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+def test_window_many_tiles(ofh, dt, D):
+    """More tiles than the GPU runs at once: 128 rows per workgroup in 16 bits, a
+    tile per wavefront in fp32; with each rule of the scores, and a NaN that half of
+    the rows do not see."""
+    B, H, Hkv, N = 3, 64, 16, 257
+    lengths = [257, 100, 190]
+    check_window(ofh, dt, B, H, Hkv, N, N, D, lengths=lengths, window=90, sink_tokens=70, seed=D)
+    check_window(ofh, dt, B, H, Hkv, N, N, D, window=33, sink_tokens=1, seed=D, slopes=True, softcap=9.0)
+    check_window(ofh, dt, B, H, Hkv, N, N, D, lengths=lengths, seed=D, scale=-0.1)
+    q, k, v = (randn(i, (B, h, N, D), dt) for i, h in ((1, H), (2, Hkv), (3, Hkv)))
+    v2 = v.clone()
+    v2[:, :, 130, 5] = NAN
+    clean, out = (f64(ofh.window_attention(q.cuda(), k.cuda(), t.cuda(), window=60)) for t in (v, v2))
+    sees = np.array([130 <= t < 190 for t in range(N)])
+    assert not np.isfinite(out[:, :, sees, 5]).any()
+    tol = 1e-5 if dt == "f32" else 2.0 ** -6
+    assert np.abs(out[:, :, ~sees] - clean[:, :, ~sees]).max() <= tol * np.abs(clean).max()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("H,Hkv", [(1, 1), (8, 8), (6, 2), (5, 1), (40, 1)])
 def test_window_head_groups(ofh, dt, H, Hkv):
     check_window(ofh, dt, 2, H, Hkv, 45, 45, 64, window=20, sink_tokens=4, seed=H)
@@ -175,6 +196,26 @@ def test_window_hidden_values_do_not_reach_a_row(ofh, dt, D, bad):
             tol = 1e-5 if dt == "f32" else 2.0 ** -6  # the redone products may sum in another order
             assert np.isfinite(out[0, :, ~sees]).all()
             assert np.abs(out[0, :, ~sees] - clean[0, :, ~sees]).max() <= tol * np.abs(clean).max()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D", [24, 40, 80, 136])
+def test_infinite_keys_of_a_padded_head_dim(ofh, dt, D):
+    """A score of -inf through an infinity in the last columns of K is a weight of
+    0, also where the kernel's columns past the head dim repeat them."""
+    H, N = 2, 200
+    q, k, v = (randn(i, (1, h, N, D), dt) for i, h in ((1, H), (2, 1), (3, 1)))
+    q[..., D - 1] = 1.0
+    k[0, 0, 3::7, D - 1] = -math.inf
+    k[0, 0, :2, D - 1] = 0.5
+    for M in (N, 1):  # staged through LDS, and streamed
+        out = f64(ofh.window_attention(q[:, :, N - M:].cuda(), k.cuda(), v.cuda(), query_offset=N - M, window=60, sink_tokens=2))
+        keep = torch.ones(N, dtype=torch.bool)
+        keep[3::7] = False
+        ref = {(0, h, t): attend_row(f64(q[0, h, N - M + t]), f64(torch.nan_to_num(k[0, 0], neginf=0.0)), f64(v[0, 0]),
+                                     N - M + t, N, window=60, sinks=2, dtype=dt, out_dtype=dt,
+                                     hidden=np.flatnonzero(~keep.numpy())) for h in range(H) for t in pick(M, 20, D)}
+        compare(out if isinstance(out, torch.Tensor) else torch.from_numpy(out), ref, dt, f"infinite keys {dt} D{D} M{M}")
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
@@ -522,6 +563,32 @@ def test_other_streams_and_threads(ofh):
         assert all(torch.equal(a, b) for a, b in zip(g, w))
 
 
+def test_a_stream_handle_given(ofh):
+    """Calls on a stream that is not the current one, whose scratch is freed as they
+    return while the stream still has them to run."""
+    F = ofh
+    side = torch.cuda.Stream()
+    kp, vp, table, _, _ = make_cache("bf16", [6000], 2, 128, 128, 16, 4)
+    n = torch.tensor([6000], dtype=torch.int32).cuda()
+    q = randn(4, (1, 8, 1, 128), "bf16").cuda()
+    attend = F.PagedAttention(kp, vp, table, n, heads=8)
+    assert attend.workspace_bytes > 0
+    want = attend(q)
+    k = randn(5, (1, 2, 6000, 128), "bf16").cuda()
+    alone = F.window_attention(q, k, k, query_offset=5999)
+    torch.cuda.synchronize()
+    outs = []
+    torch.cuda._sleep(20_000_000)  # the side stream waits, the host goes on
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        outs.append((attend(q, stream=side.cuda_stream), F.window_attention(q, k, k, query_offset=5999, stream=side.cuda_stream)))
+        for _ in range(8):  # what the current stream allocates now must not be that scratch
+            torch.empty(attend.workspace_bytes, dtype=torch.uint8, device="cuda").fill_(255)
+    torch.cuda.synchronize()
+    for a, b in outs:
+        assert torch.equal(a, want) and torch.equal(b, alone)
+
+
 def test_captured_and_replayed(ofh):
     """Two graphs captured on one stream, replayed in turn with eager calls
     between them and at the same time: each replay is the eager result of the
@@ -625,6 +692,9 @@ def test_python_refusals(ofh):
             (lambda: F.window_attention(q[:, :3], k, k), "multiple of Hkv"),
             (lambda: F.paged_attention(q, pool, pool, table.long(), n), "page_table must be an int32"),
             (lambda: F.paged_attention(q, pool, pool, table, n.repeat(2)), "lengths must be an int32"),
+            (lambda: F.paged_attention(q.repeat(2, 1, 1, 1), pool, pool, table.expand(2, 2), n.repeat(2)), "broadcast"),
+            (lambda: F.cache_write(k.repeat(2, 1, 1, 1), k.repeat(2, 1, 1, 1), pool, pool, table.expand(2, 2), n.repeat(2)),
+             "broadcast"),
             (lambda: F.paged_attention(q[:, :3], pool, pool, table, n), "multiple of the cache's heads"),
             (lambda: F.paged_attention(q.half(), pool, pool, table, n), "q must be a torch.float32"),
             (lambda: F.paged_attention(q, pool, pool[:4], table, n), "k_pages must be"),
