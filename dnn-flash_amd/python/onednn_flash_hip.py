@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parents[1]
@@ -188,8 +189,9 @@ class WindowParams(ctypes.Structure):
     ]
 
 
-class _FlatWindowParams(ctypes.Structure):
-    _fields_ = _flat_fields(WindowParams._fields_)
+# WindowParams as one pack of its fields: a quarter of a Structure's construction
+_pack_window = struct.Struct("@I7Q2i12q2f5Qi0Q")
+assert _pack_window.size == ctypes.sizeof(WindowParams)
 
 
 class PagedParams(ctypes.Structure):
@@ -687,7 +689,7 @@ def _check_slopes(torch, slopes, heads, device):
 
 def _check_counts(**values):
     for name, x in values.items():
-        if type(x) is not int or x < 0:
+        if type(x) is not int or x < 0 or x >= 1 << (31 if name == "max_key_splits" else 63):
             raise ValueError(f"{name} must be a non-negative integer")
 
 
@@ -717,7 +719,7 @@ def _new_workspace(torch, need, device, stream):
 
 def _workspace_need(query, p) -> int:
     need = ctypes.c_size_t()
-    rc = query(ctypes.addressof(p), ctypes.byref(need))
+    rc = query(p if isinstance(p, bytes) else ctypes.addressof(p), ctypes.byref(need))
     if rc != OFH_SUCCESS:
         check(rc)
     return need.value
@@ -752,7 +754,10 @@ def window_attention(q, k, v, *, window: int = 0, sink_tokens: int = 0, scale: f
     Dv = v.shape[3]
     if k.shape != (B, Hkv, N, D) or v.shape != (B, Hkv, N, Dv) or H % Hkv != 0:
         raise ValueError("k must be [B, Hkv, N, D] and v [B, Hkv, N, Dv] with H a multiple of Hkv")
-    _check_counts(window=window, sink_tokens=sink_tokens, query_offset=query_offset, max_key_splits=max_key_splits)
+    if not (type(window) is int is type(sink_tokens) is type(query_offset) is type(max_key_splits)
+            and 0 <= window < 1 << 63 and 0 <= sink_tokens < 1 << 63 and 0 <= query_offset < 1 << 63
+            and 0 <= max_key_splits < 1 << 31):
+        _check_counts(window=window, sink_tokens=sink_tokens, query_offset=query_offset, max_key_splits=max_key_splits)
     if lengths is not None:
         _check_ints(torch, "lengths", lengths, (B,), dev)
     if alibi_slopes is not None:
@@ -767,14 +772,14 @@ def window_attention(q, k, v, *, window: int = 0, sink_tokens: int = 0, scale: f
         if out_dtype is not None and out.dtype != out_dtype:
             raise ValueError("out and out_dtype disagree")
         o_strides = _axis_strides("out", out)
-    p = _FlatWindowParams(
-        ctypes.sizeof(WindowParams), B, H, Hkv, M, N, D, Dv, _DTYPE_CODES[dtype], _DTYPE_CODES[out.dtype],
+    p = _pack_window.pack(
+        _pack_window.size, B, H, Hkv, M, N, D, Dv, _DTYPE_CODES[dtype], _DTYPE_CODES[out.dtype],
         *_axis_strides("q", q), *_axis_strides("k", k), *_axis_strides("v", v), *o_strides,
         (1.0 / math.sqrt(D)) if scale is None else scale, softcap,
-        None if alibi_slopes is None else alibi_slopes.data_ptr(), window, sink_tokens, query_offset,
-        None if lengths is None else lengths.data_ptr(), max_key_splits)
+        0 if alibi_slopes is None else alibi_slopes.data_ptr(), window, sink_tokens, query_offset,
+        0 if lengths is None else lengths.data_ptr(), max_key_splits)
     L = lib()
-    args = (ctypes.addressof(p), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr())
+    args = (p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr())
     if workspace is not None:
         _check_workspace(torch, workspace, dev)
         rc = _launch(torch, dev, stream, L.ofh_window_attention_fwd, *args, workspace.data_ptr(), workspace.numel())
