@@ -189,7 +189,8 @@ int window_args(const ofh_window_params* p, bool check_ptrs, const void* q, cons
         return rc;
     if (p->key_tokens == 0) return invalid("attention dimensions must be non-zero");
     // (positions of whole row tiles are 32-bit)
-    if (p->key_tokens > (size_t)kMaxTokens || p->query_offset + p->query_tokens > (size_t)kMaxTokens)
+    if (p->key_tokens > (size_t)kMaxTokens || p->query_offset > (size_t)kMaxTokens ||
+        p->query_offset + p->query_tokens > (size_t)kMaxTokens)
         return unsupported("attention dimensions exceed the 32-bit index range");
     int64_t qs[3], ks[3], vs[3], os[3];
     resolve_strides(qs, p->q_strides, p->heads, p->query_tokens, p->head_dim);

@@ -100,6 +100,14 @@ def test_paged_refusals(ofh, fields, code, text):
     status(ofh, L.ofh_paged_attention_workspace_bytes(ctypes.addressof(p), ctypes.byref(n)), code, text)
 
 
+def test_window_query_offset_does_not_wrap(ofh):
+    """A position of 2^64 - 5 + 33 wraps to 28: refused for what it is."""
+    lib, need = ofh.lib(), ctypes.c_size_t()
+    p = window(ofh, query_offset=(1 << 64) - 5)
+    status(ofh, lib.ofh_window_attention_workspace_bytes(ctypes.addressof(p), ctypes.byref(need)), 2,
+           "32-bit index range")
+
+
 def test_pointers_are_checked(ofh):
     L = ofh.lib()
     for p, fwd in ((window(ofh), L.ofh_window_attention_fwd), (paged(ofh), L.ofh_paged_attention_fwd)):
