@@ -3,7 +3,11 @@
 //
 // What bounds it: reading K and V once (2 bytes of K and V per product of a
 // row's tile, far below what the matrix cores need). So nothing goes through
-// LDS: with S^T = K Q^T and O^T = V^T P^T
+// LDS. Measured: f16 B1 H32/8 of 131,000 keys D128 95 us, 5.7 TB/s, and 5 us of
+// the join; bf16 B64 H32/8 of 65-4096 keys 119 us, 4.7 TB/s (the longest run on
+// alone); fp32 prompts, bound by the matrix cores instead, B2 H8 N1000-2047 D64
+// window 512 58 us.
+// With S^T = K Q^T and O^T = V^T P^T
 //  * a K fragment (16 keys x 32 columns in 16 bits, 16 x 16 in fp32) is one
 //    16-byte load per lane from the key's row;
 //  * a V row is read 16 bytes per lane with 16 lanes on a row's 128 columns
@@ -104,7 +108,8 @@ __device__ __forceinline__ float sum4(float x) {
 // what rounding P to 16 bits costs, but ten times the rest of an fp32 score's. So
 // fp32 takes Lambert's continued fraction up to |y| = cap, cut where it is right
 // to 2^-37 (z (135135 + 17325 z^2 + 378 z^4 + z^6) / (135135 + 62370 z^2 +
-// 3150 z^4 + 28 z^6)): B2 H8 N1000 D64 cap 30 1.2e-6 off 64 bits through the exponential, 2.8e-7 so (relative, rms).
+// 3150 z^4 + 28 z^6)): B2 H8 N1000 D64 cap 30 is 1.2e-6 off 64 bits through the
+// exponential, 2.8e-7 so (relative, rms).
 __device__ __forceinline__ float cap_tanh16(float y, float cap) {
     const float u = __builtin_amdgcn_exp2f(y * (2.0f * kLog2e / cap));
     return __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(u + 1.0f), cap);
@@ -684,31 +689,31 @@ void stream_fwd_kernel(StreamArgs a) {
     for (int i = 0; i < RT; ++i) {
         float top = w.m[i], sum = w.l[i];
         if constexpr (MODE != kOwn) {
-        float ms[kWaves], ls[kWaves];
-        ms[0] = w.m[i];
-        ls[0] = w.l[i];
+            float ms[kWaves], ls[kWaves];
+            ms[0] = w.m[i];
+            ls[0] = w.l[i];
 #pragma unroll
-        for (int k = 1; k < kWaves; ++k) {
-            const float* st = lds + (k - 1) * STATE + 64 * 4 * S::NO * RT;
-            ms[k] = st[64 * (2 * i) + lane];
-            ls[k] = st[64 * (2 * i + 1) + lane];
-            top = fmaxf(top, ms[k]);
-        }
-        const float mu = top == kNegInf ? 0.0f : top;
-        const float keep = __builtin_amdgcn_exp2f(w.m[i] - mu);
-        sum = ls[0] * keep;
-#pragma unroll
-        for (int c = 0; c < S::NO; ++c) w.o[i][c] *= keep;
-#pragma unroll
-        for (int k = 1; k < kWaves; ++k) {
-            const float f = __builtin_amdgcn_exp2f(ms[k] - mu);
-            sum += f * ls[k];
-#pragma unroll
-            for (int c = 0; c < S::NO; ++c) {
-                const f32x4 v = *(const f32x4*)(lds + (k - 1) * STATE + 4 * (64 * (i * S::NO + c) + lane));
-                w.o[i][c] += f * v;
+            for (int k = 1; k < kWaves; ++k) {
+                const float* st = lds + (k - 1) * STATE + 64 * 4 * S::NO * RT;
+                ms[k] = st[64 * (2 * i) + lane];
+                ls[k] = st[64 * (2 * i + 1) + lane];
+                top = fmaxf(top, ms[k]);
             }
-        }
+            const float mu = top == kNegInf ? 0.0f : top;
+            const float keep = __builtin_amdgcn_exp2f(w.m[i] - mu);
+            sum = ls[0] * keep;
+#pragma unroll
+            for (int c = 0; c < S::NO; ++c) w.o[i][c] *= keep;
+#pragma unroll
+            for (int k = 1; k < kWaves; ++k) {
+                const float f = __builtin_amdgcn_exp2f(ms[k] - mu);
+                sum += f * ls[k];
+#pragma unroll
+                for (int c = 0; c < S::NO; ++c) {
+                    const f32x4 v = *(const f32x4*)(lds + (k - 1) * STATE + 4 * (64 * (i * S::NO + c) + lane));
+                    w.o[i][c] += f * v;
+                }
+            }
         }
         // row n, columns 16 VW c + VW (4 g + e) + 0 .. VW - 1
         const int row = at.rt * W::ROWS + 16 * i + w.n;

@@ -4,10 +4,16 @@
 // A workgroup's rows see the first tokens' tiles and then the tiles from the
 // oldest row's window to the youngest row's diagonal; no other tile is loaded.
 // A wavefront skips the tiles that none of its 32 rows sees and masks element
-// by element only in those that some of its rows see partly. Eight wavefronts
-// take 256 rows, or share the keys of 128 or 64 rows among two or four groups
-// (fold_groups): a workgroup reads its window and its rows' own span, so small
-// windows waste least with few rows, and small calls fill the GPU.
+// by element only in those that some of its rows see partly. Four wavefronts
+// take 128 rows, or share the keys of 64 rows between two groups (fold_groups):
+// a workgroup reads its window and its rows' own span, so small windows waste
+// least with few rows, and small calls fill the GPU.
+//
+// What bounds it: the products and the softmax of a wavefront one after the
+// other (bf16 D128 B4 H32/8 N2048 window 1024, 4 first tokens: 139-157 us by
+// card, 746-658 TFLOP/s; N300-2048 in one batch 104 us, matrix cores 33 % and
+// vector ALUs 40 % of the busy CUs' time, no LDS conflicts). K and V of a window
+// are read once per 128 rows, mostly from L2.
 //
 // Masked tiles: a key that a row does not see has probability 0, which does
 // not hide a NaN or an infinity in its V row from the product: O then holds a
@@ -26,7 +32,7 @@ namespace {
 // keys in compute steps of BN and staged tiles of SN: two stages in at most 64
 // KB, so that two workgroups share a CU and one's start, barriers and stores run
 // beside the other's products (at D = 256 the registers hold one). Measured
-// against eight wavefronts on tiles of 128 keys (us, one box): bf16 D128 B4
+// against eight wavefronts on tiles of 128 keys (us, one card): bf16 D128 B4
 // H32/8 N2048 window 1024 140 / 151, B2 N4096 window 128 72 / 84, B1 H32 N4096
 // without one 148 / 155, N16384 window 4096 983 / 949.
 template <int D, int KS>
