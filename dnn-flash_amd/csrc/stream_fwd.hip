@@ -45,6 +45,7 @@
 
 #include "flash_wave32.h"
 #include "serving_kernels.h"
+#include "serving_softcap.h"
 
 namespace ofh {
 namespace {
@@ -102,23 +103,6 @@ __device__ __forceinline__ float max4(float x) {  // over the four lane groups o
 __device__ __forceinline__ float sum4(float x) {
     x += __shfl_xor(x, 16);
     return x + __shfl_xor(x, 32);
-}
-// cap tanh(y / cap). Through the exponential, cap (1 - 2 / (2^u + 1)) with u =
-// 2 log2(e) y / cap, its error is a few 2^-24 cap however small y is: less than
-// what rounding P to 16 bits costs, but ten times the rest of an fp32 score's. So
-// fp32 takes Lambert's continued fraction up to |y| = cap, cut where it is right
-// to 2^-37 (z (135135 + 17325 z^2 + 378 z^4 + z^6) / (135135 + 62370 z^2 +
-// 3150 z^4 + 28 z^6)): B2 H8 N1000 D64 cap 30 is 1.2e-6 off 64 bits through the
-// exponential, 2.8e-7 so (relative, rms).
-__device__ __forceinline__ float cap_tanh16(float y, float cap) {
-    const float u = __builtin_amdgcn_exp2f(y * (2.0f * kLog2e / cap));
-    return __builtin_fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(u + 1.0f), cap);
-}
-__device__ __forceinline__ float cap_tanh(float y, float cap) {
-    const float z = y / cap, w = z * z;
-    const float num = y * __builtin_fmaf(__builtin_fmaf(w + 378.0f, w, 17325.0f), w, 135135.0f);
-    const float den = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(28.0f, w, 3150.0f), w, 62370.0f), w, 135135.0f);
-    return __builtin_fabsf(z) <= 1.0f ? num / den : cap_tanh16(y, cap);
 }
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
@@ -440,7 +424,16 @@ struct StreamWave {
         for (int j = 0; j < S::NB; ++j)
 #pragma unroll
             for (int t = 0; t < 4; ++t) x[4 * j + t] = sc[j][t] * to_log2;
-        if (a.alibi != nullptr || a.softcap > 0.0f) {
+        if (!F32 && a.softcap > kCapExp) {
+#pragma unroll
+            for (int j = 0; j < S::NB; ++j)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    float y = sc[j][t] * a.scale;
+                    if (a.alibi != nullptr) y = __builtin_fmaf(slope[i], (float)(key0[j] + 4 * g + t - pos[i]), y);
+                    x[4 * j + t] = cap_tanh_wide(y, a.softcap) * kLog2e;
+                }
+        } else if (a.alibi != nullptr || a.softcap > 0.0f) {
 #pragma unroll
             for (int j = 0; j < S::NB; ++j)
 #pragma unroll

@@ -24,6 +24,7 @@
 
 #include "flash_wave32.h"
 #include "serving_kernels.h"
+#include "serving_softcap.h"
 
 namespace ofh {
 namespace {
@@ -45,6 +46,11 @@ struct WindowTiles {
     static constexpr int WAVES_PER_SIMD = D <= 128 ? 2 : 1;
     static_assert(SB % KS == 0, "the groups share a tile's steps");
 };
+
+// What happens to a score: the scale alone; ALiBi, a soft-cap of at most kCapExp, or
+// both; a wider cap, with or without ALiBi (in one kernel the two forms of the cap
+// held more registers: f16 H32 N4096 D64 cap 50 186 us, with a kernel each 182).
+enum WindowScores { kScoresPlain, kScoresMod, kScoresWideCap };
 
 template <bool B>
 struct Bool {
@@ -117,8 +123,9 @@ struct WindowWave : Wave32<T, D, MOD_PLAIN, false, WindowTiles<D, KS>::THREADS, 
     __device__ __forceinline__ bool seen(int key) const { return key < hi && (key >= lo || key < sinks); }
 
     // Online softmax of the scores in s (keys k0 ..): as Wave32::softmax.
-    template <bool GENERAL>
+    template <WindowScores SCORES>
     __device__ __forceinline__ void softmax_window(int k0, bool mask) {
+        constexpr bool GENERAL = SCORES != kScoresPlain;
         float mx = kNegInf;
         const bool raw = !GENERAL && !mask && a.scale_log2 >= 0.0f;  // s holds dot products
         // At D = 64 the softmax's arithmetic bounds a step: p is taken against the
@@ -147,7 +154,7 @@ struct WindowWave : Wave32<T, D, MOD_PLAIN, false, WindowTiles<D, KS>::THREADS, 
             mx *= a.scale_log2;
         } else {
             if (GENERAL) {
-                const bool cap = a.softcap > 0.0f;
+                const bool cap = SCORES == kScoresMod && a.softcap > 0.0f;
                 const float c = cap ? 2.0f * kLog2e * a.inv_softcap : kLog2e;
                 const float sl = slope * c, base = sl * (float)(k0 + 8 * g - pos), c_s = a.scale * c;
                 const float cap_hi = a.softcap * kLog2e;
@@ -162,6 +169,13 @@ struct WindowWave : Wave32<T, D, MOD_PLAIN, false, WindowTiles<D, KS>::THREADS, 
                                                cap_hi);
                         s[sb][e] = u;
                     }
+                if (SCORES == kScoresWideCap) {
+                    const float cap_log2 = a.softcap * kLog2e;
+#pragma unroll
+                    for (int sb = 0; sb < BN / 32; ++sb)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) s[sb][e] = cap_tanh_wide(s[sb][e], cap_log2);
+                }
             } else {
 #pragma unroll
                 for (int sb = 0; sb < BN / 32; ++sb) s[sb] *= a.scale_log2;
@@ -270,13 +284,13 @@ struct WindowWave : Wave32<T, D, MOD_PLAIN, false, WindowTiles<D, KS>::THREADS, 
     }
 
     // SEEN: partly masked tiles are added key by key.
-    template <bool GENERAL, bool SEEN>
+    template <WindowScores SCORES, bool SEEN>
     __device__ __forceinline__ void step(int stage, int sub, int k0) {
         const bool mask = partly(k0);
         __builtin_amdgcn_s_setprio(1);
         this->qk(stage, sub);
         __builtin_amdgcn_s_setprio(0);
-        softmax_window<GENERAL>(k0, mask);
+        softmax_window<SCORES>(k0, mask);
         if (SEEN && mask) {
             pv_seen(stage, sub, k0);
             return;
@@ -310,7 +324,7 @@ __device__ __forceinline__ void window_work(const WindowArgs& wa, int id, int& b
     qt = nqt - 1 - t;
 }
 
-template <typename T, int D, int KS, bool GENERAL>
+template <typename T, int D, int KS, WindowScores SCORES>
 __global__ __launch_bounds__((WindowTiles<D, KS>::THREADS), (WindowTiles<D, KS>::WAVES_PER_SIMD))
 void window_fwd_kernel(WindowArgs wa) {
     using W = WindowWave<T, D, KS>;
@@ -349,7 +363,7 @@ void window_fwd_kernel(WindowArgs wa) {
 #pragma unroll
             for (int i = 0; i < SB / KS; ++i) {
                 const int sub = i * KS + kg, k0 = tile(st) * SN + sub * W::BN;
-                if (w.sees(k0)) w.template step<GENERAL, decltype(seen)::value>(stage, sub, k0);
+                if (w.sees(k0)) w.template step<SCORES, decltype(seen)::value>(stage, sub, k0);
             }
             wait_vm_loads();
             if (st + 1 < steps) {
@@ -373,10 +387,12 @@ void window_fwd_kernel(WindowArgs wa) {
 template <typename T, int D, int KS>
 hipError_t launch_window_groups(const WindowArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)a.f.B * a.f.H * a.f.num_q_tiles)), block(WindowTiles<D, KS>::THREADS);
-    if (a.f.alibi != nullptr || a.f.softcap > 0.0f)
-        hipLaunchKernelGGL((window_fwd_kernel<T, D, KS, true>), grid, block, 0, s, a);
+    if (a.f.softcap > kCapExp)
+        hipLaunchKernelGGL((window_fwd_kernel<T, D, KS, kScoresWideCap>), grid, block, 0, s, a);
+    else if (a.f.alibi != nullptr || a.f.softcap > 0.0f)
+        hipLaunchKernelGGL((window_fwd_kernel<T, D, KS, kScoresMod>), grid, block, 0, s, a);
     else
-        hipLaunchKernelGGL((window_fwd_kernel<T, D, KS, false>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((window_fwd_kernel<T, D, KS, kScoresPlain>), grid, block, 0, s, a);
     return hipGetLastError();
 }
 template <typename T, int D>

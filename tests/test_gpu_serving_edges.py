@@ -87,3 +87,63 @@ def test_padding_rows_of_prompts(ofh, dt, H, Hkv, options, bad):
                                                length, window=options.get("window", 0),
                                                sinks=options.get("sink_tokens", 0), dtype=dt, out_dtype=dt)
     compare(out, rows, dt, f"padded prompts {dt} H{H}/{Hkv} {options}")
+
+
+# --- soft-caps far from the scores --------------------------------------------
+
+def capped_row(q, k, v, position, scale, slope, cap, dt):
+    """The row of attend_row with a soft-cap, and its bound where the cap's error goes
+    by the score's size instead of the cap's: 16 u |y| (of z = y / cap, its square,
+    the fraction's two polynomials and their quotient, each a rounding or two, and past
+    |z| = 1 a few u cap < 1.4 u |y|)."""
+    u = 2.0 ** -24
+    j = np.arange(position + 1)
+    k, v = k[j], v[j]
+    bias = slope * (j - position)
+    y = (k @ q) * scale + bias
+    err = q.size * u * (np.abs(k) @ np.abs(q)) * scale + 6 * u * (np.abs(y) + np.abs(bias)) + 16 * u * np.abs(y)
+    cap = float(np.float32(cap))
+    x = cap * np.tanh(y / cap)
+    err += 2 * u * (np.abs(x) + abs(x.max()) + 8)
+    w = np.exp(x - x.max())
+    w /= w.sum()
+    o = w @ v
+    half = {"f32": 0.0, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[dt]
+    e = err + 2 * u + half
+    bound = (w * e) @ np.abs(v - o) / (1 - e.max()) + (j.size + 8) * u * (w @ np.abs(v) + np.abs(o))
+    return o, bound + 1e-30
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("scale,cap", [(0.125, 257.0), (8.0, 300.0), (0.125, 3e4), (0.125, 1e9), (0.125, 3e38), (8.0, 1e6)])
+def test_large_soft_caps(ofh, dt, slopes, scale, cap):
+    """Caps far past the scores leave them as they are, in every kernel."""
+    H, N, D = 4, 150, 64
+    q, k, v = (randn(i, (1, h, N, D), dt) for i, h in ((1, H), (2, 1), (3, 1)))
+    alibi = 2.0 ** -torch.arange(1.0, H + 1)
+    given = alibi.cuda() if slopes else None
+    options = dict(scale=scale, softcap=cap, alibi_slopes=given, out_dtype=torch.float32)
+    table = torch.arange(10, dtype=torch.int32)[None].cuda()
+    pools = [torch.nn.functional.pad(t, (0, 0, 0, 160 - N)).view(10, 1, 16, D).cuda() for t in (k[0, 0], v[0, 0])]
+    n = torch.tensor([N], dtype=torch.int32).cuda()
+    for M, out in [(N, ofh.window_attention(q.cuda(), k.cuda(), v.cuda(), **options)),
+                   (1, ofh.window_attention(q[:, :, N - 1:].cuda(), k.cuda(), v.cuda(), query_offset=N - 1, **options)),
+                   (3, ofh.paged_attention(q[:, :, N - 3:].cuda(), *pools, table, n, **options))]:
+        rows = {(0, h, t): capped_row(f64(q[0, h, N - M + t]), f64(k[0, 0]), f64(v[0, 0]), N - M + t, scale,
+                                      float(alibi[h]) if slopes else 0.0, cap, dt)
+                for h in range(H) for t in sorted({0, M // 3, M // 2, M - 1})}
+        compare(out, rows, dt, f"cap {cap} {dt} scale {scale} M{M}")
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D", [48, 128, 256])
+@pytest.mark.parametrize("B,H,N", [(1, 2, 150), (8, 16, 300)])
+def test_large_soft_caps_by_head_dim(ofh, dt, D, B, H, N):
+    """Every head dim's kernels, with 64 and with 128 rows per workgroup."""
+    q, k, v = (randn(i, (B, h, N, D), dt) for i, h in ((1, H), (2, 1), (3, 1)))
+    scale, cap = 1.0 / math.sqrt(D), 1e5
+    out = ofh.window_attention(q.cuda(), k.cuda(), v.cuda(), softcap=cap, out_dtype=torch.float32)
+    rows = {(b, h, t): capped_row(f64(q[b, h, t]), f64(k[b, 0]), f64(v[b, 0]), t, scale, 0.0, cap, dt)
+            for b in {0, B - 1} for h in {0, H - 1} for t in (0, 63, N - 1)}
+    compare(out, rows, dt, f"cap {cap} {dt} B{B} H{H} N{N} D{D}")
