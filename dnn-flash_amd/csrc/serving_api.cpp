@@ -87,6 +87,10 @@ int check_common(size_t batch, size_t heads, size_t kv_heads, size_t tokens, siz
     return OFH_SUCCESS;
 }
 
+// The cap as the kernels take it. Their 2 log2(e) / cap has no value for a cap
+// near 2^-126, and scores within 2^-40 of 0 have the same weights in 32 bits.
+float kernel_softcap(float softcap) { return softcap > 0.0f ? std::max(softcap, 0x1p-40f) : 0.0f; }
+
 size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Split of a row tile's keys over workgroups. The lengths are on the device, so
@@ -215,7 +219,7 @@ int window_args(const ofh_window_params* p, bool check_ptrs, const void* q, cons
     a.window = (int)p->window;
     a.sinks = (int)p->sink_tokens;
     a.scale = p->scale;
-    a.softcap = p->softcap;
+    a.softcap = kernel_softcap(p->softcap);
     a.alibi = p->alibi_slopes;
     a.out_f32 = p->out_dtype == OFH_DTYPE_F32;
     return OFH_SUCCESS;
@@ -355,7 +359,7 @@ int paged_args(const ofh_paged_params* p, bool check_ptrs, const void* q, const 
     a.window = (int)p->window;
     a.sinks = (int)p->sink_tokens;
     a.scale = p->scale;
-    a.softcap = p->softcap;
+    a.softcap = kernel_softcap(p->softcap);
     a.alibi = p->alibi_slopes;
     a.out_f32 = p->out_dtype == OFH_DTYPE_F32;
     return OFH_SUCCESS;

@@ -147,3 +147,19 @@ def test_large_soft_caps_by_head_dim(ofh, dt, D, B, H, N):
     rows = {(b, h, t): capped_row(f64(q[b, h, t]), f64(k[b, 0]), f64(v[b, 0]), t, scale, 0.0, cap, dt)
             for b in {0, B - 1} for h in {0, H - 1} for t in (0, 63, N - 1)}
     compare(out, rows, dt, f"cap {cap} {dt} B{B} H{H} N{N} D{D}")
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("cap", [1e-45, 1e-39, 1e-30, 1e-13])
+def test_tiny_soft_caps(ofh, dt, cap):
+    """Caps next to zero leave every score next to zero: the mean of the values that
+    are seen, also where a score is exactly 0 and the cap is subnormal."""
+    H, N, D = 4, 150, 64
+    q, k, v = (randn(i, (1, h, N, D), dt) for i, h in ((1, H), (2, 1), (3, 1)))
+    k[0, 0, ::5] = 0.0
+    for M in (N, 1):
+        out = ofh.window_attention(q[:, :, N - M:].cuda(), k.cuda(), v.cuda(), query_offset=N - M, softcap=cap,
+                                   out_dtype=torch.float32)
+        rows = {(0, h, t): capped_row(f64(q[0, h, N - M + t]), f64(k[0, 0]), f64(v[0, 0]), N - M + t, 0.125, 0.0,
+                                      max(cap, 1e-30), dt) for h in range(H) for t in sorted({0, M // 2, M - 1})}
+        compare(out, rows, dt, f"cap {cap} {dt} M{M}")
