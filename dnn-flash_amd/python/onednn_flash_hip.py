@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 import struct
 from pathlib import Path
 
@@ -971,6 +972,30 @@ def cache_write(k, v, k_pages, v_pages, page_table, lengths, *, counts=None, str
     CacheWriter(k_pages, v_pages, page_table, lengths, counts=counts)(k, v, stream=stream)
 
 
+def _page_numbers(torch, name, x, pages):
+    """x, a row of integers on the host, as contiguous int32."""
+    if not isinstance(x, torch.Tensor):
+        try:
+            x = list(x)
+            if set(map(type, x)) - {int}:  # integers of other kinds, but no truth values
+                if any("bool" in str(getattr(i, "dtype", type(i))) for i in x):
+                    raise TypeError
+                x = [operator.index(i) for i in x]
+        except TypeError:
+            raise ValueError(f"{name} must be a row of integers on the host") from None
+        try:
+            x = torch.tensor(x, dtype=torch.int64)
+        except (OverflowError, RuntimeError, ValueError):  # past 64 bits
+            raise ValueError(f"{name}: copied pages must be within the pool") from None
+    if x.dim() != 1 or x.device.type != "cpu" or x.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be a row of integers on the host")
+    if x.dtype == torch.int64:
+        if x.numel() and (int(x.min()) < 0 or int(x.max()) >= pages):
+            raise ValueError(f"{name}: copied pages must be within the pool")
+        x = x.to(torch.int32)
+    return x if x.is_contiguous() else x.contiguous()
+
+
 def copy_pages(pools, src, dst, *, stream=None) -> None:
     """Copies pages src[i] -> dst[i] of every pool. pools: device tensors
     [P, ...] of one shape and dtype whose pages are contiguous; src, dst: page
@@ -997,18 +1022,7 @@ def copy_pages(pools, src, dst, *, stream=None) -> None:
     if between < page:
         raise ValueError("pools: pages must not overlap")
 
-    def numbers(name, x):
-        if not isinstance(x, torch.Tensor):
-            x = torch.tensor(list(x), dtype=torch.int64)
-        if x.dim() != 1 or x.device.type != "cpu" or x.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"{name} must be a row of integers on the host")
-        if x.dtype == torch.int64:
-            if x.numel() and (int(x.min()) < 0 or int(x.max()) >= shape[0]):
-                raise ValueError(f"{name}: copied pages must be within the pool")
-            x = x.to(torch.int32)
-        return x if x.is_contiguous() else x.contiguous()
-
-    src, dst = numbers("src", src), numbers("dst", dst)
+    src, dst = _page_numbers(torch, "src", src, shape[0]), _page_numbers(torch, "dst", dst, shape[0])
     count, size = src.numel(), first.element_size()
     if count != dst.numel():
         raise ValueError("src and dst must have the same length")

@@ -163,3 +163,31 @@ def test_tiny_soft_caps(ofh, dt, cap):
         rows = {(0, h, t): capped_row(f64(q[0, h, N - M + t]), f64(k[0, 0]), f64(v[0, 0]), N - M + t, 0.125, 0.0,
                                       max(cap, 1e-30), dt) for h in range(H) for t in sorted({0, M // 2, M - 1})}
         compare(out, rows, dt, f"cap {cap} {dt} M{M}")
+
+
+# --- page numbers ------------------------------------------------------------
+
+@pytest.mark.parametrize("numbers", [[1.5], [1.0, 2.0], [True], [False, 1], ["1"], [None], np.array([1.0]), torch.tensor([1.5]),
+                                     torch.tensor([True])])
+def test_page_numbers_are_integers(ofh, numbers):
+    """What is no integer is refused, not rounded to a page; nothing is copied."""
+    pool = torch.arange(8.0 * 16, device="cuda").view(8, 16)
+    before = pool.clone()
+    other = [5, 6][:len(numbers)]
+    for src, dst in ((numbers, other), (other, numbers)):
+        with pytest.raises(ValueError, match="integers"):
+            ofh.copy_pages([pool], src, dst)
+    assert torch.equal(pool, before)
+
+
+@pytest.mark.parametrize("numbers", [[1, 2], (1, 2), range(1, 3), np.array([1, 2]), [np.int32(1), np.int64(2)],
+                                     torch.tensor([1, 2]), torch.tensor([1, 2], dtype=torch.int32),
+                                     [torch.tensor(1), torch.tensor(2)]])
+def test_page_numbers_of_every_integer_kind(ofh, numbers):
+    pool = torch.arange(8.0 * 16, device="cuda").view(8, 16)
+    want = pool.clone()
+    want[5:7] = want[1:3]
+    ofh.copy_pages([pool], numbers, [5, 6])
+    assert torch.equal(pool, want)
+    with pytest.raises(ValueError, match="within the pool"):
+        ofh.copy_pages([pool], [1 << 70], [1])
