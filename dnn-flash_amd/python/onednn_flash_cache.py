@@ -27,6 +27,23 @@ _I64 = ctypes.c_int64
 _SZ = ctypes.c_size_t
 
 
+def _fit(name, x, kind):
+    """x as a C integer (ctypes itself drops the bits that do not fit)."""
+    c = kind(x)
+    if c.value != x:
+        raise ValueError(f"{name} is out of range")
+    return c
+
+
+def _row(name, xs, kind):
+    """A C array of the integers xs, of one element at least."""
+    xs = list(xs)
+    row = (kind * max(len(xs), 1))(*xs)
+    if any(a != b for a, b in zip(row, xs)):
+        raise ValueError(f"{name} are out of range")
+    return row
+
+
 class PagePool:
     """Which sequences hold which of num_pages pages of page_size tokens."""
 
@@ -37,7 +54,8 @@ class PagePool:
         self.num_pages, self.page_size = num_pages, page_size
         self._lib = F.lib()
         handle = ctypes.c_void_p()
-        F.check(self._lib.ofh_page_pool_create(num_pages, page_size, ctypes.byref(handle)))
+        F.check(self._lib.ofh_page_pool_create(_fit("num_pages", num_pages, _SZ), _fit("page_size", page_size, _SZ),
+                                               ctypes.byref(handle)))
         self._handle = handle
         weakref.finalize(self, self._lib.ofh_page_pool_destroy, handle)
 
@@ -55,24 +73,25 @@ class PagePool:
         if len(tokens) != n or any(isinstance(t, bool) or int(t) != t or t < 0 for t in tokens):
             raise ValueError("tokens must be a non-negative integer per sequence")
         src, dst, copies = (_I32 * max(n, 1))(), (_I32 * max(n, 1))(), _SZ()
-        F.check(self._lib.ofh_page_pool_extend(self._handle, (_I64 * max(n, 1))(*sequences), (_SZ * max(n, 1))(*tokens),
-                                               n, src, dst, ctypes.byref(copies)))
+        F.check(self._lib.ofh_page_pool_extend(self._handle, _row("sequences", sequences, _I64),
+                                               _row("tokens", tokens, _SZ), n, src, dst, ctypes.byref(copies)))
         return list(src[:copies.value]), list(dst[:copies.value])
 
     def fork(self, sequence: int) -> int:
         """A new sequence with the same tokens."""
         child = _I64()
-        F.check(self._lib.ofh_page_pool_fork(self._handle, sequence, ctypes.byref(child)))
+        F.check(self._lib.ofh_page_pool_fork(self._handle, _fit("sequence", sequence, _I64), ctypes.byref(child)))
         return child.value
 
     def truncate(self, sequence: int, length: int) -> None:
         """Drops the tokens of a sequence from `length` on."""
         if length < 0:
             raise ValueError("length must be non-negative")
-        F.check(self._lib.ofh_page_pool_truncate(self._handle, sequence, length))
+        F.check(self._lib.ofh_page_pool_truncate(self._handle, _fit("sequence", sequence, _I64),
+                                                 _fit("length", length, _SZ)))
 
     def free(self, sequence: int) -> None:
-        F.check(self._lib.ofh_page_pool_free(self._handle, sequence))
+        F.check(self._lib.ofh_page_pool_free(self._handle, _fit("sequence", sequence, _I64)))
 
     def compact(self, most: int | None = None) -> tuple[list[int], list[int]]:
         """Moves used pages (at most `most`) to the lowest numbers. Returns the
@@ -87,8 +106,11 @@ class PagePool:
     def table(self, sequences, max_pages: int) -> tuple[list[list[int]], list[int]]:
         """Page table rows (unused entries -1) and lengths."""
         n = len(sequences)
+        if max_pages < 0:
+            raise ValueError("max_pages must be non-negative")
         rows, lengths = (_I32 * max(n * max_pages, 1))(), (_I32 * max(n, 1))()
-        F.check(self._lib.ofh_page_pool_table(self._handle, (_I64 * max(n, 1))(*sequences), n, rows, max_pages, lengths))
+        F.check(self._lib.ofh_page_pool_table(self._handle, _row("sequences", sequences, _I64), n, rows,
+                                              _fit("max_pages", max_pages, _SZ), lengths))
         return [list(rows[i * max_pages:(i + 1) * max_pages]) for i in range(n)], list(lengths[:n])
 
     @property
@@ -99,7 +121,7 @@ class PagePool:
 
     def length(self, sequence: int) -> int:
         n = _SZ()
-        F.check(self._lib.ofh_page_pool_length(self._handle, sequence, ctypes.byref(n)))
+        F.check(self._lib.ofh_page_pool_length(self._handle, _fit("sequence", sequence, _I64), ctypes.byref(n)))
         return n.value
 
 
