@@ -181,6 +181,7 @@ class CacheBatch:
     def __init__(self, cache: PagedCache, sequences, tokens):
         torch = cache._torch
         self.cache = cache
+        self._fewest = min(tokens)
         size = cache.pool.page_size
         longest = max(cache.pool.length(s) for s in sequences)
         rows, lengths = cache.pool.table(sequences, max(1, -(-longest // size)))
@@ -195,6 +196,12 @@ class CacheBatch:
                       counts=self.counts)
 
     def attend(self, layer: int, q, **options):
-        """q: [B,H,T,D], the last T tokens of each sequence; options as paged_attention."""
+        """q: [B,H,T,D], the last T of the batch's new tokens of each sequence; options as
+        paged_attention. A sequence with fewer than T new tokens is refused: rows
+        laid out as write takes them, from the front, would be attended at positions
+        from the back (such batches go in parts of one T, or prompts through
+        window_attention with the batch's lengths)."""
+        if q.dim() == 4 and q.shape[2] > self._fewest:
+            raise ValueError(f"q has {q.shape[2]} tokens per sequence, the batch {self._fewest} new ones for some")
         return F.paged_attention(q, self.cache.k_pages[layer], self.cache.v_pages[layer], self.page_table,
                                  self.lengths, **options)

@@ -191,3 +191,31 @@ def test_page_numbers_of_every_integer_kind(ofh, numbers):
     assert torch.equal(pool, want)
     with pytest.raises(ValueError, match="within the pool"):
         ofh.copy_pages([pool], [1 << 70], [1])
+
+
+# --- a batch with uneven numbers of new tokens ----------------------------------
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_uneven_batches_by_their_last_tokens(ofh, dt):
+    """write takes the rows of each sequence from the front; attend the last tokens
+    that every sequence has, and no more."""
+    import onednn_flash_cache as C
+    H, D, counts = 4, 64, [5, 2, 3]
+    cache = C.PagedCache(layers=1, num_pages=12, page_size=16, kv_heads=1, head_dim=D, dtype=TYPES[dt])
+    seqs = [cache.add() for _ in counts]
+    first = cache.extend(seqs, [17, 17, 17])
+    old = [randn(i, (3, 1, 17, D), dt) for i in (1, 2)]
+    first.write(0, *(t.cuda() for t in old))
+    batch = cache.extend(seqs, counts)
+    new = [randn(i, (3, 1, 5, D), dt) for i in (3, 4)]
+    batch.write(0, *(t.cuda() for t in new))
+    q = randn(5, (3, H, 2, D), dt)
+    rows = {}
+    for b, n in enumerate(counts):
+        k, v = (f64(torch.cat([o[b, 0], t[b, 0, :n]])) for o, t in zip(old, new))
+        for h in range(H):
+            for t in range(2):
+                rows[b, h, t] = attend_row(f64(q[b, h, t]), k, v, 17 + n - 2 + t, 17 + n, dtype=dt, out_dtype=dt)
+    compare(batch.attend(0, q.cuda()), rows, dt, f"uneven batch {dt}")
+    with pytest.raises(ValueError, match="q has 5 tokens"):
+        batch.attend(0, randn(5, (3, H, 5, D), dt).cuda())
