@@ -181,7 +181,7 @@ class CacheBatch:
     def __init__(self, cache: PagedCache, sequences, tokens):
         torch = cache._torch
         self.cache = cache
-        self._fewest = min(tokens)
+        self._fewest, self._most = min(tokens), max(tokens)
         size = cache.pool.page_size
         longest = max(cache.pool.length(s) for s in sequences)
         rows, lengths = cache.pool.table(sequences, max(1, -(-longest // size)))
@@ -192,6 +192,8 @@ class CacheBatch:
 
     def write(self, layer: int, k, v) -> None:
         """k: [B,Hkv,T,D], v: [B,Hkv,T,Dv]; the first tokens[i] rows of each sequence."""
+        if k.dim() == 4 and k.shape[2] < self._most:  # (their places would keep what the pages held)
+            raise ValueError(f"k has {k.shape[2]} tokens per sequence, the batch {self._most} new ones")
         F.cache_write(k, v, self.cache.k_pages[layer], self.cache.v_pages[layer], self.page_table, self.lengths,
                       counts=self.counts)
 

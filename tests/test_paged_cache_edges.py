@@ -27,3 +27,18 @@ def test_queries_of_a_batch_with_uneven_counts():
         batch.attend(0, torch.zeros(2, 4, 1, 8))
     with pytest.raises(ValueError, match="GPU tensor"):
         c.extend([a, b], [3, 3]).attend(0, torch.zeros(2, 4, 3, 8))
+
+
+def test_rows_missing_from_a_write():
+    """A write that has fewer rows than the batch made room for would fill the last
+    places and leave the others as they were."""
+    c = cache()
+    a, b = c.add(), c.add()
+    batch = c.extend([a, b], [3, 1])
+    for T in (1, 2):
+        rows = torch.zeros(2, 2, T, 8)
+        with pytest.raises(ValueError, match=f"k has {T} tokens per sequence, the batch 3 new"):
+            batch.write(0, rows, rows)
+    rows = torch.zeros(2, 2, 4, 8)
+    with pytest.raises(ValueError, match="GPU tensor"):  # padded: to the kernel's own checks
+        batch.write(0, rows, rows)
