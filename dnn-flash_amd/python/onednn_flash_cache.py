@@ -135,6 +135,8 @@ class PagedCache:
         import torch
         self._torch = torch
         self.pool = PagePool(num_pages, page_size)
+        if page_size < 16 or page_size & (page_size - 1):  # (what the kernels read and write)
+            raise ValueError("page_size must be a power of two, 16 or more")
         dtype = torch.bfloat16 if dtype is None else dtype
         shape = (layers, num_pages, kv_heads, page_size)
         # (zeros: what a page holds past its tokens is never seen, but a program may look)

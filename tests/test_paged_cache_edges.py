@@ -42,3 +42,10 @@ def test_rows_missing_from_a_write():
     rows = torch.zeros(2, 2, 4, 8)
     with pytest.raises(ValueError, match="GPU tensor"):  # padded: to the kernel's own checks
         batch.write(0, rows, rows)
+
+
+@pytest.mark.parametrize("size", [1, 8, 24, 48])
+def test_page_sizes_that_no_kernel_takes(size):
+    with pytest.raises(ValueError, match="power of two, 16 or more"):
+        cache(page_size=size)
+    assert cache(page_size=64).pool.page_size == 64
