@@ -710,11 +710,13 @@ def _check_workspace(torch, workspace, device):
 
 
 def _new_workspace(torch, need, device, stream):
-    """Scratch of one call on `stream` (a handle; None: the current stream). It is
-    freed when the call returns, so it belongs to the stream that uses it."""
+    """Scratch of one call on `stream` (a handle or a torch stream; None: the current
+    one). It is freed when the call returns, so it belongs to the stream that uses it."""
     if stream is None:
         return torch.empty(need, dtype=torch.uint8, device=device)
-    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    with torch.cuda.stream(stream):
         return torch.empty(need, dtype=torch.uint8, device=device)
 
 

@@ -219,3 +219,26 @@ def test_uneven_batches_by_their_last_tokens(ofh, dt):
     compare(batch.attend(0, q.cuda()), rows, dt, f"uneven batch {dt}")
     with pytest.raises(ValueError, match="q has 5 tokens"):
         batch.attend(0, randn(5, (3, H, 5, D), dt).cuda())
+
+
+# --- streams -------------------------------------------------------------------
+
+def test_a_torch_stream_given(ofh):
+    """A torch stream in place of its handle, also for calls that take scratch on it."""
+    side = torch.cuda.Stream()
+    q = randn(1, (1, 8, 1, 128), "bf16").cuda()
+    k = randn(2, (1, 2, 6000, 128), "bf16").cuda()
+    pools = k.view(2, 375, 16, 128).transpose(0, 1).contiguous()
+    table = torch.arange(375, dtype=torch.int32)[None].cuda()
+    n = torch.tensor([6000], dtype=torch.int32).cuda()
+    attend = ofh.PagedAttention(pools, pools, table, n, heads=8)
+    assert attend.workspace_bytes > 0
+    want = ofh.window_attention(q, k, k, query_offset=5999), attend(q)
+    row, pool = randn(3, (1, 2, 1, 128), "bf16").cuda(), pools.clone()
+    torch.cuda.synchronize()
+    got = ofh.window_attention(q, k, k, query_offset=5999, stream=side), attend(q, stream=side)
+    ofh.cache_write(row, row, pool, pool, table, n, stream=side)
+    ofh.copy_pages([pool], [374], [0], stream=side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(pool[374, :, 15], row[0, :, 0]) and torch.equal(pool[0], pool[374])
