@@ -703,10 +703,13 @@ def _check_out(torch, out, shape, dtype, device):
     _check_written("out", out)
 
 
-def _check_workspace(torch, workspace, device):
+def _given_workspace(torch, workspace, out):
+    """Address and bytes of a caller's workspace. An empty one has no address, which
+    would mean the library's scratch: out's stands for it, with no bytes."""
     if not isinstance(workspace, torch.Tensor) or workspace.dtype != torch.uint8 or not workspace.is_contiguous() \
-            or workspace.device != device:
-        raise ValueError(f"workspace must be a contiguous uint8 tensor on {device}")
+            or workspace.device != out.device:
+        raise ValueError(f"workspace must be a contiguous uint8 tensor on {out.device}")
+    return workspace.data_ptr() or out.data_ptr(), workspace.numel()
 
 
 def _new_workspace(torch, need, device, stream):
@@ -784,8 +787,7 @@ def window_attention(q, k, v, *, window: int = 0, sink_tokens: int = 0, scale: f
     L = lib()
     args = (p, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr())
     if workspace is not None:
-        _check_workspace(torch, workspace, dev)
-        rc = _launch(torch, dev, stream, L.ofh_window_attention_fwd, *args, workspace.data_ptr(), workspace.numel())
+        rc = _launch(torch, dev, stream, L.ofh_window_attention_fwd, *args, *_given_workspace(torch, workspace, out))
     else:
         # most calls need none: first with an empty one, which a call that does refuses
         rc = _launch(torch, dev, stream, L.ofh_window_attention_fwd, *args, out.data_ptr(), 0)
@@ -886,11 +888,12 @@ class PagedAttention:
             _check_out(torch, out, self._out_shape, self._dtype, dev)
             p.out_dtype = _DTYPE_CODES[out.dtype]
             p.o_strides[:] = _axis_strides("out", out)
+        ws, ws_bytes = None, 0
         if workspace is not None:
-            _check_workspace(torch, workspace, dev)
+            ws, ws_bytes = _given_workspace(torch, workspace, out)
         elif self._need:
             workspace = _new_workspace(torch, self._need, dev, stream)
-        ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
+            ws, ws_bytes = workspace.data_ptr(), self._need
         rc = _launch(torch, dev, stream, self._fwd, ctypes.addressof(p), q.data_ptr(), *self._ptrs, out.data_ptr(), ws,
                      ws_bytes)
         if rc != OFH_SUCCESS:

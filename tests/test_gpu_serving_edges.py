@@ -242,3 +242,23 @@ def test_a_torch_stream_given(ofh):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert torch.equal(pool[374, :, 15], row[0, :, 0]) and torch.equal(pool[0], pool[374])
+
+
+# --- workspaces ------------------------------------------------------------------
+
+def test_an_empty_workspace_is_none_of_the_librarys(ofh):
+    """A given workspace is the one that a call uses: an empty one is refused where
+    scratch is needed, and does where it is not."""
+    q = randn(1, (1, 8, 1, 128), "bf16").cuda()
+    k = randn(2, (1, 2, 6000, 128), "bf16").cuda()
+    pools = k.view(2, 375, 16, 128).transpose(0, 1).contiguous()
+    table = torch.arange(375, dtype=torch.int32)[None].cuda()
+    n = torch.tensor([6000], dtype=torch.int32).cuda()
+    empty = torch.empty(0, dtype=torch.uint8, device="cuda")
+    for call in (lambda **o: ofh.window_attention(q, k, k, query_offset=5999, **o),
+                 lambda **o: ofh.paged_attention(q, pools, pools, table, n, **o)):
+        with pytest.raises(ofh.OfhError) as e:
+            call(workspace=empty)
+        assert e.value.code == ofh.OFH_ERROR_WORKSPACE_TOO_SMALL
+        assert torch.equal(call(workspace=empty, max_key_splits=1), call(max_key_splits=1))
+        assert torch.equal(call(workspace=torch.empty(1 << 24, dtype=torch.uint8, device="cuda")), call())
