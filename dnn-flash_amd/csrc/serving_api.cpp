@@ -108,9 +108,9 @@ struct Split {
 // N4000 4 parts 31.6, 16 36.0; D256 B4 H16/4 N20000 16 parts 65, 32 71; two per CU
 // pay off with long parts: f32 D128 B8 H16 N2000-8000 2 parts 140, 4 133, D64 B16
 // H16 N2000-8000 1 part 82, 2 75, but B32 N100-600 1 part 15.4, 2 20.1. Parts of a
-// step per wavefront (4): one sequence of 1001 keys 10.6, of 8 steps 11.8, of 16
-// 14.7; with less than four such parts in all the join costs more than they save:
-// B4 N300 split 11.6, unsplit 10.1.
+// step per wavefront (4): one sequence of 1001 keys 12.5, of 8 steps 12.7, of 16
+// 16.3; with less than four such parts in all the join costs more than they save:
+// B4 N300 split 12.8, unsplit 9.8.
 Split plan_split(const ofh::StreamArgs& a, int dtype, int max_key_splits) {
     Split s{};
     const int dk = ofh::stream_kernel_dim(a.D, a.Dv);

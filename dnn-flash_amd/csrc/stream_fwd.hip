@@ -6,7 +6,7 @@
 // LDS. Measured: f16 B1 H32/8 of 131,000 keys D128 95 us, 5.7 TB/s, and 5 us of
 // the join; bf16 B64 H32/8 of 65-4096 keys 119 us, 4.7 TB/s (the longest run on
 // alone); fp32 prompts, bound by the matrix cores instead, B2 H8 N1000-2047 D64
-// window 512 58 us.
+// window 512 56 us.
 // With S^T = K Q^T and O^T = V^T P^T
 //  * a K fragment (16 keys x 32 columns in 16 bits, 16 x 16 in fp32) is one
 //    16-byte load per lane from the key's row;
@@ -135,9 +135,9 @@ __device__ __forceinline__ StreamRange stream_range(const StreamArgs& a, int b, 
         r.sink_blocks = min((min(a.sinks, end) + kStreamKeys - 1) / kStreamKeys, nb);
         r.first_block = max(r.first_block, r.sink_blocks);
     }
-    // A tile of padding rows alone takes no step: its P are 0, which a NaN or an
-    // infinity in V would turn into one (and fp32 B8 H8 N275-2048 D64 355 -> 210 us
-    // without the masked work, window 512 145 -> 126).
+    // A tile of padding rows alone takes no step. Its probabilities would be 0, and 0
+    // times a NaN or an infinity in V is a NaN; and it would read and multiply for
+    // nothing (fp32 B8 H8 N275-2048 D64 355 us, this 210; window 512 145, 126).
     const bool padding = !a.positions_from_end && a.lengths != nullptr && r.first_pos + r.t0 >= r.length;
     r.blocks = padding ? 0 : r.sink_blocks + max(0, nb - r.first_block);
     return r;
@@ -757,8 +757,11 @@ hipError_t launch_stream_rt(const StreamArgs& a, hipStream_t s) {
         // Enough tiles for every SIMD's wavefront to have one: nothing to fold.
         // Without a window the last tiles, whose keys are most, would end alone
         // (us, a workgroup per tile / a wavefront per tile: f32 D64 B2 H8 N2047
-        // window 512 82 / 64, B4 H16 N4096 window 1024 860 / 734; causal B2 H8
-        // N2048 120 / 177; D128 B1 H8 N2000 window 256, 504 tiles, 43 / 60).
+        // window 512 69 / 59, B4 H16 N4096 window 1024 737 / 673; causal B2 H8 N2048
+        // 110 / 177; 1024 tiles, B1 H8 N2047 window 512, 37 / 32; 500 tiles, N1000
+        // window 256, 16 / 20, D128 B1 H4 N2000 26 / 37. A padded batch
+        // has fewer tiles with work, which is not known here: B2 H8 N1000-2047
+        // window 512 51 / 56, B8 N275-2048 148 / 126).
         if constexpr (RT == 2 || DK == 256 || sizeof(T) == 4)
             if (a.window > 0 && a.row_tiles >= kWaves && (int64_t)a.B * a.Hkv * a.row_tiles >= 4 * kComputeUnits)
                 return launch_stream_mode<T, DK, RT, kOwn>(a, s);
@@ -795,7 +798,7 @@ int stream_kernel_dim(int D, int Dv) {
 // against 109 with 16; f32 187 against 219. At kernel dim 256 their accumulators
 // exceed the registers, and many fp32 rows (prompts) are bound by the products,
 // which two wavefronts of 16 rows per SIMD overlap better: D64 B4 H16 N4096 window
-// 1024 735 us, with 16 rows 671.
+// 1024 707 us, with 16 rows 673.
 int stream_tile_rows(int dtype, int kernel_dim, int rows) {
     return kernel_dim > 128 || rows <= 16 || (dtype == DT_F32 && rows > 256) ? 16 : 32;
 }

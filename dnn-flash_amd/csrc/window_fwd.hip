@@ -11,7 +11,7 @@
 //
 // What bounds it: the products and the softmax of a wavefront one after the
 // other (bf16 D128 B4 H32/8 N2048 window 1024, 4 first tokens: 139-157 us by
-// card, 746-658 TFLOP/s; N300-2048 in one batch 104 us, matrix cores 33 % and
+// card, 746-658 TFLOP/s; N300-2048 in one batch 104 us, matrix cores 34 % and
 // vector ALUs 40 % of the busy CUs' time, no LDS conflicts). K and V of a window
 // are read once per 128 rows, mostly from L2.
 //
