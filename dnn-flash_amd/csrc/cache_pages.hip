@@ -70,13 +70,33 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(CacheWriteAr
         if (to[i] >= 0 && chunk < chunks) *(C*)(dst + to[i]) = x[i];
 }
 
+// The widest chunk that every address allows.
+int write_chunk(const CacheWriteArgs& a) {
+    const int64_t strides = a.k_sb | a.k_sh | a.k_st | a.v_sb | a.v_sh | a.v_st | a.kp_sp | a.kp_sh | a.kp_st |
+                            a.vp_sp | a.vp_sh | a.vp_st;
+    const uint64_t all = (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.k_pages | (uintptr_t)a.v_pages |
+                         (uint64_t)(strides * a.elem) | (uint64_t)a.k_bytes | (uint64_t)a.v_bytes;
+    return all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : all % 4 == 0 ? 4 : 2;
+}
+
+// Workgroups of a call, and whether each takes four tokens (0: past what a launch holds).
+int64_t write_grid(const CacheWriteArgs& a, bool& many) {
+    const int w = write_chunk(a);
+    const int64_t tokens = (int64_t)a.B * a.T, chunks = (int64_t)a.Hkv * (a.k_bytes / w + a.v_bytes / w);
+    const int64_t blocks = (chunks + kCacheThreads - 1) / kCacheThreads;
+    // (chunks of a token, tokens and workgroups are 32-bit in the kernel)
+    if (chunks >= ((int64_t)1 << 31) || tokens >= ((int64_t)1 << 32)) return 0;
+    many = tokens * blocks >= 16 * kComputeUnits;
+    const int64_t wgs = (many ? (tokens + 3) / 4 : tokens) * blocks;
+    return grid_fits(wgs, kCacheThreads) ? wgs : 0;
+}
+
 template <int W>
 hipError_t launch_write(const CacheWriteArgs& a, hipStream_t s) {
     const int kc = a.k_bytes / W, vc = a.v_bytes / W;
-    const int64_t tokens = (int64_t)a.B * a.T, blocks = ((int64_t)a.Hkv * (kc + vc) + kCacheThreads - 1) / kCacheThreads;
-    const bool many = tokens * blocks >= 16 * kComputeUnits;
-    const int64_t wgs = (many ? (tokens + 3) / 4 : tokens) * blocks;
-    if (!grid_fits(wgs, kCacheThreads) || tokens >= ((int64_t)1 << 32)) return hipErrorInvalidValue;
+    bool many = false;
+    const int64_t wgs = write_grid(a, many);
+    if (wgs == 0) return hipErrorInvalidValue;
     if (many) hipLaunchKernelGGL((cache_write_kernel<W, 4>), dim3((unsigned)wgs), dim3(kCacheThreads), 0, s, a, kc, vc);
     else hipLaunchKernelGGL((cache_write_kernel<W, 1>), dim3((unsigned)wgs), dim3(kCacheThreads), 0, s, a, kc, vc);
     return hipGetLastError();
@@ -126,15 +146,18 @@ hipError_t launch_copy(const CopyPagesArgs& a, hipStream_t s) {
 
 }  // namespace
 
+bool cache_write_fits(const CacheWriteArgs& a) {
+    bool many = false;
+    return write_grid(a, many) > 0;
+}
+
 hipError_t launch_cache_write(const CacheWriteArgs& a, hipStream_t s) {
-    const int64_t strides = a.k_sb | a.k_sh | a.k_st | a.v_sb | a.v_sh | a.v_st | a.kp_sp | a.kp_sh | a.kp_st |
-                            a.vp_sp | a.vp_sh | a.vp_st;
-    const uint64_t all = (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.k_pages | (uintptr_t)a.v_pages |
-                         (uint64_t)(strides * a.elem) | (uint64_t)a.k_bytes | (uint64_t)a.v_bytes;
-    if (all % 16 == 0) return launch_write<16>(a, s);
-    if (all % 8 == 0) return launch_write<8>(a, s);
-    if (all % 4 == 0) return launch_write<4>(a, s);
-    return launch_write<2>(a, s);
+    switch (write_chunk(a)) {
+        case 16: return launch_write<16>(a, s);
+        case 8: return launch_write<8>(a, s);
+        case 4: return launch_write<4>(a, s);
+        default: return launch_write<2>(a, s);
+    }
 }
 
 hipError_t launch_copy_pages(const CopyPagesArgs& a, hipStream_t s) {

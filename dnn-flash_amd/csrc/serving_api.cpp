@@ -489,9 +489,7 @@ int ofh_cache_write(const ofh_cache_write_params* p, const void* k, const void* 
         a.elem = elem_size(p->dtype);
         a.k_bytes = (int)p->head_dim * a.elem;
         a.v_bytes = (int)p->value_dim * a.elem;
-        // workgroups of a token, with chunks of an element, times tokens
-        const double blocks = std::floor((double)p->kv_heads * (double)(p->head_dim + p->value_dim) * (a.elem / 2) / 256.0) + 1.0;
-        if ((double)p->batch * (double)p->tokens * blocks * 256.0 >= 4294967040.0)
+        if (!ofh::cache_write_fits(a))
             return unsupported("cache write exceeds the launch range");
         OFH_HIP_CHECK(ofh::launch_cache_write(a, static_cast<hipStream_t>(stream)));
         return OFH_SUCCESS;

@@ -92,6 +92,7 @@ struct CacheWriteArgs {
     int k_bytes, v_bytes;  // bytes of a K and a V row
     int elem;              // bytes of an element
 };
+bool cache_write_fits(const CacheWriteArgs& a);  // in one launch
 hipError_t launch_cache_write(const CacheWriteArgs& a, hipStream_t s);
 
 // Whole pages src -> dst in several pools of one geometry. The words of a

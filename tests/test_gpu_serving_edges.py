@@ -262,3 +262,22 @@ def test_an_empty_workspace_is_none_of_the_librarys(ofh):
         assert e.value.code == ofh.OFH_ERROR_WORKSPACE_TOO_SMALL
         assert torch.equal(call(workspace=empty, max_key_splits=1), call(max_key_splits=1))
         assert torch.equal(call(workspace=torch.empty(1 << 24, dtype=torch.uint8, device="cuda")), call())
+
+
+# --- many tokens in one write ------------------------------------------------------
+
+def test_writes_of_half_a_million_tokens(ofh):
+    """32 prompts of 16384 tokens and 32 heads: as many work items as 16-byte chunks
+    need, which a launch holds. (One sequence's rows stand for all of them, and only
+    the last pages of two sequences have a place.)"""
+    B, H, T, D, page = 32, 32, 16384, 128, 16
+    k = randn(1, (1, H, T, D), "bf16").cuda()
+    v = randn(2, (1, H, T, D), "bf16").cuda()
+    pools = [torch.full((3, H, page, D), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    table = torch.full((B, T // page), -1, dtype=torch.int32)
+    table[0, -1], table[B - 1, -1] = 2, 0
+    n = torch.full((B,), T, dtype=torch.int32).cuda()
+    ofh.cache_write(k.expand(B, H, T, D), v.expand(B, H, T, D), *pools, table.cuda(), n)
+    for rows, pool in ((k, pools[0]), (v, pools[1])):
+        last = rows[0, :, T - page:]
+        assert torch.equal(pool[2], last) and torch.equal(pool[0], last) and bool((pool[1] == 7.0).all())
