@@ -95,6 +95,45 @@ struct CacheWriteArgs {
 bool cache_write_fits(const CacheWriteArgs& a);  // in one launch
 hipError_t launch_cache_write(const CacheWriteArgs& a, hipStream_t s);
 
+// Rotary positions. The first R columns of a row are R / 2 pairs, (i, i + R / 2)
+// or interleaved (2 i, 2 i + 1); pair i turns by position freq[i] radians.
+struct Rotation {
+    const double* freq;
+    int R, interleaved;
+    float magnitude;
+    int transpose;  // turn back
+};
+constexpr int kRotaryMaxDim = 1024;  // of a head
+
+struct RotaryArgs {
+    const void* x;
+    void* o;
+    int64_t x_sb, x_sh, x_st;  // batch, head, token
+    int64_t o_sb, o_sh, o_st;
+    int B, H, T, D;
+    Rotation r;
+    // position of token (b, t): positions[b pos_sb + t], or lengths[b] - T + t, or offset + t
+    const int32_t* positions;
+    int64_t pos_sb;
+    const int32_t* lengths;
+    int64_t offset;
+};
+bool rotary_fits(const RotaryArgs& a, int dtype);  // in one launch
+hipError_t launch_rotary(const RotaryArgs& a, int dtype, hipStream_t s);
+
+// New rows into pages with K turned on the way, and Q turned into q_out (H 0: no Q).
+struct CacheAppendArgs {
+    CacheWriteArgs w;
+    const void* q;
+    void* q_out;
+    int64_t q_sb, q_sh, q_st;
+    int64_t o_sb, o_sh, o_st;
+    int H, D, Dv;
+    Rotation r;
+};
+bool cache_append_fits(const CacheAppendArgs& a, int dtype);
+hipError_t launch_cache_append(const CacheAppendArgs& a, int dtype, hipStream_t s);
+
 // Whole pages src -> dst in several pools of one geometry. The words of a
 // launch (its arguments hold 4 KB) are the pools' addresses, low word first, then
 // the pairs: a word each, dst above src, or with `wide` (pages past 2^16) two.

@@ -6,9 +6,10 @@ GPU. A decode step of a program that serves sequences:
 
     cache = PagedCache(layers=L, num_pages=P, page_size=16, kv_heads=8, head_dim=128)
     seqs = [cache.add() for _ in prompts]
+    rotary = F.Rotary(128)
     batch = cache.extend(seqs, [1] * len(seqs))       # room for one token each
     for layer in range(L):
-        batch.write(layer, k, v)                      # [B,Hkv,1,D]
+        q = batch.append(layer, k, v, rotary, q)      # [B,Hkv,1,D]; turned by their positions
         out = batch.attend(layer, q)                  # [B,H,1,D]
 
 `fork` shares pages until one of the sequences grows; `free` and `truncate`
@@ -192,12 +193,22 @@ class CacheBatch:
         self.lengths = torch.tensor(lengths, dtype=torch.int32, device=device)
         self.counts = torch.tensor(list(tokens), dtype=torch.int32, device=device)
 
-    def write(self, layer: int, k, v) -> None:
-        """k: [B,Hkv,T,D], v: [B,Hkv,T,Dv]; the first tokens[i] rows of each sequence."""
+    def _check_tokens(self, k) -> None:
         if k.dim() == 4 and k.shape[2] < self._most:  # (their places would keep what the pages held)
             raise ValueError(f"k has {k.shape[2]} tokens per sequence, the batch {self._most} new ones")
+
+    def write(self, layer: int, k, v) -> None:
+        """k: [B,Hkv,T,D], v: [B,Hkv,T,Dv]; the first tokens[i] rows of each sequence."""
+        self._check_tokens(k)
         F.cache_write(k, v, self.cache.k_pages[layer], self.cache.v_pages[layer], self.page_table, self.lengths,
                       counts=self.counts)
+
+    def append(self, layer: int, k, v, rotary, q=None):
+        """`write` with K turned by `rotary` (a Rotary) on the way. Returns q
+        [B,H,T,D], the queries of the same tokens, turned too (None without)."""
+        self._check_tokens(k)
+        return F.cache_append(k, v, self.cache.k_pages[layer], self.cache.v_pages[layer], self.page_table, self.lengths,
+                              rotary, q=q, counts=self.counts)
 
     def attend(self, layer: int, q, **options):
         """q: [B,H,T,D], the last T of the batch's new tokens of each sequence; options as

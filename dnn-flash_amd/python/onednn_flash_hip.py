@@ -53,6 +53,10 @@ EXPORTED_SYMBOLS = (
     "ofh_paged_attention_fwd",
     "ofh_cache_write_params_init",
     "ofh_cache_write",
+    "ofh_rotary_params_init",
+    "ofh_rotary_fwd",
+    "ofh_cache_append_params_init",
+    "ofh_cache_append",
     "ofh_cache_copy_pages",
     "ofh_page_pool_create",
     "ofh_page_pool_destroy",
@@ -248,6 +252,45 @@ class CacheWriteParams(ctypes.Structure):
     ]
 
 
+class RotaryFields(ctypes.Structure):
+    _fields_ = [
+        ("frequencies", ctypes.c_void_p),
+        ("rotary_dim", ctypes.c_size_t),
+        ("interleaved", ctypes.c_int32),
+        ("magnitude", ctypes.c_float),
+    ]
+
+
+class RotaryParams(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("batch", ctypes.c_size_t),
+        ("heads", ctypes.c_size_t),
+        ("tokens", ctypes.c_size_t),
+        ("head_dim", ctypes.c_size_t),
+        ("dtype", ctypes.c_int32),
+        ("transpose", ctypes.c_int32),
+        ("x_strides", ctypes.c_int64 * 3),
+        ("o_strides", ctypes.c_int64 * 3),
+        ("rotary", RotaryFields),
+        ("positions", ctypes.c_void_p),
+        ("position_stride", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+        ("offset", ctypes.c_int64),
+    ]
+
+
+class CacheAppendParams(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("cache", CacheWriteParams),
+        ("rotary", RotaryFields),
+        ("heads", ctypes.c_size_t),
+        ("q_strides", ctypes.c_int64 * 3),
+        ("o_strides", ctypes.c_int64 * 3),
+    ]
+
+
 class OfhError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"[ofh status {code}] {message}")
@@ -299,6 +342,10 @@ def lib() -> ctypes.CDLL:
                 ("ofh_paged_attention_fwd", ctypes.c_int, [vp] * 6 + [sz, vp]),
                 ("ofh_cache_write_params_init", None, [vp]),
                 ("ofh_cache_write", ctypes.c_int, [vp] * 6),
+                ("ofh_rotary_params_init", None, [vp]),
+                ("ofh_rotary_fwd", ctypes.c_int, [vp] * 4),
+                ("ofh_cache_append_params_init", None, [vp]),
+                ("ofh_cache_append", ctypes.c_int, [vp] * 8),
                 ("ofh_cache_copy_pages", ctypes.c_int, [vp, sz, sz, sz, sz, vp, vp, sz, vp]),
                 ("ofh_page_pool_create", ctypes.c_int, [sz, sz, ctypes.POINTER(vp)]),
                 ("ofh_page_pool_destroy", ctypes.c_int, [vp]),
@@ -951,8 +998,8 @@ class CacheWriter:
         self._write = L.ofh_cache_write
         self._ptrs = (k_pages.data_ptr(), v_pages.data_ptr())
 
-    def __call__(self, k, v, *, stream=None) -> None:
-        """k: [B,Hkv,T,D], v: [B,Hkv,T,Dv], the (padded) new rows."""
+    def _check_new(self, k, v) -> int:
+        """Checks the new rows; returns how many there are per sequence."""
         torch, dev = self._torch, self._device
         B, Hkv, D, Dv = self._row
         if not (_is_rows(torch, k, self._dtype, dev) and _is_rows(torch, v, self._dtype, dev)):
@@ -961,6 +1008,12 @@ class CacheWriter:
         T = k.shape[2]
         if k.shape != (B, Hkv, T, D) or v.shape != (B, Hkv, T, Dv):
             raise ValueError(f"k must be {(B, Hkv, 'T', D)} and v {(B, Hkv, 'T', Dv)}")
+        return T
+
+    def __call__(self, k, v, *, stream=None) -> None:
+        """k: [B,Hkv,T,D], v: [B,Hkv,T,Dv], the (padded) new rows."""
+        torch, dev = self._torch, self._device
+        T = self._check_new(k, v)
         p = CacheWriteParams.from_buffer_copy(self._params)
         p.tokens = T
         if not k.is_contiguous():
@@ -975,6 +1028,217 @@ class CacheWriter:
 def cache_write(k, v, k_pages, v_pages, page_table, lengths, *, counts=None, stream=None) -> None:
     """One call of CacheWriter."""
     CacheWriter(k_pages, v_pages, page_table, lengths, counts=counts)(k, v, stream=stream)
+
+
+def rotary_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: dict | None = None) -> list[float]:
+    """Radians per position of the rotary_dim / 2 pairs: f_i = base ** (-2 i / rotary_dim).
+    `scaling` stretches them by a factor for contexts longer than trained on:
+
+    {"type": "linear", "factor": s}: f_i / s.
+    {"type": "base", "factor": s}: base * s ** (rotary_dim / (rotary_dim - 2)) for base,
+        which leaves the fastest pair and divides the slowest by s.
+    {"type": "parts", "factor": s, "original_tokens": n, "low": l, "high": h}: by the
+        turns r_i = n f_i / (2 pi) of a pair over the original length: f_i from h turns
+        on, f_i / s up to l, in between f_i g + f_i / s (1 - g), g = (r_i - l) / (h - l)
+        (l = 1 and h = 32 unless given)."""
+    if type(rotary_dim) is not int or rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be a positive even integer")
+    if not (base > 0 and math.isfinite(base)):
+        raise ValueError("base must be positive")
+    keys = {"linear": {"factor"}, "base": {"factor"}, "parts": {"factor", "original_tokens", "low", "high"}}
+    options = dict(scaling or {})
+    kind = options.pop("type", None)
+    if scaling is not None:
+        if kind not in keys:
+            raise ValueError("scaling must have a type: 'linear', 'base' or 'parts'")
+        if set(options) - keys[kind]:
+            raise ValueError(f"scaling of type {kind!r} takes {sorted(keys[kind])}")
+        if not (options.get("factor", 0) > 0 and math.isfinite(options["factor"])):
+            raise ValueError("scaling needs a positive factor")
+    factor = options.get("factor", 1.0)
+    if kind == "base":
+        if rotary_dim == 2:
+            raise ValueError("scaling of the base needs two pairs at least")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    f = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
+    if kind == "linear":
+        return [x / factor for x in f]
+    if kind == "parts":
+        n, low, high = options.get("original_tokens", 0), options.get("low", 1.0), options.get("high", 32.0)
+        if not (n > 0 and 0 <= low < high):
+            raise ValueError("scaling by parts needs positive original_tokens and 0 <= low < high")
+        keep = [min(1.0, max(0.0, (n * x / (2.0 * math.pi) - low) / (high - low))) for x in f]
+        return [x * g + x / factor * (1.0 - g) for x, g in zip(f, keep)]
+    return f
+
+
+class Rotary:
+    """Rotary positions of rows of head_dim columns, of which the first rotary_dim
+    (all, unless given) are turned in pairs: columns i and i + rotary_dim / 2, or
+    with `interleaved` 2 i and 2 i + 1. Pair i at position p turns by the angle
+    p * frequencies[i] and is scaled by `magnitude`. Frequencies: numbers in
+    radians per position, or those of rotary_frequencies(rotary_dim, base=,
+    scaling=). They are kept on `device`."""
+
+    def __init__(self, head_dim: int, *, rotary_dim: int | None = None, base: float = 10000.0, scaling: dict | None = None,
+                 frequencies=None, interleaved: bool = False, magnitude: float = 1.0, device="cuda"):
+        torch = _torch()
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        if type(head_dim) is not int or type(rotary_dim) is not int or not 2 <= rotary_dim <= head_dim or rotary_dim % 2:
+            raise ValueError("rotary_dim must be even, from 2 to head_dim")
+        if not math.isfinite(magnitude):
+            raise ValueError("magnitude must be finite")
+        if frequencies is None:
+            frequencies = rotary_frequencies(rotary_dim, base=base, scaling=scaling)
+        elif scaling is not None:
+            raise ValueError("pass either frequencies or scaling, not both")
+        frequencies = torch.as_tensor(frequencies, dtype=torch.float64)
+        if tuple(frequencies.shape) != (rotary_dim // 2,):
+            raise ValueError("frequencies must be rotary_dim / 2 numbers")
+        if not bool(torch.isfinite(frequencies).all()):
+            raise ValueError("frequencies must be finite")
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError("device must be a GPU")
+        self.head_dim, self.rotary_dim, self.interleaved = head_dim, rotary_dim, bool(interleaved)
+        self.magnitude = float(magnitude)
+        # (its own copy: a program may go on with its tensor)
+        self.frequencies = frequencies.detach().to(device, copy=True).contiguous()
+        self._torch, self._device = torch, self.frequencies.device
+        p = RotaryParams()
+        self._lib = lib()
+        self._lib.ofh_rotary_params_init(ctypes.addressof(p))
+        p.head_dim = head_dim
+        self._fields(p.rotary)
+        self._params = bytes(p)
+
+    def _fields(self, r: RotaryFields) -> None:
+        r.frequencies, r.rotary_dim = self.frequencies.data_ptr(), self.rotary_dim
+        r.interleaved, r.magnitude = int(self.interleaved), self.magnitude
+
+    def __call__(self, x, *, offset: int = 0, positions=None, lengths=None, transpose: bool = False, out=None,
+                 stream=None):
+        """x: [B,H,T,D] (f32/bf16/f16, last axis contiguous). Token t of a sequence
+        is at position offset + t; or positions[t] or positions[b, t] (int32
+        device [T] or [B,T]); or lengths[b] - T + t (int32 device [B]: the last
+        T of lengths[b] tokens). `transpose` turns back: the gradient of x from
+        that of the result. out: x itself, or a tensor like it. Returns out."""
+        torch, dev = self._torch, self._device
+        if not (isinstance(x, torch.Tensor) and x.dtype in _DTYPE_CODES and _is_rows(torch, x, x.dtype, dev)):
+            _check_rows(torch, "x", x, 4, None, dev)
+        B, H, T, D = x.shape
+        if D != self.head_dim:
+            raise ValueError(f"x must have rows of {self.head_dim} columns")
+        if type(offset) is not int or not -(1 << 31) <= offset < 1 << 31:
+            raise ValueError("offset must be an integer within 32 bits")
+        if (positions is not None) + (lengths is not None) + (offset != 0) > 1:
+            raise ValueError("pass one of offset, positions and lengths")
+        p = RotaryParams.from_buffer_copy(self._params)
+        p.batch, p.heads, p.tokens, p.dtype, p.offset = B, H, T, _DTYPE_CODES[x.dtype], offset
+        p.transpose = int(bool(transpose))
+        if positions is not None:
+            _check_ints(torch, "positions", positions, (T,) if isinstance(positions, torch.Tensor) and positions.dim() == 1
+                        else (B, T), dev)
+            if min(positions.stride()) < 0:
+                raise ValueError("positions: strides must be non-negative")
+            p.positions = positions.data_ptr()
+            p.position_stride = positions.stride(0) if positions.dim() == 2 and B > 1 else 0
+        elif lengths is not None:
+            _check_ints(torch, "lengths", lengths, (B,), dev)
+            p.lengths = lengths.data_ptr()
+        if not x.is_contiguous():
+            p.x_strides[:] = _axis_strides("x", x)
+        if out is None:
+            out = torch.empty((B, H, T, D), dtype=x.dtype, device=dev)
+        else:
+            _check_rows(torch, "out", out, 4, x.dtype, dev)
+            if out.shape != x.shape:
+                raise ValueError(f"out must have shape {tuple(x.shape)}")
+            _check_written("out", out)
+        if not out.is_contiguous():
+            p.o_strides[:] = _axis_strides("out", out)
+        if out.data_ptr() == x.data_ptr():
+            # (axes of one element have any stride)
+            if _axis_strides("out", out) != _axis_strides("x", x):
+                raise ValueError("x turned in place must keep its strides")
+            p.o_strides[:] = p.x_strides[:]
+        rc = _launch(torch, dev, stream, self._lib.ofh_rotary_fwd, ctypes.addressof(p), x.data_ptr(), out.data_ptr())
+        if rc != OFH_SUCCESS:
+            check(rc)
+        return out
+
+
+class CacheAppender:
+    """CacheWriter with the rotation on the way: K rows are turned by their
+    positions into the pages, V rows copied, and the queries of the same tokens
+    turned too. One launch for what follows a layer's projections in a decode
+    step. Position and place of token t < counts[b] of sequence b are
+    CacheWriter's, lengths[b] - counts[b] + t."""
+
+    def __init__(self, k_pages, v_pages, page_table, lengths, rotary: Rotary, *, counts=None):
+        writer = CacheWriter(k_pages, v_pages, page_table, lengths, counts=counts)
+        if not isinstance(rotary, Rotary) or rotary.head_dim != k_pages.shape[3] or rotary._device != k_pages.device:
+            raise ValueError("rotary must be a Rotary of the cache's head_dim on its device")
+        self._writer, self._rotary = writer, rotary
+        p = CacheAppendParams()
+        L = lib()
+        L.ofh_cache_append_params_init(ctypes.addressof(p))
+        p.cache = CacheWriteParams.from_buffer_copy(writer._params)
+        rotary._fields(p.rotary)
+        self._params = bytes(p)
+        self._append = L.ofh_cache_append
+
+    def __call__(self, k, v, q=None, *, q_out=None, stream=None):
+        """k: [B,Hkv,T,D], v: [B,Hkv,T,Dv], the (padded) new rows; q: [B,H,T,D].
+        Returns the turned q (q_out: q itself, or a tensor like it), whose rows at
+        t >= counts[b] are 0; None without q."""
+        w = self._writer
+        torch, dev, dtype = w._torch, w._device, w._dtype
+        T = w._check_new(k, v)
+        B, _, D, _ = w._row
+        p = CacheAppendParams.from_buffer_copy(self._params)
+        p.cache.tokens = T
+        if not k.is_contiguous():
+            p.cache.k_strides[:] = _axis_strides("k", k)
+        if not v.is_contiguous():
+            p.cache.v_strides[:] = _axis_strides("v", v)
+        q_ptr = out_ptr = None
+        if q is not None:
+            if not _is_rows(torch, q, dtype, dev):
+                _check_rows(torch, "q", q, 4, dtype, dev)
+            H = q.shape[1]
+            if q.shape != (B, H, T, D):
+                raise ValueError(f"q must be {(B, 'H', T, D)}")
+            p.heads = H
+            if not q.is_contiguous():
+                p.q_strides[:] = _axis_strides("q", q)
+            if q_out is None:
+                q_out = torch.empty((B, H, T, D), dtype=dtype, device=dev)
+            else:
+                _check_rows(torch, "q_out", q_out, 4, dtype, dev)
+                if q_out.shape != q.shape:
+                    raise ValueError(f"q_out must have shape {tuple(q.shape)}")
+                _check_written("q_out", q_out)
+            if not q_out.is_contiguous():
+                p.o_strides[:] = _axis_strides("q_out", q_out)
+            q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
+            if q_ptr == out_ptr:
+                if _axis_strides("q_out", q_out) != _axis_strides("q", q):
+                    raise ValueError("q turned in place must keep its strides")
+                p.o_strides[:] = p.q_strides[:]
+        elif q_out is not None:
+            raise ValueError("q_out needs q")
+        rc = _launch(torch, dev, stream, self._append, ctypes.addressof(p), k.data_ptr(), v.data_ptr(), q_ptr, *w._ptrs,
+                     out_ptr)
+        if rc != OFH_SUCCESS:
+            check(rc)
+        return q_out
+
+
+def cache_append(k, v, k_pages, v_pages, page_table, lengths, rotary: Rotary, *, q=None, q_out=None, counts=None,
+                 stream=None):
+    """One call of CacheAppender."""
+    return CacheAppender(k_pages, v_pages, page_table, lengths, rotary, counts=counts)(k, v, q, q_out=q_out, stream=stream)
 
 
 def _page_numbers(torch, name, x, pages):

@@ -384,6 +384,64 @@ void ofh_cache_write_params_init(ofh_cache_write_params* p);
 int ofh_cache_write(const ofh_cache_write_params* p, const void* k, const void* v, void* k_pages, void* v_pages,
                     void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Rotary positions. No counterparts in the reference.
+ *
+ * The first rotary_dim columns of a row are rotary_dim / 2 pairs (x, y): columns
+ * i and i + rotary_dim / 2, or interleaved 2 i and 2 i + 1. At position p, pair i
+ * becomes
+ *     magnitude (x cos a - y sin a), magnitude (y cos a + x sin a), a = p frequencies[i]
+ * and the columns past rotary_dim stay. The transposed form turns by -a: it takes
+ * the gradient of the result to the gradient of x. Angles are formed in 64 bits,
+ * the rest in fp32, rounded once.
+ *
+ * fp32, bf16 and fp16, head dims up to 1024, rotary_dim even; any alignment and
+ * strides (rows of 16-byte words run faster). */
+typedef struct ofh_rotary {
+    const double* frequencies; /* device [rotary_dim / 2], radians per position */
+    size_t rotary_dim;
+    int32_t interleaved;
+    float magnitude;
+} ofh_rotary;
+
+typedef struct ofh_rotary_params {
+    uint32_t struct_size; /* set by ofh_rotary_params_init */
+    size_t batch, heads, tokens, head_dim;
+    int32_t dtype;
+    int32_t transpose;
+    int64_t x_strides[3], o_strides[3]; /* batch, head, token of X[B,H,T,D]; all zero: contiguous */
+    ofh_rotary rotary;
+    /* Position of token t of sequence b: positions[b * position_stride + t] where
+     * positions (device) are given; else lengths[b] - tokens + t (device [B], as
+     * paged attention's) where lengths are; else offset + t. */
+    const int32_t* positions;
+    int64_t position_stride; /* 0: one row for every sequence */
+    const int32_t* lengths;
+    int64_t offset; /* within 32 bits */
+} ofh_rotary_params;
+
+/* Defaults: fp32, magnitude 1, everything else zero. */
+void ofh_rotary_params_init(ofh_rotary_params* p);
+
+/* out may be x itself (with x's strides), and overlaps it in no other way. */
+int ofh_rotary_fwd(const ofh_rotary_params* p, const void* x, void* out, void* stream);
+
+/* ofh_cache_write with K turned on the way: the K row of position p is turned
+ * by p, V rows are copied. With `heads`, the queries of the same tokens are
+ * turned too: Q[B,H,T,D] -> q_out (q itself, or no overlap); their rows at
+ * t >= counts[b] are padding, written as 0. */
+typedef struct ofh_cache_append_params {
+    uint32_t struct_size; /* set by ofh_cache_append_params_init */
+    ofh_cache_write_params cache; /* its struct_size is set too */
+    ofh_rotary rotary;
+    size_t heads; /* 0: no queries (q and q_out are not read) */
+    int64_t q_strides[3], o_strides[3]; /* batch, head, token; all zero: contiguous */
+} ofh_cache_append_params;
+
+void ofh_cache_append_params_init(ofh_cache_append_params* p);
+int ofh_cache_append(const ofh_cache_append_params* p, const void* k, const void* v, const void* q, void* k_pages,
+                     void* v_pages, void* q_out, void* stream);
+
 /* Copies pages src[i] -> dst[i] of every pool. A page is page_bytes contiguous
  * bytes, page_stride_bytes from the next (0: page_bytes). `pools`, src and dst
  * are host arrays, read before the call returns. Refused: pages outside
