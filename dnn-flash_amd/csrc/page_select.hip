@@ -1,0 +1,333 @@
+// Selection of pages by a cheap score: the bounds of a page's keys, the scores of
+// a sequence's pages for a token, and the choice of the highest.
+//
+// Score of a page for a token and key-value head, an upper bound of q.k over the
+// page's keys k when q is a head of its group:
+//     max over the group's heads of sum_d q_d (q_d > 0 ? hi_d : lo_d),
+// hi and lo the columns' largest and smallest values in the page. The sum is
+// formed in 64 bits and rounded to fp32: its order then decides no rank.
+
+#include "serving_kernels.h"
+#include "flash_wave32.h"
+
+namespace ofh {
+namespace {
+
+constexpr int kSelectThreads = 256;
+constexpr int kSelectWaves = kSelectThreads / 64;
+
+// Elements of a 16-byte word, as floats.
+template <typename T>
+struct Words {
+    static constexpr int W = 16 / (int)sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(W)));
+    static __device__ __forceinline__ void get(u32x4 x, float (&f)[W]) {
+        const vec v = __builtin_bit_cast(vec, x);
+#pragma unroll
+        for (int i = 0; i < W; ++i) f[i] = (float)v[i];
+    }
+    static __device__ __forceinline__ u32x4 put(const float (&f)[W]) {
+        vec v;
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = (T)f[i];
+        return __builtin_bit_cast(u32x4, v);
+    }
+};
+
+// A NaN stays.
+__device__ __forceinline__ float lower(float a, float b) { return b < a || b != b ? b : a; }
+__device__ __forceinline__ float upper(float a, float b) { return b > a || b != b ? b : a; }
+
+// Lanes per row of `words` 16-byte words: a power of two.
+__device__ __forceinline__ int row_lanes(int words) { return words <= 1 ? 1 : 1 << (32 - __builtin_clz(words - 1)); }
+
+// A wavefront per touched page and key-value head: its lanes take the words of a
+// row and, beside each other, several rows, four of which are in flight per lane.
+// Bound by reading the page's keys once; a decode step's few pages by the launch.
+template <typename T>
+__global__ __launch_bounds__(kSelectThreads) void page_bounds_kernel(PageBoundsArgs a) {
+    using X = Words<T>;
+    constexpr int W = X::W, AHEAD = 4;
+    const int lane = threadIdx.x & 63;
+    const int64_t item = (int64_t)blockIdx.x * kSelectWaves + (threadIdx.x >> 6);
+    const int64_t bi = item / a.Hkv;
+    const int hk = (int)(item - bi * a.Hkv), b = (int)(bi / a.touched), i = (int)(bi - (int64_t)b * a.touched);
+    if (b >= a.B) return;
+    const int size = 1 << a.page_shift;
+    const int count = a.counts != nullptr ? max(0, min(a.counts[b], a.T)) : a.T;
+    const int64_t length = a.lengths[b], first = max((int64_t)0, length - count);
+    const int64_t place = (first >> a.page_shift) + i;
+    if (count == 0 || place >= a.max_pages || place << a.page_shift >= length) return;
+    const int page = a.table[b * a.table_stride + place];
+    if ((unsigned)page >= (unsigned)a.num_pages) return;
+    const int rows = (int)min((int64_t)size, length - (place << a.page_shift));
+    const int words = a.D / W, lanes = row_lanes(words), groups = 64 / lanes;
+    const int word = min(lane % lanes, words - 1), group = lane / lanes;
+    const T* keys = (const T*)a.k_pages + page * a.k_sp + hk * a.k_sh + word * W;
+    float lo[W], hi[W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        lo[j] = __builtin_huge_valf();
+        hi[j] = kNegInf;
+    }
+    for (int r = group; r < rows; r += AHEAD * groups) {
+        u32x4 x[AHEAD];
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) x[n] = *(const u32x4*)(keys + (int64_t)min(r + n * groups, rows - 1) * a.k_st);
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) {
+            float f[W];
+            X::get(x[n], f);
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                lo[j] = lower(lo[j], f[j]);
+                hi[j] = upper(hi[j], f[j]);
+            }
+        }
+    }
+    for (int d = lanes; d < 64; d *= 2)
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            lo[j] = lower(lo[j], __shfl_xor(lo[j], d));
+            hi[j] = upper(hi[j], __shfl_xor(hi[j], d));
+        }
+    if (lane >= words) return;
+    T* out = (T*)a.bounds + page * a.b_sp + hk * a.b_sh + word * W;
+    *(u32x4*)out = X::put(lo);
+    *(u32x4*)(out + a.b_st) = X::put(hi);
+}
+
+// Pages with keys up to token (b, t): the candidates.
+__device__ __forceinline__ int candidates(const SelectArgs& a, int b, int t) {
+    const int capacity = a.max_pages << a.page_shift;
+    const int seen = max(0, min(a.lengths[b], capacity)) - a.T + t + 1;
+    return (max(0, seen) + (1 << a.page_shift) - 1) >> a.page_shift;
+}
+
+// Scores as numbers whose order is theirs: -0 counts as 0, NaN is above all. 0 is
+// below every score: pages without a place in the pool.
+__device__ __forceinline__ unsigned score_rank(float x) {
+    if (x != x) return ~0u;
+    const unsigned u = __builtin_bit_cast(unsigned, x + 0.0f);
+    return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)u, CTRL, 0xf, 0xf, true);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(u >> 32), CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Sum over `lanes` neighbouring lanes, valid in the first of them.
+__device__ __forceinline__ double sum_lanes(double x, int lanes) {
+    if (lanes >= 2) x += dpp<0xB1>(x);   // quad_perm [1,0,3,2]
+    if (lanes >= 4) x += dpp<0x4E>(x);   // quad_perm [2,3,0,1]
+    if (lanes >= 8) x += dpp<0x104>(x);  // row_shl:4
+    if (lanes >= 16) x += dpp<0x108>(x); // row_shl:8
+    if (lanes >= 32) x += __shfl_xor(x, 16);
+    if (lanes >= 64) x += __shfl_xor(x, 32);
+    return x;
+}
+
+constexpr int kScorePages = 64;     // of a workgroup
+constexpr int kScoreQuery = 8192;   // numbers of Q that a workgroup keeps: 64 KB
+
+// A workgroup scores up to 64 pages for one token and key-value head. Q is in LDS in
+// 64 bits; the lanes of a row of bounds take a word of lo and of hi each, and
+// several pages stand beside each other in a wavefront. Tokens that see no more
+// pages than they may take need no scores.
+template <typename T>
+__global__ __launch_bounds__(kSelectThreads) void page_score_kernel(SelectArgs a, int chunks) {
+    using X = Words<T>;
+    constexpr int W = X::W;
+    __shared__ __attribute__((aligned(16))) double q[kScoreQuery];
+    const int64_t row = blockIdx.x / chunks;  // (b, hk, t)
+    const int chunk = (int)(blockIdx.x - row * chunks);
+    const int t = (int)(row % a.T), hk = (int)(row / a.T % a.Hkv), b = (int)(row / a.T / a.Hkv);
+    const int have = candidates(a, b, t);
+    const int page0 = chunk * kScorePages, page1 = min(have, page0 + kScorePages);
+    if (have <= a.pages || page0 >= have) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int words = a.D / W, lanes = row_lanes(words), beside = 64 / lanes;
+    const int word = min(lane % lanes, words - 1), slot = lane / lanes;
+    const int most = kScoreQuery / a.D;  // heads at a time
+    for (int g0 = 0; g0 < a.G; g0 += most) {
+        const int heads = min(most, a.G - g0);
+        __syncthreads();
+        for (int n = threadIdx.x; n < heads * a.D; n += kSelectThreads) {
+            const int g = n / a.D, d = n - g * a.D;
+            const double x = (double)(float)((const T*)a.q)[b * a.q_sb + (int64_t)(hk * a.G + g0 + g) * a.q_sh + t * a.q_st + d];
+            q[n] = a.negative ? -x : x;
+        }
+        __syncthreads();
+        for (int p = page0 + wave * beside + slot; p - slot < page1; p += kSelectWaves * beside) {
+            const int place = min(p, page1 - 1);
+            const int page = a.table[b * a.table_stride + place];
+            const bool ok = (unsigned)page < (unsigned)a.num_pages;
+            const T* at = (const T*)a.bounds + (ok ? page : 0) * a.b_sp + hk * a.b_sh + word * W;
+            float lo[W], hi[W];
+            X::get(*(const u32x4*)at, lo);
+            X::get(*(const u32x4*)(at + a.b_st), hi);
+            unsigned best = 0;
+            for (int g = 0; g < heads; ++g) {
+                const double* x = q + g * a.D + word * W;
+                double sum = 0.0;
+#pragma unroll
+                for (int j = 0; j < W; ++j) sum = __builtin_fma(x[j], (double)(x[j] > 0.0 ? hi[j] : lo[j]), sum);
+                if (lane % lanes >= words) sum = 0.0;
+                best = max(best, score_rank((float)sum_lanes(sum, lanes)));
+            }
+            if (lane % lanes == 0 && p < page1) {
+                uint32_t* out = a.scores + row * a.max_pages + p;
+                if (!ok) best = 0;
+                *out = g0 > 0 ? max(*out, best) : best;
+            }
+        }
+    }
+}
+
+constexpr int kSelectKept = 16384;  // scores that a workgroup keeps in LDS
+
+// A workgroup per token and key-value head. The need-th highest score of the
+// candidates between the first and the recent ones is found a byte at a time, from
+// the counts of its values among the scores that share the bytes before; then each
+// thread takes a stretch of the candidates, counts what is above and what is equal
+// to it, and after a sum over the threads before writes its share: ascending, ties
+// to the lower page.
+__global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectArgs a) {
+    __shared__ uint32_t kept[kSelectKept];
+    __shared__ int count[256];
+    __shared__ int found[2];
+    __shared__ int sums[2][kSelectWaves];
+    const int64_t row = blockIdx.x;
+    const int t = (int)(row % a.T), b = (int)(row / a.T / a.Hkv);
+    const int have = candidates(a, b, t);
+    int32_t* out = a.selected + row * a.pages;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (have <= a.pages) {
+        for (int i = tid; i < a.pages; i += kSelectThreads) out[i] = i < have ? i : -1;
+        return;
+    }
+    const uint32_t* scores = a.scores + row * a.max_pages + a.first_pages;
+    const int n = have - a.first_pages - a.recent_pages, need = a.pages - a.first_pages - a.recent_pages;
+    const bool keep = n <= kSelectKept;
+    if (keep)
+        for (int i = tid; i < n; i += kSelectThreads) kept[i] = scores[i];
+    // (the first and the recent pages)
+    for (int i = tid; i < a.first_pages; i += kSelectThreads) out[i] = i;
+    for (int i = tid; i < a.recent_pages; i += kSelectThreads) out[a.pages - a.recent_pages + i] = have - a.recent_pages + i;
+    if (need == 0) return;
+    auto score = [&](int i) { return keep ? kept[i] : scores[i]; };
+    uint32_t limit = 0;
+    int rest = need;  // of the scores that share the bytes so far
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        count[tid] = 0;
+        __syncthreads();
+        const uint32_t above = shift == 24 ? 0u : ~0u << (shift + 8);
+        for (int i = tid; i < n; i += kSelectThreads) {
+            const uint32_t x = score(i);
+            if ((x & above) == (limit & above)) atomicAdd(&count[x >> shift & 255], 1);
+        }
+        __syncthreads();
+        // of the values from the highest down: the first at which `rest` are reached
+        const int mine = count[255 - tid];
+        int upto = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int x = __shfl_up(upto, d);
+            if (lane >= d) upto += x;
+        }
+        if (lane == 63) sums[0][wave] = upto;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) upto += sums[0][w];
+        if (upto >= rest && upto - mine < rest) {
+            found[0] = 255 - tid;
+            found[1] = rest - (upto - mine);
+        }
+        __syncthreads();
+        limit |= (uint32_t)found[0] << shift;
+        rest = found[1];
+    }
+    // all above the limit, and the first `rest` equal to it
+    const int per = (n + kSelectThreads - 1) / kSelectThreads, begin = min(n, tid * per), end = min(n, begin + per);
+    int above = 0, equal = 0;
+    for (int i = begin; i < end; ++i) {
+        const uint32_t x = score(i);
+        above += x > limit;
+        equal += x == limit;
+    }
+    int above_upto = above, equal_upto = equal;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int x = __shfl_up(above_upto, d), y = __shfl_up(equal_upto, d);
+        if (lane >= d) {
+            above_upto += x;
+            equal_upto += y;
+        }
+    }
+    __syncthreads();
+    if (lane == 63) {
+        sums[0][wave] = above_upto;
+        sums[1][wave] = equal_upto;
+    }
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) {
+        above_upto += sums[0][w];
+        equal_upto += sums[1][w];
+    }
+    int ties = equal_upto - equal;
+    int at = a.first_pages + above_upto - above + min(ties, rest);
+    for (int i = begin; i < end; ++i) {
+        const uint32_t x = score(i);
+        if (x > limit || (x == limit && ties++ < rest)) out[at++] = a.first_pages + i;
+    }
+}
+
+template <typename T>
+hipError_t launch_score(const SelectArgs& a, int chunks, hipStream_t s) {
+    hipLaunchKernelGGL((page_score_kernel<T>), dim3((unsigned)((int64_t)a.B * a.Hkv * a.T * chunks)), dim3(kSelectThreads), 0,
+                       s, a, chunks);
+    return hipGetLastError();
+}
+
+int64_t bounds_grid(const PageBoundsArgs& a) {
+    return ((int64_t)a.B * a.touched * a.Hkv + kSelectWaves - 1) / kSelectWaves;
+}
+int score_chunks(const SelectArgs& a) { return (a.max_pages + kScorePages - 1) / kScorePages; }
+
+}  // namespace
+
+bool page_bounds_fits(const PageBoundsArgs& a) { return grid_fits(bounds_grid(a), kSelectThreads); }
+
+hipError_t launch_page_bounds(const PageBoundsArgs& a, int dtype, hipStream_t s) {
+    const dim3 grid((unsigned)bounds_grid(a)), block(kSelectThreads);
+    switch (dtype) {
+        case DT_F32: hipLaunchKernelGGL((page_bounds_kernel<float>), grid, block, 0, s, a); break;
+        case DT_BF16: hipLaunchKernelGGL((page_bounds_kernel<__bf16>), grid, block, 0, s, a); break;
+        case DT_F16: hipLaunchKernelGGL((page_bounds_kernel<_Float16>), grid, block, 0, s, a); break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+
+bool page_select_fits(const SelectArgs& a) {
+    return grid_fits((int64_t)a.B * a.Hkv * a.T * score_chunks(a), kSelectThreads);
+}
+
+hipError_t launch_page_select(const SelectArgs& a, int dtype, hipStream_t s) {
+    if (a.max_pages > a.pages) {
+        hipError_t e;
+        switch (dtype) {
+            case DT_F32: e = launch_score<float>(a, score_chunks(a), s); break;
+            case DT_BF16: e = launch_score<__bf16>(a, score_chunks(a), s); break;
+            case DT_F16: e = launch_score<_Float16>(a, score_chunks(a), s); break;
+            default: return hipErrorInvalidValue;
+        }
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(page_select_kernel, dim3((unsigned)((int64_t)a.B * a.Hkv * a.T)), dim3(kSelectThreads), 0, s, a);
+    return hipGetLastError();
+}
+
+}  // namespace ofh

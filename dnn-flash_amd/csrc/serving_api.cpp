@@ -116,7 +116,23 @@ void unsplit(Split& s) {
     s.bytes = 0;
 }
 
-int run_stream(ofh::StreamArgs& a, int dtype, Split s, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+// The call's scratch: the caller's, or the library's of the stream (held by `lease`).
+int take_workspace(size_t need, void*& workspace, size_t workspace_bytes, hipStream_t stream, ofh::ScratchLease& lease) {
+    const std::string small = "workspace too small: need " + std::to_string(need) + " bytes";
+    if (need > 0 && workspace == nullptr) {
+        bool fits = true;
+        if (int rc = lease.acquire(need, stream, fits)) return rc;
+        if (!fits) return api_error(OFH_ERROR_WORKSPACE_TOO_SMALL, small);
+        workspace = lease.ptr;
+    } else if (need > workspace_bytes) {
+        return api_error(OFH_ERROR_WORKSPACE_TOO_SMALL, small);
+    }
+    if (need > 0 && ((uintptr_t)workspace & 15) != 0) return unsupported("workspace must be 16-byte aligned");
+    return OFH_SUCCESS;
+}
+
+int run_stream(ofh::StreamArgs& a, int dtype, Split s, void* workspace, size_t workspace_bytes, hipStream_t stream,
+               hipError_t (*launch)(const ofh::StreamArgs&, int, hipStream_t) = ofh::launch_stream) {
     if (!ofh::grid_fits(s.units * s.splits, ofh::kStreamThreads) ||
         !ofh::grid_fits((int64_t)a.B * a.Hkv * a.T * a.G * ((a.Dv + 31) / 32), 64))
         return unsupported("attention call exceeds the launch range");
@@ -138,7 +154,7 @@ int run_stream(ofh::StreamArgs& a, int dtype, Split s, void* workspace, size_t w
         a.part_o = static_cast<float*>(workspace);
         a.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + round256(rows * a.Dv * 4));
     }
-    OFH_HIP_CHECK(ofh::launch_stream(a, dtype, stream));
+    OFH_HIP_CHECK(launch(a, dtype, stream));
     return lease.release();
 }
 
@@ -322,6 +338,173 @@ int paged_args(const ofh_paged_params* p, bool check_ptrs, const void* q, const 
     return OFH_SUCCESS;
 }
 
+// The bounds of a pool's pages, [page, kv_head, 2, head_dim].
+int check_bounds(size_t batch, size_t kv_heads, size_t D, int dtype, const int64_t in[3], const void* bounds,
+                 bool check_ptr, int64_t strides[3]) {
+    if (batch == 0 || kv_heads == 0 || D == 0) return invalid("cache dimensions must be non-zero");
+    if (!known_dtype(dtype)) return invalid("unknown dtype");
+    const size_t step = dtype == OFH_DTYPE_F32 ? 4 : 8;
+    if (D % step != 0 || D > 256) return unsupported("head_dim must be a multiple of " + std::to_string(step) + " up to 256");
+    if (batch > (size_t)kMaxTokens || kv_heads > (size_t)kMaxTokens)
+        return unsupported("cache dimensions exceed the 32-bit index range");
+    resolve_strides(strides, in, kv_heads, 2, D);
+    return check_tensor({"bounds", bounds, strides, D}, elem_size(dtype), check_ptr, 1);
+}
+
+int select_args(const ofh_select_params* p, bool check_ptrs, const void* q, const void* bounds, int32_t* selected,
+                ofh::SelectArgs& a) {
+    if (p == nullptr) return invalid("params must be non-null");
+    if (p->struct_size != sizeof(*p))
+        return invalid("ofh_select_params.struct_size mismatch (call ofh_select_params_init)");
+    if (p->heads == 0 || p->query_tokens == 0) return invalid("attention dimensions must be non-zero");
+    int64_t qs[3], bs[3];
+    if (int rc = check_bounds(p->batch, p->kv_heads, p->head_dim, p->dtype, p->bounds_strides, bounds, check_ptrs, bs))
+        return rc;
+    if (p->heads % p->kv_heads != 0) return invalid("heads must be a multiple of kv_heads");
+    if (int rc = check_pages(p->num_pages, p->page_size, p->max_pages, p->table_stride, p->page_table, p->lengths, check_ptrs))
+        return rc;
+    if (p->pages == 0) return invalid("pages must be non-zero");
+    if (p->first_pages > p->pages || p->recent_pages > p->pages - p->first_pages)
+        return invalid("first_pages and recent_pages must be at most pages together");
+    if (p->heads > (size_t)kMaxTokens || p->query_tokens > (size_t)kMaxTokens || p->pages > (size_t)kMaxTokens ||
+        (uint64_t)p->heads * p->query_tokens > (uint64_t)kMaxTokens ||
+        (uint64_t)p->batch * p->heads * p->query_tokens > (uint64_t)kMaxTokens)
+        return unsupported("attention dimensions exceed the 32-bit index range");
+    resolve_strides(qs, p->q_strides, p->heads, p->query_tokens, p->head_dim);
+    for (int i = 0; i < 3; ++i)
+        if (qs[i] < 0) return invalid("q strides must be non-negative");
+    if (check_ptrs && (q == nullptr || selected == nullptr)) return invalid("q and selected must be non-null");
+    if (check_ptrs && ((uintptr_t)q % elem_size(p->dtype) != 0 || (uintptr_t)selected % 4 != 0))
+        return unsupported("q and selected must be aligned to their elements");
+    a = ofh::SelectArgs{};
+    a.q = q;
+    a.bounds = bounds;
+    a.selected = selected;
+    a.q_sb = qs[0]; a.q_sh = qs[1]; a.q_st = qs[2];
+    a.b_sp = bs[0]; a.b_sh = bs[1]; a.b_st = bs[2];
+    a.table = p->page_table;
+    a.table_stride = p->table_stride != 0 ? p->table_stride : (int64_t)p->max_pages;
+    a.num_pages = (int)p->num_pages;
+    a.page_shift = log2_of(p->page_size);
+    a.max_pages = (int)p->max_pages;
+    a.lengths = p->lengths;
+    a.B = (int)p->batch;
+    a.Hkv = (int)p->kv_heads;
+    a.G = (int)(p->heads / p->kv_heads);
+    a.T = (int)p->query_tokens;
+    a.D = (int)p->head_dim;
+    a.pages = (int)p->pages;
+    a.first_pages = (int)p->first_pages;
+    a.recent_pages = (int)p->recent_pages;
+    a.negative = p->negative != 0;
+    return OFH_SUCCESS;
+}
+
+// Scores, where a sequence can have more pages than it may take.
+size_t select_bytes(const ofh::SelectArgs& a) {
+    return a.max_pages > a.pages ? (size_t)a.B * a.Hkv * a.T * a.max_pages * 4 : 0;
+}
+
+// A batch in groups that share pages.
+struct PrefixPlan {
+    Split tail;
+    int tiles, splits, min_steps;
+    size_t tail_o, tail_ml, prefix_o, prefix_ml;  // bytes
+    size_t bytes() const { return tail_o + tail_ml + prefix_o + prefix_ml; }
+};
+
+int prefix_args(const ofh_paged_params* p, const ofh_prefix_groups* g, bool check_ptrs, const void* q, const void* k,
+                const void* v, void* out, ofh::StreamArgs& a) {
+    if (int rc = paged_args(p, check_ptrs, q, k, v, out, a)) return rc;
+    if (g == nullptr) return invalid("groups must be non-null");
+    if (g->struct_size != sizeof(*g))
+        return invalid("ofh_prefix_groups.struct_size mismatch (call ofh_prefix_groups_init)");
+    if (g->groups == 0 || g->groups > p->batch) return invalid("groups must be 1 to batch");
+    if (check_ptrs && (g->starts == nullptr || g->shared_tokens == nullptr))
+        return invalid("starts and shared_tokens must be non-null");
+    if (g->least_shared > g->most_shared || g->most_shared > p->max_pages * p->page_size)
+        return invalid("least_shared and most_shared must be within the table's tokens, in this order");
+    // (rows of all sequences are numbered in 32 bits)
+    if ((uint64_t)p->batch * p->heads * p->query_tokens > (uint64_t)kMaxTokens)
+        return unsupported("attention dimensions exceed the 32-bit index range");
+    a.group_starts = g->starts;
+    a.shared = g->shared_tokens;
+    a.groups = (int)g->groups;
+    a.max_shared = (int)g->most_shared;
+    return OFH_SUCCESS;
+}
+
+PrefixPlan plan_prefix(const ofh::StreamArgs& a, int dtype, const ofh_prefix_groups* g, int max_key_splits) {
+    PrefixPlan plan{};
+    ofh::StreamArgs own = a;
+    own.capacity = std::max(a.capacity - (int)g->least_shared, 1);
+    plan.tail = plan_split(own, dtype, max_key_splits);
+    const int dk = ofh::stream_kernel_dim(a.D, a.Dv);
+    const int rows = ofh::prefix_tile_rows(a, dtype), step = ofh::stream_step_keys(dtype, dk);
+    plan.min_steps = ofh::kStreamThreads / 64;
+    plan.tiles = (int)(((int64_t)a.B * a.T * a.G + (int64_t)a.groups * (rows - 1)) / rows);
+    const int64_t units = (int64_t)a.Hkv * plan.tiles, steps = ((int64_t)g->most_shared + step - 1) / step;
+    const int64_t n = std::min<int64_t>({(2 * ofh::kComputeUnits + units - 1) / units, steps / plan.min_steps,
+                                         max_key_splits > 0 ? max_key_splits : 128});
+    plan.splits = (int)std::max<int64_t>(1, n);
+    const size_t tail_rows = (size_t)plan.tail.units * plan.tail.splits * plan.tail.tile_rows;
+    const size_t prefix_rows = (size_t)a.B * a.Hkv * a.T * a.G * plan.splits;
+    plan.tail_o = round256(tail_rows * a.Dv * 4);
+    plan.tail_ml = round256(tail_rows * 8);
+    plan.prefix_o = round256(prefix_rows * a.Dv * 4);
+    plan.prefix_ml = round256(prefix_rows * 8);
+    return plan;
+}
+
+int run_prefix(ofh::StreamArgs& a, int dtype, const PrefixPlan& plan, void* workspace, size_t workspace_bytes,
+               hipStream_t stream) {
+    if (!ofh::grid_fits(plan.tail.units * plan.tail.splits, ofh::kStreamThreads) ||
+        !ofh::grid_fits((int64_t)a.Hkv * plan.tiles * plan.splits, ofh::kStreamThreads) ||
+        !ofh::grid_fits((int64_t)a.B * a.Hkv * a.T * a.G * ((a.Dv + 31) / 32), 64))
+        return unsupported("attention call exceeds the launch range");
+    ofh::ScratchLease lease;
+    if (int rc = take_workspace(plan.bytes(), workspace, workspace_bytes, stream, lease)) return rc;
+    a.row_tiles = plan.tail.row_tiles;
+    a.splits = plan.tail.splits;
+    a.min_steps = plan.tail.min_steps;
+    a.prefix_tiles = plan.tiles;
+    a.prefix_splits = plan.splits;
+    a.prefix_min_steps = plan.min_steps;
+    char* at = static_cast<char*>(workspace);
+    a.part_o = reinterpret_cast<float*>(at);
+    a.part_ml = reinterpret_cast<float*>(at += plan.tail_o);
+    a.prefix_o = reinterpret_cast<float*>(at += plan.tail_ml);
+    a.prefix_ml = reinterpret_cast<float*>(at += plan.prefix_o);
+    OFH_HIP_CHECK(ofh::launch_stream_prefix(a, dtype, stream));
+    OFH_HIP_CHECK(ofh::launch_stream_tail(a, dtype, stream));
+    return lease.release();
+}
+
+// Attention over selected pages: a token is a sequence of the kernels.
+int selected_args(const ofh_paged_params* p, size_t pages, bool check_ptrs, const int32_t* selected, const void* q,
+                  const void* k, const void* v, void* out, ofh::StreamArgs& a) {
+    if (int rc = paged_args(p, check_ptrs, q, k, v, out, a)) return rc;
+    if (pages == 0) return invalid("pages must be non-zero");
+    if (p->window != 0) return unsupported("selected pages take no window");
+    if (check_ptrs && selected == nullptr) return invalid("selected must be non-null");
+    if (pages > (size_t)kMaxTokens || (uint64_t)pages * p->page_size > (uint64_t)kMaxTokens)
+        return unsupported("selected pages exceed the 32-bit index range");
+    if ((uint64_t)p->batch * p->heads * p->query_tokens > (uint64_t)kMaxTokens)
+        return unsupported("attention dimensions exceed the 32-bit index range");
+    a.selected = selected;
+    a.num_selected = (int)pages;
+    a.tokens = a.T;
+    a.B *= a.T;
+    a.T = 1;
+    return OFH_SUCCESS;
+}
+
+Split plan_selected(const ofh::StreamArgs& a, int dtype, int max_key_splits) {
+    ofh::StreamArgs seen = a;
+    seen.capacity = (int)std::min<int64_t>(a.capacity, (int64_t)a.num_selected << a.page_shift);
+    return plan_split(seen, dtype, max_key_splits);
+}
+
 }  // namespace
 
 extern "C" {
@@ -380,6 +563,129 @@ int ofh_paged_attention_fwd(const ofh_paged_params* p, const void* q, const void
         if (int rc = paged_args(p, true, q, k_pages, v_pages, out, a)) return rc;
         return run_stream(a, p->dtype, plan_split(a, p->dtype, p->max_key_splits), workspace, workspace_bytes,
                           static_cast<hipStream_t>(stream));
+    });
+}
+
+void ofh_prefix_groups_init(ofh_prefix_groups* g) {
+    if (g == nullptr) return;
+    std::memset(g, 0, sizeof(*g));
+    g->struct_size = sizeof(*g);
+}
+
+int ofh_shared_prefix_workspace_bytes(const ofh_paged_params* p, const ofh_prefix_groups* g, size_t* bytes) {
+    return guarded([&]() -> int {
+        if (bytes == nullptr) return invalid("bytes must be non-null");
+        ofh::StreamArgs a;
+        if (int rc = prefix_args(p, g, false, nullptr, nullptr, nullptr, nullptr, a)) return rc;
+        *bytes = plan_prefix(a, p->dtype, g, p->max_key_splits).bytes();
+        return OFH_SUCCESS;
+    });
+}
+
+int ofh_shared_prefix_attention_fwd(const ofh_paged_params* p, const ofh_prefix_groups* g, const void* q,
+                                    const void* k_pages, const void* v_pages, void* out, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+    return guarded([&]() -> int {
+        ofh::StreamArgs a;
+        if (int rc = prefix_args(p, g, true, q, k_pages, v_pages, out, a)) return rc;
+        return run_prefix(a, p->dtype, plan_prefix(a, p->dtype, g, p->max_key_splits), workspace, workspace_bytes,
+                          static_cast<hipStream_t>(stream));
+    });
+}
+
+int ofh_selected_attention_workspace_bytes(const ofh_paged_params* p, size_t pages, size_t* bytes) {
+    return guarded([&]() -> int {
+        if (bytes == nullptr) return invalid("bytes must be non-null");
+        ofh::StreamArgs a;
+        if (int rc = selected_args(p, pages, false, nullptr, nullptr, nullptr, nullptr, nullptr, a)) return rc;
+        *bytes = plan_selected(a, p->dtype, p->max_key_splits).bytes;
+        return OFH_SUCCESS;
+    });
+}
+
+int ofh_selected_attention_fwd(const ofh_paged_params* p, const int32_t* selected, size_t pages, const void* q,
+                               const void* k_pages, const void* v_pages, void* out, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+    return guarded([&]() -> int {
+        ofh::StreamArgs a;
+        if (int rc = selected_args(p, pages, true, selected, q, k_pages, v_pages, out, a)) return rc;
+        return run_stream(a, p->dtype, plan_selected(a, p->dtype, p->max_key_splits), workspace, workspace_bytes,
+                          static_cast<hipStream_t>(stream), ofh::launch_stream_selected);
+    });
+}
+
+void ofh_page_bounds_params_init(ofh_page_bounds_params* p) {
+    if (p == nullptr) return;
+    std::memset(p, 0, sizeof(*p));
+    p->struct_size = sizeof(*p);
+}
+
+int ofh_page_bounds(const ofh_page_bounds_params* p, const void* k_pages, void* bounds, void* stream) {
+    return guarded([&]() -> int {
+        if (p == nullptr) return invalid("params must be non-null");
+        if (p->struct_size != sizeof(*p))
+            return invalid("ofh_page_bounds_params.struct_size mismatch (call ofh_page_bounds_params_init)");
+        if (p->tokens == 0) return invalid("cache dimensions must be non-zero");
+        int64_t ks[3], bs[3];
+        if (int rc = check_bounds(p->batch, p->kv_heads, p->head_dim, p->dtype, p->bounds_strides, bounds, true, bs)) return rc;
+        if (p->tokens > (size_t)kMaxTokens) return unsupported("cache dimensions exceed the 32-bit index range");
+        if (int rc = check_pages(p->num_pages, p->page_size, p->max_pages, p->table_stride, p->page_table, p->lengths, true))
+            return rc;
+        resolve_strides(ks, p->k_page_strides, p->kv_heads, p->page_size, p->head_dim);
+        if (int rc = check_tensor({"k_pages", k_pages, ks, p->head_dim}, elem_size(p->dtype), true, 1)) return rc;
+        ofh::PageBoundsArgs a{};
+        a.k_pages = k_pages;
+        a.bounds = bounds;
+        a.k_sp = ks[0]; a.k_sh = ks[1]; a.k_st = ks[2];
+        a.b_sp = bs[0]; a.b_sh = bs[1]; a.b_st = bs[2];
+        a.table = p->page_table;
+        a.table_stride = p->table_stride != 0 ? p->table_stride : (int64_t)p->max_pages;
+        a.num_pages = (int)p->num_pages;
+        a.page_shift = log2_of(p->page_size);
+        a.max_pages = (int)p->max_pages;
+        a.lengths = p->lengths;
+        a.counts = p->counts;
+        a.B = (int)p->batch;
+        a.Hkv = (int)p->kv_heads;
+        a.T = (int)p->tokens;
+        a.D = (int)p->head_dim;
+        // a page's last token, and what comes after it
+        a.touched = (int)std::min<size_t>((p->tokens + p->page_size - 2) / p->page_size + 1, p->max_pages);
+        if (!ofh::page_bounds_fits(a)) return unsupported("page bounds exceed the launch range");
+        OFH_HIP_CHECK(ofh::launch_page_bounds(a, p->dtype, static_cast<hipStream_t>(stream)));
+        return OFH_SUCCESS;
+    });
+}
+
+void ofh_select_params_init(ofh_select_params* p) {
+    if (p == nullptr) return;
+    std::memset(p, 0, sizeof(*p));
+    p->struct_size = sizeof(*p);
+    p->query_tokens = 1;
+}
+
+int ofh_select_pages_workspace_bytes(const ofh_select_params* p, size_t* bytes) {
+    return guarded([&]() -> int {
+        if (bytes == nullptr) return invalid("bytes must be non-null");
+        ofh::SelectArgs a;
+        if (int rc = select_args(p, false, nullptr, nullptr, nullptr, a)) return rc;
+        *bytes = select_bytes(a);
+        return OFH_SUCCESS;
+    });
+}
+
+int ofh_select_pages(const ofh_select_params* p, const void* q, const void* bounds, int32_t* selected, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+    return guarded([&]() -> int {
+        ofh::SelectArgs a;
+        if (int rc = select_args(p, true, q, bounds, selected, a)) return rc;
+        if (!ofh::page_select_fits(a)) return unsupported("selection exceeds the launch range");
+        ofh::ScratchLease lease;
+        if (int rc = take_workspace(select_bytes(a), workspace, workspace_bytes, static_cast<hipStream_t>(stream), lease))
+            return rc;
+        a.scores = static_cast<uint32_t*>(workspace);
+        OFH_HIP_CHECK(ofh::launch_page_select(a, p->dtype, static_cast<hipStream_t>(stream)));
+        return lease.release();
     });
 }
 

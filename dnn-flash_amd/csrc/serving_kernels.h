@@ -47,6 +47,33 @@ struct StreamArgs {
     int splits, min_steps;
     float* part_o;   // [tiles][splits][rows of a tile][Dv]
     float* part_ml;  // [tiles][splits][rows of a tile][2]: max (log2 units), sum
+
+    // A batch in groups whose sequences share their first keys. Those are read by
+    // tiles of all rows of a group (kPrefix), the rest by each sequence's own
+    // (kTail). Group g has the sequences [group_starts[g], group_starts[g + 1]), of
+    // which each shares its first shared[b] keys, whole pages, in the pages of the
+    // group's first sequence.
+    const int32_t* group_starts;
+    const int32_t* shared;
+    int groups, max_shared;
+    int prefix_tiles, prefix_splits, prefix_min_steps;
+    float* prefix_o;   // [prefix_splits][B Hkv T G][Dv]
+    float* prefix_ml;  // [prefix_splits][B Hkv T G][2]
+
+    // Selected pages (kSelected): row (b, hk, t) of `selected` lists the pages,
+    // by their places in b's table row, whose keys the token sees. B counts tokens
+    // then (of `tokens` per sequence) and T is 1.
+    const int32_t* selected;
+    int num_selected, tokens;
+};
+
+// Where a tile's rows find their keys.
+enum StreamSource {
+    kContiguous,
+    kPaged,
+    kTail,      // paged, behind what the sequence's group shares
+    kPrefix,    // the pages that a group shares; rows of all its sequences
+    kSelected,  // selected pages
 };
 
 constexpr int kStreamThreads = 256;
@@ -59,6 +86,51 @@ int stream_tile_rows(int dtype, int kernel_dim, int rows);
 // Keys of a wavefront's step.
 int stream_step_keys(int dtype, int kernel_dim);
 hipError_t launch_stream(const StreamArgs& a, int dtype, hipStream_t s);
+
+// Attention over groups of sequences that share pages, and over selected pages.
+// The prefix writes its partial rows (prefix_*); the tail's launch reads the rest
+// and joins both.
+int prefix_tile_rows(const StreamArgs& a, int dtype);
+hipError_t launch_stream_prefix(const StreamArgs& a, int dtype, hipStream_t s);
+hipError_t launch_stream_tail(const StreamArgs& a, int dtype, hipStream_t s);
+hipError_t launch_stream_selected(const StreamArgs& a, int dtype, hipStream_t s);
+
+// Bounds of the keys of pages: the pages that hold the last counts[b] tokens of each
+// sequence (`touched` of them at most). bounds [page][head][lo, hi][D].
+struct PageBoundsArgs {
+    const void* k_pages;
+    void* bounds;
+    int64_t k_sp, k_sh, k_st;  // page, head, token
+    int64_t b_sp, b_sh, b_st;  // page, head, from lo to hi
+    const int32_t* table;
+    int64_t table_stride;
+    int num_pages, page_shift, max_pages;
+    const int32_t* lengths;
+    const int32_t* counts;  // or null: T
+    int B, Hkv, T, D, touched;
+};
+bool page_bounds_fits(const PageBoundsArgs& a);
+hipError_t launch_page_bounds(const PageBoundsArgs& a, int dtype, hipStream_t s);
+
+// `pages` places of the table's row for each (b, hk, t): the first and the recent
+// ones of those with keys up to the token, and the others of the highest score.
+struct SelectArgs {
+    const void* q;
+    const void* bounds;
+    int32_t* selected;  // [B][Hkv][T][pages], ascending, then -1
+    uint32_t* scores;   // [B][Hkv][T][max_pages]
+    int64_t q_sb, q_sh, q_st;
+    int64_t b_sp, b_sh, b_st;
+    const int32_t* table;
+    int64_t table_stride;
+    int num_pages, page_shift, max_pages;
+    const int32_t* lengths;
+    int B, Hkv, G, T, D;
+    int pages, first_pages, recent_pages;
+    int negative;  // scores of -q
+};
+bool page_select_fits(const SelectArgs& a);
+hipError_t launch_page_select(const SelectArgs& a, int dtype, hipStream_t s);
 
 // Prompts on the matrix cores with K and V staged through LDS (window_fwd.hip).
 struct WindowArgs {

@@ -128,11 +128,12 @@ class PagePool:
 
 class PagedCache:
     """The K and V pools of `layers` layers, [layers, P, Hkv, S, D], and the
-    sequences in them. Copies run on the current stream; a program that uses the
+    sequences in them; with `bounds` also the bounds of the pages' keys, [layers, P,
+    Hkv, 2, D], which batches keep up to date and attend_selected reads. Copies run on the current stream; a program that uses the
     cache from several streams orders them itself."""
 
     def __init__(self, *, layers: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int,
-                 value_dim: int | None = None, dtype=None, device="cuda"):
+                 value_dim: int | None = None, dtype=None, device="cuda", bounds: bool = False):
         import torch
         self._torch = torch
         self.pool = PagePool(num_pages, page_size)
@@ -143,6 +144,9 @@ class PagedCache:
         # (zeros: what a page holds past its tokens is never seen, but a program may look)
         self.k_pages = torch.zeros((*shape, head_dim), dtype=dtype, device=device)
         self.v_pages = torch.zeros((*shape, head_dim if value_dim is None else value_dim), dtype=dtype, device=device)
+        self.k_bounds = None
+        if bounds:
+            self.k_bounds = torch.zeros((layers, num_pages, kv_heads, 2, head_dim), dtype=dtype, device=device)
 
     def add(self) -> int:
         return self.pool.add()
@@ -158,8 +162,9 @@ class PagedCache:
 
     def _copy(self, src, dst):
         if src:
-            for pages in (self.k_pages, self.v_pages):
-                F.copy_pages(list(pages.unbind(0)), src, dst)
+            for pages in (self.k_pages, self.v_pages, self.k_bounds):
+                if pages is not None:
+                    F.copy_pages(list(pages.unbind(0)), src, dst)
 
     def compact(self, most: int | None = None) -> int:
         """Moves pages in use to the front of the pools; returns how many moved.
@@ -189,6 +194,7 @@ class CacheBatch:
         longest = max(cache.pool.length(s) for s in sequences)
         rows, lengths = cache.pool.table(sequences, max(1, -(-longest // size)))
         device = cache.k_pages.device
+        self._rows, self._groups = rows, None
         self.page_table = torch.tensor(rows, dtype=torch.int32, device=device)
         self.lengths = torch.tensor(lengths, dtype=torch.int32, device=device)
         self.counts = torch.tensor(list(tokens), dtype=torch.int32, device=device)
@@ -202,13 +208,21 @@ class CacheBatch:
         self._check_tokens(k)
         F.cache_write(k, v, self.cache.k_pages[layer], self.cache.v_pages[layer], self.page_table, self.lengths,
                       counts=self.counts)
+        self._renew_bounds(layer)
+
+    def _renew_bounds(self, layer: int) -> None:
+        if self.cache.k_bounds is not None and self._most > 0:
+            F.page_bounds(self.cache.k_pages[layer], self.cache.k_bounds[layer], self.page_table, self.lengths,
+                          tokens=self._most, counts=self.counts)
 
     def append(self, layer: int, k, v, rotary, q=None):
         """`write` with K turned by `rotary` (a Rotary) on the way. Returns q
         [B,H,T,D], the queries of the same tokens, turned too (None without)."""
         self._check_tokens(k)
-        return F.cache_append(k, v, self.cache.k_pages[layer], self.cache.v_pages[layer], self.page_table, self.lengths,
-                              rotary, q=q, counts=self.counts)
+        q = F.cache_append(k, v, self.cache.k_pages[layer], self.cache.v_pages[layer], self.page_table, self.lengths,
+                           rotary, q=q, counts=self.counts)
+        self._renew_bounds(layer)
+        return q
 
     def attend(self, layer: int, q, **options):
         """q: [B,H,T,D], the last T of the batch's new tokens of each sequence; options as
@@ -216,7 +230,53 @@ class CacheBatch:
         laid out as write takes them, from the front, would be attended at positions
         from the back (such batches go in parts of one T, or prompts through
         window_attention with the batch's lengths)."""
-        if q.dim() == 4 and q.shape[2] > self._fewest:
-            raise ValueError(f"q has {q.shape[2]} tokens per sequence, the batch {self._fewest} new ones for some")
+        self._check_queries(q)
         return F.paged_attention(q, self.cache.k_pages[layer], self.cache.v_pages[layer], self.page_table,
                                  self.lengths, **options)
+
+    def _check_queries(self, q) -> None:
+        if q.dim() == 4 and q.shape[2] > self._fewest:
+            raise ValueError(f"q has {q.shape[2]} tokens per sequence, the batch {self._fewest} new ones for some")
+
+    @property
+    def groups(self) -> F.PrefixGroups:
+        """Neighbouring sequences that begin with the same pages (forks), in groups
+        that together save the most reading: a sequence joins the group before it when
+        the group's shared pages, times the sequences after its first, do not get
+        fewer by it."""
+        if self._groups is None:
+            size, groups = self.cache.pool.page_size, []
+            first, count, shared = self._rows[0], 1, None
+            for row in self._rows[1:]:
+                common = 0
+                for a, b in zip(first if shared is None else first[:shared], row):
+                    if a != b or a < 0:
+                        break
+                    common += 1
+                if common > 0 and (shared is None or count * common >= (count - 1) * shared):
+                    count, shared = count + 1, common
+                else:
+                    groups.append((count, (shared or 0) * size))
+                    first, count, shared = row, 1, None
+            groups.append((count, (shared or 0) * size))
+            self._groups = F.PrefixGroups(groups, page_size=size, device=self.page_table.device)
+        return self._groups
+
+    def attend_shared(self, layer: int, q, **options):
+        """`attend`, with the pages that forks share read once for all of them."""
+        self._check_queries(q)
+        return F.shared_prefix_attention(q, self.cache.k_pages[layer], self.cache.v_pages[layer], self.page_table,
+                                         self.lengths, groups=self.groups, **options)
+
+    def attend_selected(self, layer: int, q, *, pages: int, selected=None, out=None, stream=None, **options):
+        """`attend` over `pages` of each sequence's pages, of a cache with bounds;
+        options as SelectedAttention."""
+        self._check_queries(q)
+        if self.cache.k_bounds is None:
+            raise ValueError("the cache has no bounds (PagedCache(bounds=True))")
+        if q.dim() != 4:
+            raise ValueError("q must be a rank-4 tensor")
+        attend = F.SelectedAttention(self.cache.k_pages[layer], self.cache.v_pages[layer], self.cache.k_bounds[layer],
+                                     self.page_table, self.lengths, heads=q.shape[1], query_tokens=q.shape[2], pages=pages,
+                                     **options)
+        return attend(q, selected=selected, out=out, stream=stream)

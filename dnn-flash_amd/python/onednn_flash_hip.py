@@ -53,6 +53,16 @@ EXPORTED_SYMBOLS = (
     "ofh_paged_attention_fwd",
     "ofh_cache_write_params_init",
     "ofh_cache_write",
+    "ofh_prefix_groups_init",
+    "ofh_shared_prefix_workspace_bytes",
+    "ofh_shared_prefix_attention_fwd",
+    "ofh_selected_attention_workspace_bytes",
+    "ofh_selected_attention_fwd",
+    "ofh_page_bounds_params_init",
+    "ofh_page_bounds",
+    "ofh_select_params_init",
+    "ofh_select_pages_workspace_bytes",
+    "ofh_select_pages",
     "ofh_rotary_params_init",
     "ofh_rotary_fwd",
     "ofh_cache_append_params_init",
@@ -252,6 +262,61 @@ class CacheWriteParams(ctypes.Structure):
     ]
 
 
+class PrefixGroupsParams(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("groups", ctypes.c_size_t),
+        ("starts", ctypes.c_void_p),
+        ("shared_tokens", ctypes.c_void_p),
+        ("least_shared", ctypes.c_size_t),
+        ("most_shared", ctypes.c_size_t),
+    ]
+
+
+class PageBoundsParams(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("batch", ctypes.c_size_t),
+        ("kv_heads", ctypes.c_size_t),
+        ("tokens", ctypes.c_size_t),
+        ("head_dim", ctypes.c_size_t),
+        ("num_pages", ctypes.c_size_t),
+        ("page_size", ctypes.c_size_t),
+        ("max_pages", ctypes.c_size_t),
+        ("table_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("k_page_strides", ctypes.c_int64 * 3),
+        ("bounds_strides", ctypes.c_int64 * 3),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+    ]
+
+
+class SelectParams(ctypes.Structure):
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32),
+        ("batch", ctypes.c_size_t),
+        ("heads", ctypes.c_size_t),
+        ("kv_heads", ctypes.c_size_t),
+        ("query_tokens", ctypes.c_size_t),
+        ("head_dim", ctypes.c_size_t),
+        ("num_pages", ctypes.c_size_t),
+        ("page_size", ctypes.c_size_t),
+        ("max_pages", ctypes.c_size_t),
+        ("table_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("negative", ctypes.c_int32),
+        ("q_strides", ctypes.c_int64 * 3),
+        ("bounds_strides", ctypes.c_int64 * 3),
+        ("page_table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("pages", ctypes.c_size_t),
+        ("first_pages", ctypes.c_size_t),
+        ("recent_pages", ctypes.c_size_t),
+    ]
+
+
 class RotaryFields(ctypes.Structure):
     _fields_ = [
         ("frequencies", ctypes.c_void_p),
@@ -342,6 +407,16 @@ def lib() -> ctypes.CDLL:
                 ("ofh_paged_attention_fwd", ctypes.c_int, [vp] * 6 + [sz, vp]),
                 ("ofh_cache_write_params_init", None, [vp]),
                 ("ofh_cache_write", ctypes.c_int, [vp] * 6),
+                ("ofh_prefix_groups_init", None, [vp]),
+                ("ofh_shared_prefix_workspace_bytes", ctypes.c_int, [vp, vp, szs]),
+                ("ofh_shared_prefix_attention_fwd", ctypes.c_int, [vp] * 7 + [sz, vp]),
+                ("ofh_selected_attention_workspace_bytes", ctypes.c_int, [vp, sz, szs]),
+                ("ofh_selected_attention_fwd", ctypes.c_int, [vp, vp, sz] + [vp] * 5 + [sz, vp]),
+                ("ofh_page_bounds_params_init", None, [vp]),
+                ("ofh_page_bounds", ctypes.c_int, [vp] * 4),
+                ("ofh_select_params_init", None, [vp]),
+                ("ofh_select_pages_workspace_bytes", ctypes.c_int, [vp, szs]),
+                ("ofh_select_pages", ctypes.c_int, [vp] * 5 + [sz, vp]),
                 ("ofh_rotary_params_init", None, [vp]),
                 ("ofh_rotary_fwd", ctypes.c_int, [vp] * 4),
                 ("ofh_cache_append_params_init", None, [vp]),
@@ -770,9 +845,9 @@ def _new_workspace(torch, need, device, stream):
         return torch.empty(need, dtype=torch.uint8, device=device)
 
 
-def _workspace_need(query, p) -> int:
+def _workspace_need(query, p, *more) -> int:
     need = ctypes.c_size_t()
-    rc = query(p if isinstance(p, bytes) else ctypes.addressof(p), ctypes.byref(need))
+    rc = query(p if isinstance(p, bytes) else ctypes.addressof(p), *more, ctypes.byref(need))
     if rc != OFH_SUCCESS:
         check(rc)
     return need.value
@@ -912,9 +987,13 @@ class PagedAttention:
         p.window, p.sink_tokens, p.max_key_splits = window, sink_tokens, max_key_splits
         p.out_dtype = _DTYPE_CODES[self._out_dtype]
         self._params = bytes(p)
-        self._need = _workspace_need(L.ofh_paged_attention_workspace_bytes, p)
-        self._fwd = L.ofh_paged_attention_fwd
         self._ptrs = (k_pages.data_ptr(), v_pages.data_ptr())
+        self._plan(L, p)
+
+    def _plan(self, L, p: PagedParams) -> None:
+        """The entry, its arguments behind the parameters, and the scratch it needs."""
+        self._fwd, self._more = L.ofh_paged_attention_fwd, ()
+        self._need = _workspace_need(L.ofh_paged_attention_workspace_bytes, p)
 
     @property
     def workspace_bytes(self) -> int:
@@ -922,10 +1001,17 @@ class PagedAttention:
 
     def __call__(self, q, *, out=None, workspace=None, stream=None):
         """q: [B,H,T,D] in the cache's dtype. Returns out, [B,H,T,Dv]."""
+        self._check_query(q)
+        return self._attend(q, self._more, out, workspace, stream)
+
+    def _check_query(self, q) -> None:
         torch, dev = self._torch, self._device
         if not (_is_rows(torch, q, self._dtype, dev) and q.shape == self._q_shape):
             raise ValueError(f"q must be a {self._dtype} tensor of shape {self._q_shape} on {dev}, its last axis "
                              "contiguous and strides non-negative")
+
+    def _attend(self, q, more, out, workspace, stream):
+        torch, dev = self._torch, self._device
         p = PagedParams.from_buffer_copy(self._params)  # (its own: calls may run on several threads)
         if not q.is_contiguous():
             p.q_strides[:] = _axis_strides("q", q)
@@ -941,8 +1027,8 @@ class PagedAttention:
         elif self._need:
             workspace = _new_workspace(torch, self._need, dev, stream)
             ws, ws_bytes = workspace.data_ptr(), self._need
-        rc = _launch(torch, dev, stream, self._fwd, ctypes.addressof(p), q.data_ptr(), *self._ptrs, out.data_ptr(), ws,
-                     ws_bytes)
+        rc = _launch(torch, dev, stream, self._fwd, ctypes.addressof(p), *more, q.data_ptr(), *self._ptrs, out.data_ptr(),
+                     ws, ws_bytes)
         if rc != OFH_SUCCESS:
             check(rc)
         return out
@@ -960,6 +1046,221 @@ def paged_attention(q, k_pages, v_pages, page_table, lengths, *, window: int = 0
                           window=window, sink_tokens=sink_tokens, scale=scale, alibi_slopes=alibi_slopes,
                           softcap=softcap, out_dtype=out_dtype, max_key_splits=max_key_splits)(
                               q, out=out, workspace=workspace, stream=stream)
+
+
+class PrefixGroups:
+    """Which sequences of a batch share prefixes: (sequences, shared tokens) of each
+    group, in the batch's order. The sequences of a group have their first shared
+    tokens, whole pages of the cache, in the same pages (0: they share nothing).
+    Kept on `device` for the calls that take it."""
+
+    def __init__(self, groups, *, page_size: int, device="cuda"):
+        torch = _torch()
+        groups = [tuple(g) for g in groups]
+        for g in groups:
+            if len(g) != 2 or any(type(x) is not int for x in g) or g[0] <= 0 or not 0 <= g[1] < 1 << 31:
+                raise ValueError("groups must be pairs of a positive number of sequences and a number of shared tokens")
+            if g[1] % page_size:
+                raise ValueError("shared tokens must be whole pages")
+        if not groups:
+            raise ValueError("groups must not be empty")
+        self.groups = groups
+        self.batch = sum(n for n, _ in groups)
+        starts, shared = [0], []
+        for n, tokens in groups:
+            starts.append(starts[-1] + n)
+            shared += [tokens] * n
+        self._held = tuple(torch.tensor(x, dtype=torch.int32, device=device) for x in (starts, shared))
+        p = PrefixGroupsParams()
+        lib().ofh_prefix_groups_init(ctypes.addressof(p))
+        p.groups, p.starts, p.shared_tokens = len(groups), *(t.data_ptr() for t in self._held)
+        p.least_shared, p.most_shared = min(shared), max(shared)
+        self._params = p
+
+
+class SharedPrefixAttention(PagedAttention):
+    """PagedAttention of a batch whose sequences share prefixes: the keys that a
+    group of sequences has in common are read once for all of it. The result is
+    PagedAttention's, up to rounding. groups: a PrefixGroups, or its list of
+    (sequences, shared tokens)."""
+
+    def __init__(self, k_pages, v_pages, page_table, lengths, *, groups, heads: int, query_tokens: int = 1, **options):
+        self._groups_given = groups
+        super().__init__(k_pages, v_pages, page_table, lengths, heads=heads, query_tokens=query_tokens, **options)
+
+    def _plan(self, L, p: PagedParams) -> None:
+        groups = self._groups_given
+        if not isinstance(groups, PrefixGroups):
+            groups = PrefixGroups(groups, page_size=p.page_size, device=self._device)
+        if groups.batch != p.batch:
+            raise ValueError(f"groups must have the batch's {p.batch} sequences together")
+        if groups._held[0].device != self._device:
+            raise ValueError(f"groups must be on {self._device}")
+        if any(tokens % p.page_size or tokens > p.max_pages * p.page_size for _, tokens in groups.groups):
+            raise ValueError("shared tokens must be whole pages of the table's rows")
+        self._groups = groups
+        self._fwd, self._more = L.ofh_shared_prefix_attention_fwd, (ctypes.addressof(groups._params),)
+        self._need = _workspace_need(L.ofh_shared_prefix_workspace_bytes, p, *self._more)
+
+
+def shared_prefix_attention(q, k_pages, v_pages, page_table, lengths, *, groups, out=None, out_dtype=None, workspace=None,
+                            stream=None, **options):
+    """One call of SharedPrefixAttention: q [B,H,T,D], the T new tokens of each sequence."""
+    if q.dim() != 4:
+        raise ValueError("q must be a rank-4 tensor")
+    if out is not None and out_dtype is not None and out.dtype != out_dtype:
+        raise ValueError("out and out_dtype disagree")
+    return SharedPrefixAttention(k_pages, v_pages, page_table, lengths, groups=groups, heads=q.shape[1],
+                                 query_tokens=q.shape[2], out_dtype=out_dtype, **options)(
+                                     q, out=out, workspace=workspace, stream=stream)
+
+
+def _check_bounds(torch, k_pages, k_bounds):
+    _check_rows(torch, "k_bounds", k_bounds, 4, k_pages.dtype, k_pages.device)
+    P, Hkv, _, D = k_pages.shape
+    if k_bounds.shape != (P, Hkv, 2, D):
+        raise ValueError("k_bounds must be [P, Hkv, 2, D]")
+
+
+class PageBounds:
+    """Keeps what SelectedAttention scores pages by: k_bounds [P,Hkv,2,D], the
+    smallest and the largest value of every column of a page's keys (NaN where one
+    is). Each call renews those of the pages that hold the last counts[b] tokens of
+    each sequence (`tokens` without counts, which are at most that): what a
+    cache_write of these tokens is followed by. The page's own tokens count, up to
+    lengths[b]; sequences that share a page agree on them."""
+
+    def __init__(self, k_pages, k_bounds, page_table, lengths, *, tokens: int, counts=None):
+        torch = _torch()
+        _check_pool(torch, k_pages, k_pages, page_table, lengths)
+        _check_bounds(torch, k_pages, k_bounds)
+        _check_written("k_bounds", k_bounds)
+        if type(tokens) is not int or not 0 < tokens < 1 << 63:
+            raise ValueError("tokens must be a positive integer")
+        P, Hkv, S, D = k_pages.shape
+        B, max_pages = page_table.shape
+        if counts is not None:
+            _check_ints(torch, "counts", counts, (B,), k_pages.device)
+        self._torch, self._device = torch, k_pages.device
+        self._held = (k_pages, k_bounds, page_table, lengths, counts)
+        p = PageBoundsParams()
+        L = lib()
+        L.ofh_page_bounds_params_init(ctypes.addressof(p))
+        p.batch, p.kv_heads, p.tokens, p.head_dim = B, Hkv, tokens, D
+        p.num_pages, p.page_size, p.max_pages, p.table_stride = P, S, max_pages, page_table.stride(0) if B > 1 else 0
+        p.dtype = _DTYPE_CODES[k_pages.dtype]
+        p.k_page_strides[:], p.bounds_strides[:] = _axis_strides("k_pages", k_pages), _axis_strides("k_bounds", k_bounds)
+        p.page_table, p.lengths = page_table.data_ptr(), lengths.data_ptr()
+        if counts is not None:
+            p.counts = counts.data_ptr()
+        self._params = p  # (read by calls, never changed)
+        self._args = (ctypes.addressof(p), k_pages.data_ptr(), k_bounds.data_ptr())
+        self._update = L.ofh_page_bounds
+
+    def __call__(self, *, stream=None) -> None:
+        rc = _launch(self._torch, self._device, stream, self._update, *self._args)
+        if rc != OFH_SUCCESS:
+            check(rc)
+
+
+def page_bounds(k_pages, k_bounds, page_table, lengths, *, tokens: int | None = None, counts=None, stream=None) -> None:
+    """One call of PageBounds; without `tokens` it renews every page of the sequences."""
+    if tokens is None:
+        tokens = 1 << 30  # (the most that a sequence has)
+    PageBounds(k_pages, k_bounds, page_table, lengths, tokens=tokens, counts=counts)(stream=stream)
+
+
+class SelectedAttention(PagedAttention):
+    """Sparse attention of new tokens over a paged cache: each token attends, for
+    each key-value head, to `pages` of its sequence's pages: the first
+    `first_pages`, the last `recent_pages` of those with keys up to the token's
+    position, and between them those of the highest score (all when there are at
+    most `pages`). The score bounds q.k over a page from its k_bounds (PageBounds):
+    the largest, over the query heads of the key-value head, of
+    sum_d q_d (q_d > 0 ? hi_d : lo_d); ties go to the lower page. Scores leave
+    ALiBi and the soft-cap out. Otherwise as PagedAttention, without a window."""
+
+    def __init__(self, k_pages, v_pages, k_bounds, page_table, lengths, *, heads: int, pages: int, first_pages: int = 1,
+                 recent_pages: int = 2, query_tokens: int = 1, scale: float | None = None, alibi_slopes=None,
+                 softcap: float = 0.0, out_dtype=None, max_key_splits: int = 0):
+        torch = _torch()
+        _check_pool(torch, k_pages, v_pages, page_table, lengths)
+        _check_bounds(torch, k_pages, k_bounds)
+        _check_counts(pages=pages, first_pages=first_pages, recent_pages=recent_pages)
+        if pages == 0 or first_pages + recent_pages > pages:
+            raise ValueError("pages must be positive and hold first_pages and recent_pages together")
+        self._pages, self._select_pages = pages, (first_pages, recent_pages)
+        self._bounds = k_bounds
+        super().__init__(k_pages, v_pages, page_table, lengths, heads=heads, query_tokens=query_tokens, scale=scale,
+                         alibi_slopes=alibi_slopes, softcap=softcap, out_dtype=out_dtype, max_key_splits=max_key_splits)
+
+    def _plan(self, L, p: PagedParams) -> None:
+        s = SelectParams()
+        L.ofh_select_params_init(ctypes.addressof(s))
+        for name in ("batch", "heads", "kv_heads", "query_tokens", "head_dim", "num_pages", "page_size", "max_pages",
+                     "table_stride", "dtype", "page_table", "lengths"):
+            setattr(s, name, getattr(p, name))
+        s.bounds_strides[:] = _axis_strides("k_bounds", self._bounds)
+        s.negative = int(p.scale < 0)
+        s.pages, (s.first_pages, s.recent_pages) = self._pages, self._select_pages
+        self._select_params = bytes(s)
+        self._select = L.ofh_select_pages
+        self._select_need = _workspace_need(L.ofh_select_pages_workspace_bytes, s)
+        self._selected_shape = (p.batch, p.kv_heads, p.query_tokens, self._pages)
+        self._fwd, self._more = L.ofh_selected_attention_fwd, ()
+        self._need = _workspace_need(L.ofh_selected_attention_workspace_bytes, p, self._pages)
+
+    @property
+    def select_workspace_bytes(self) -> int:
+        return self._select_need
+
+    def _check_selected(self, selected) -> None:
+        _check_ints(self._torch, "selected", selected, self._selected_shape, self._device)
+        if not selected.is_contiguous():
+            raise ValueError("selected must be contiguous")
+
+    def _run_select(self, q, address, workspace, stream) -> None:
+        torch, dev = self._torch, self._device
+        s = SelectParams.from_buffer_copy(self._select_params)
+        if not q.is_contiguous():
+            s.q_strides[:] = _axis_strides("q", q)
+        ws, ws_bytes = None, 0
+        if workspace is not None:
+            ws, ws_bytes = _given_workspace(torch, workspace, q)
+        elif self._select_need:
+            workspace = _new_workspace(torch, self._select_need, dev, stream)
+            ws, ws_bytes = workspace.data_ptr(), self._select_need
+        rc = _launch(torch, dev, stream, self._select, ctypes.addressof(s), q.data_ptr(), self._bounds.data_ptr(), address,
+                     ws, ws_bytes)
+        if rc != OFH_SUCCESS:
+            check(rc)
+
+    def select(self, q, *, out=None, workspace=None, stream=None):
+        """The pages that the tokens of q [B,H,T,D] attend to: int32
+        [B,Hkv,T,pages], places in the sequence's row of the page table, ascending,
+        then -1. workspace: of select_workspace_bytes."""
+        self._check_query(q)
+        if out is None:
+            out = self._torch.empty(self._selected_shape, dtype=self._torch.int32, device=self._device)
+        else:
+            self._check_selected(out)
+        self._run_select(q, out.data_ptr(), workspace, stream)
+        return out
+
+    def __call__(self, q, *, selected=None, out=None, workspace=None, stream=None):
+        """q: [B,H,T,D] in the cache's dtype. selected: of select() for these or other
+        queries (several layers or steps may share one), or of the program's own
+        making; without it the call selects. Returns out, [B,H,T,Dv]. workspace: of
+        workspace_bytes, for the attention."""
+        self._check_query(q)
+        if selected is None:
+            held = _new_workspace(self._torch, 4 * math.prod(self._selected_shape), self._device, stream)
+            address = held.data_ptr()
+            self._run_select(q, address, None, stream)
+        else:
+            self._check_selected(selected)
+            address = selected.data_ptr()
+        return self._attend(q, (address, self._pages), out, workspace, stream)
 
 
 class CacheWriter:

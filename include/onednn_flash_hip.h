@@ -362,6 +362,92 @@ int ofh_paged_attention_workspace_bytes(const ofh_paged_params* p, size_t* bytes
 int ofh_paged_attention_fwd(const ofh_paged_params* p, const void* q, const void* k_pages, const void* v_pages,
                             void* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Attention of a batch whose sequences share prefixes: ofh_paged_attention_fwd,
+ * with the keys that a group of sequences has in common read once for all of it.
+ * The result is that call's, up to rounding. */
+typedef struct ofh_prefix_groups {
+    uint32_t struct_size; /* set by ofh_prefix_groups_init */
+    size_t groups;        /* 1 to batch */
+    /* Device int32 [groups + 1]: group g has the sequences [starts[g], starts[g + 1]),
+     * from starts[0] = 0 to starts[groups] = batch. */
+    const int32_t* starts;
+    /* Device int32 [batch], one number for the sequences of a group: each of them
+     * has its first shared_tokens[b] keys in the pages that the group's first
+     * sequence has them in. Taken down to whole pages; 0 shares nothing. (Numbers
+     * that differ within a group leave its rows undefined, inside their memory.) */
+    const int32_t* shared_tokens;
+    /* The least and the most of them, as the host knows them: how the work is
+     * divided goes by these, the result does not. */
+    size_t least_shared, most_shared;
+} ofh_prefix_groups;
+
+void ofh_prefix_groups_init(ofh_prefix_groups* g);
+
+/* Partial rows: this call always has scratch. With workspace NULL it is the
+ * library's of the stream; under graph capture a call that does not fit it fails
+ * with OFH_ERROR_WORKSPACE_TOO_SMALL. */
+int ofh_shared_prefix_workspace_bytes(const ofh_paged_params* p, const ofh_prefix_groups* g, size_t* bytes);
+int ofh_shared_prefix_attention_fwd(const ofh_paged_params* p, const ofh_prefix_groups* g, const void* q,
+                                    const void* k_pages, const void* v_pages, void* out, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* Attention over selected pages: token t of sequence b sees, for the query heads
+ * of key-value head h, the keys up to its position that are in the pages selected
+ * [b][h][t][0 .. pages) (device int32, contiguous): places in b's table row,
+ * strictly ascending, then -1. Entries outside the row, or not above the one
+ * before, select nothing. Otherwise as ofh_paged_attention_fwd, without a window. */
+int ofh_selected_attention_workspace_bytes(const ofh_paged_params* p, size_t pages, size_t* bytes);
+int ofh_selected_attention_fwd(const ofh_paged_params* p, const int32_t* selected, size_t pages, const void* q,
+                               const void* k_pages, const void* v_pages, void* out, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* What selects them. The bounds of a page are the smallest and the largest value
+ * of every column of its keys (NaN where one is): bounds[page, kv_head, 2, head_dim],
+ * lo then hi, in the cache's type. This call writes the bounds of the pages that
+ * hold the last counts[b] tokens of each sequence, over the tokens that it has in
+ * them. Head dims as the attention's, 16-byte rows. */
+typedef struct ofh_page_bounds_params {
+    uint32_t struct_size; /* set by ofh_page_bounds_params_init */
+    size_t batch, kv_heads, tokens, head_dim;
+    size_t num_pages, page_size, max_pages;
+    int64_t table_stride;
+    int32_t dtype;
+    int64_t k_page_strides[3]; /* page, head, token; all zero: contiguous */
+    int64_t bounds_strides[3]; /* page, head, lo to hi; all zero: contiguous */
+    const int32_t* page_table;
+    const int32_t* lengths;
+    const int32_t* counts; /* device [B], taken between 0 and tokens, or NULL: tokens */
+} ofh_page_bounds_params;
+
+void ofh_page_bounds_params_init(ofh_page_bounds_params* p);
+int ofh_page_bounds(const ofh_page_bounds_params* p, const void* k_pages, void* bounds, void* stream);
+
+/* selected[b][h][t][pages]: of the pages with keys up to token t's position, all
+ * when they are at most `pages`; else the first first_pages, the last recent_pages,
+ * and between them those of the highest score, ties to the lower page. Score: the
+ * largest, over the query heads of h, of sum_d q_d (q_d > 0 ? hi_d : lo_d), summed
+ * in 64 bits and rounded to fp32 (`negative`: of -q, for a negative scale). NaN
+ * scores are above all others, pages outside the pool below. */
+typedef struct ofh_select_params {
+    uint32_t struct_size; /* set by ofh_select_params_init */
+    size_t batch, heads, kv_heads, query_tokens, head_dim;
+    size_t num_pages, page_size, max_pages;
+    int64_t table_stride;
+    int32_t dtype;
+    int32_t negative;
+    int64_t q_strides[3];      /* batch, head, token; all zero: contiguous */
+    int64_t bounds_strides[3];
+    const int32_t* page_table;
+    const int32_t* lengths;    /* as ofh_paged_params' */
+    size_t pages, first_pages, recent_pages; /* first and recent: at most `pages` together */
+} ofh_select_params;
+
+void ofh_select_params_init(ofh_select_params* p);
+int ofh_select_pages_workspace_bytes(const ofh_select_params* p, size_t* bytes);
+/* workspace: as ofh_shared_prefix_attention_fwd's. */
+int ofh_select_pages(const ofh_select_params* p, const void* q, const void* bounds, int32_t* selected, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
 /* New rows into the pages: token t < counts[b] of sequence b goes to position
  * lengths[b] - counts[b] + t. K[B,Hkv,T,D] and V[B,Hkv,T,Dv] of any alignment.
  * Tokens whose position is negative or past the table's row, or whose page is
