@@ -88,7 +88,7 @@ int ofh_rotary_fwd(const ofh_rotary_params* p, const void* x, void* out, void* s
         a.pos_sb = p->position_stride;
         a.lengths = p->lengths;
         a.offset = p->offset;
-        if (!ofh::rotary_fits(a, p->dtype)) return unsupported("rotary call exceeds the launch range");
+        if (!ofh::rotary_fits(a)) return unsupported("rotary call exceeds the launch range");
         OFH_HIP_CHECK(ofh::launch_rotary(a, p->dtype, static_cast<hipStream_t>(stream)));
         return OFH_SUCCESS;
     });
@@ -130,7 +130,7 @@ int ofh_cache_append(const ofh_cache_append_params* p, const void* k, const void
         a.H = (int)p->heads;
         a.D = (int)p->cache.head_dim;
         a.Dv = (int)p->cache.value_dim;
-        if (!ofh::cache_append_fits(a, p->cache.dtype)) return unsupported("cache append exceeds the launch range");
+        if (!ofh::cache_append_fits(a)) return unsupported("cache append exceeds the launch range");
         OFH_HIP_CHECK(ofh::launch_cache_append(a, p->cache.dtype, static_cast<hipStream_t>(stream)));
         return OFH_SUCCESS;
     });

@@ -7,8 +7,10 @@
 // hi and lo the columns' largest and smallest values in the page. The sum is
 // formed in 64 bits and rounded to fp32: its order then decides no rank.
 
-#include "serving_kernels.h"
+#include <algorithm>
+
 #include "flash_wave32.h"
+#include "serving_kernels.h"
 
 namespace ofh {
 namespace {
@@ -119,66 +121,103 @@ __device__ __forceinline__ double dpp(double x) {
     const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(u >> 32), CTRL, 0xf, 0xf, true);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-// Sum over `lanes` neighbouring lanes, valid in the first of them.
+// Sum over `lanes` neighbouring lanes (up to 16), valid in the first of them.
 __device__ __forceinline__ double sum_lanes(double x, int lanes) {
     if (lanes >= 2) x += dpp<0xB1>(x);   // quad_perm [1,0,3,2]
     if (lanes >= 4) x += dpp<0x4E>(x);   // quad_perm [2,3,0,1]
     if (lanes >= 8) x += dpp<0x104>(x);  // row_shl:4
     if (lanes >= 16) x += dpp<0x108>(x); // row_shl:8
-    if (lanes >= 32) x += __shfl_xor(x, 16);
-    if (lanes >= 64) x += __shfl_xor(x, 32);
     return x;
 }
 
-constexpr int kScorePages = 64;     // of a workgroup
-constexpr int kScoreQuery = 8192;   // numbers of Q that a workgroup keeps: 64 KB
+// Bits of x where m has ones, of y elsewhere. (Written as such: the compiler takes
+// the select apart again into two masks and an or for every other column.)
+__device__ __forceinline__ unsigned bit_select(unsigned m, unsigned x, unsigned y) {
+    unsigned r;
+    asm("v_bfi_b32 %0, %1, %2, %3" : "=v"(r) : "v"(m), "v"(x), "v"(y));
+    return r;
+}
 
-// A workgroup scores up to 64 pages for one token and key-value head. Q is in LDS in
-// 64 bits; the lanes of a row of bounds take a word of lo and of hi each, and
-// several pages stand beside each other in a wavefront. Tokens that see no more
-// pages than they may take need no scores.
+constexpr int kScoreWords = 4;      // of a bounds row that a lane takes
+constexpr int kScoreQuery = 4096;   // numbers of Q that a workgroup keeps at most: 32 KB
+
+// A workgroup scores up to `per` pages for one token and key-value head. `lanes`
+// neighbouring lanes share a page, each with four words of lo and of hi, so that a
+// sum takes few lane exchanges. Q is in LDS in 64 bits, beside it a mask of its
+// positive numbers in the layout of the bounds, so that hi or lo is one bit select
+// for a word. Tokens that see no more pages than they may take need no scores.
+//
+// What bounds it (bf16, 32 sequences of 2000-32768 tokens, pages of 32, H32/8 D128: 71 MB
+// of bounds, 22.5 us): half the sums, half the reading of 512 bytes here and there
+// (without the sums 17); the same sums in fp32 save nothing. Workgroups are
+// numbered chunk by chunk, since row by row the late chunks, which only long
+// sequences have, fall on the same XCDs: 26.6.
 template <typename T>
-__global__ __launch_bounds__(kSelectThreads) void page_score_kernel(SelectArgs a, int chunks) {
+__global__ __launch_bounds__(kSelectThreads) void page_score_kernel(SelectArgs a, int per, int lanes, int heads_kept) {
     using X = Words<T>;
     constexpr int W = X::W;
-    __shared__ __attribute__((aligned(16))) double q[kScoreQuery];
-    const int64_t row = blockIdx.x / chunks;  // (b, hk, t)
-    const int chunk = (int)(blockIdx.x - row * chunks);
+    extern __shared__ __attribute__((aligned(16))) double q[];
+    u32x4* masks = (u32x4*)(q + heads_kept * a.D);
+    const int rows = a.B * a.Hkv * a.T, chunk = blockIdx.x / rows;
+    const int64_t row = blockIdx.x - (int64_t)chunk * rows;  // (b, hk, t)
     const int t = (int)(row % a.T), hk = (int)(row / a.T % a.Hkv), b = (int)(row / a.T / a.Hkv);
     const int have = candidates(a, b, t);
-    const int page0 = chunk * kScorePages, page1 = min(have, page0 + kScorePages);
+    const int page0 = chunk * per, page1 = min(have, page0 + per);
     if (have <= a.pages || page0 >= have) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int words = a.D / W, lanes = row_lanes(words), beside = 64 / lanes;
-    const int word = min(lane % lanes, words - 1), slot = lane / lanes;
-    const int most = kScoreQuery / a.D;  // heads at a time
-    for (int g0 = 0; g0 < a.G; g0 += most) {
-        const int heads = min(most, a.G - g0);
+    const int words = a.D / W, beside = 64 / lanes;
+    const int sub = lane & (lanes - 1), slot = lane / lanes;
+    for (int g0 = 0; g0 < a.G; g0 += heads_kept) {
+        const int heads = min(heads_kept, a.G - g0);
         __syncthreads();
-        for (int n = threadIdx.x; n < heads * a.D; n += kSelectThreads) {
-            const int g = n / a.D, d = n - g * a.D;
-            const double x = (double)(float)((const T*)a.q)[b * a.q_sb + (int64_t)(hk * a.G + g0 + g) * a.q_sh + t * a.q_st + d];
-            q[n] = a.negative ? -x : x;
+        for (int n = threadIdx.x; n < heads * words; n += kSelectThreads) {
+            const int g = n / words, w = n - g * words;
+            const T* at = (const T*)a.q + b * a.q_sb + (int64_t)(hk * a.G + g0 + g) * a.q_sh + t * a.q_st + w * W;
+            unsigned on[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const float x = a.negative ? -(float)at[j] : (float)at[j];
+                q[n * W + j] = (double)x;
+                on[j] = x > 0.0f ? ~0u : 0u;
+            }
+            u32x4 m;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m[j] = sizeof(T) == 4 ? on[j] : bit_select(0xffffu, on[2 * j % W], on[(2 * j + 1) % W]);
+            masks[n] = m;
         }
         __syncthreads();
         for (int p = page0 + wave * beside + slot; p - slot < page1; p += kSelectWaves * beside) {
-            const int place = min(p, page1 - 1);
-            const int page = a.table[b * a.table_stride + place];
+            const int page = a.table[b * a.table_stride + min(p, page1 - 1)];
             const bool ok = (unsigned)page < (unsigned)a.num_pages;
-            const T* at = (const T*)a.bounds + (ok ? page : 0) * a.b_sp + hk * a.b_sh + word * W;
-            float lo[W], hi[W];
-            X::get(*(const u32x4*)at, lo);
-            X::get(*(const u32x4*)(at + a.b_st), hi);
+            const T* at = (const T*)a.bounds + (ok ? page : 0) * a.b_sp + hk * a.b_sh;
+            u32x4 lo[kScoreWords], hi[kScoreWords];
+#pragma unroll
+            for (int c = 0; c < kScoreWords; ++c) {
+                const int word = min(sub + lanes * c, words - 1);
+                lo[c] = *(const u32x4*)(at + word * W);
+                hi[c] = *(const u32x4*)(at + a.b_st + word * W);
+            }
+#pragma unroll
+            for (int c = 0; c < kScoreWords; ++c)  // a word past the row counts as 0
+                if (sub + lanes * c >= words) lo[c] = hi[c] = u32x4{0u, 0u, 0u, 0u};
             unsigned best = 0;
             for (int g = 0; g < heads; ++g) {
-                const double* x = q + g * a.D + word * W;
-                double sum = 0.0;
+                double sum[2] = {0.0, 0.0};
 #pragma unroll
-                for (int j = 0; j < W; ++j) sum = __builtin_fma(x[j], (double)(x[j] > 0.0 ? hi[j] : lo[j]), sum);
-                if (lane % lanes >= words) sum = 0.0;
-                best = max(best, score_rank((float)sum_lanes(sum, lanes)));
+                for (int c = 0; c < kScoreWords; ++c) {
+                    const int word = g * words + min(sub + lanes * c, words - 1);
+                    const u32x4 m = masks[word];
+                    u32x4 bound;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) bound[j] = bit_select(m[j], hi[c][j], lo[c][j]);
+                    float f[W];
+                    X::get(bound, f);
+#pragma unroll
+                    for (int j = 0; j < W; ++j) sum[j & 1] = __builtin_fma(q[word * W + j], (double)f[j], sum[j & 1]);
+                }
+                best = max(best, score_rank((float)sum_lanes(sum[0] + sum[1], lanes)));
             }
-            if (lane % lanes == 0 && p < page1) {
+            if (sub == 0 && p < page1) {
                 uint32_t* out = a.scores + row * a.max_pages + p;
                 if (!ok) best = 0;
                 *out = g0 > 0 ? max(*out, best) : best;
@@ -189,49 +228,75 @@ __global__ __launch_bounds__(kSelectThreads) void page_score_kernel(SelectArgs a
 
 constexpr int kSelectKept = 16384;  // scores that a workgroup keeps in LDS
 
+// (us, 256 / 512 / 1024 threads: one sequence of 2047 pages 10.8 / 9.4 / 9.9, 32 of up to
+// 1024 pages 8.5 / 8.4 / 9.7)
+constexpr int kPickThreads = 512, kPickWaves = kPickThreads / 64;
+
 // A workgroup per token and key-value head. The need-th highest score of the
-// candidates between the first and the recent ones is found a byte at a time, from
-// the counts of its values among the scores that share the bytes before; then each
-// thread takes a stretch of the candidates, counts what is above and what is equal
-// to it, and after a sum over the threads before writes its share: ascending, ties
-// to the lower page.
-__global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectArgs a) {
+// candidates between the first and the recent ones is found from counts of the
+// scores' bits; then each thread takes a stretch of the candidates, counts what is
+// above and what is equal to it, and after a sum over the threads before writes its
+// share: ascending, ties to the lower page.
+__global__ __launch_bounds__(kPickThreads) void page_select_kernel(SelectArgs a) {
     __shared__ uint32_t kept[kSelectKept];
     __shared__ int count[256];
-    __shared__ int found[2];
-    __shared__ int sums[2][kSelectWaves];
+    __shared__ int found[3];
+    __shared__ int sums[2][kPickWaves];
+    __shared__ uint32_t ends[2][kPickWaves];
     const int64_t row = blockIdx.x;
     const int t = (int)(row % a.T), b = (int)(row / a.T / a.Hkv);
     const int have = candidates(a, b, t);
     int32_t* out = a.selected + row * a.pages;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (have <= a.pages) {
-        for (int i = tid; i < a.pages; i += kSelectThreads) out[i] = i < have ? i : -1;
+        for (int i = tid; i < a.pages; i += kPickThreads) out[i] = i < have ? i : -1;
         return;
     }
     const uint32_t* scores = a.scores + row * a.max_pages + a.first_pages;
     const int n = have - a.first_pages - a.recent_pages, need = a.pages - a.first_pages - a.recent_pages;
     const bool keep = n <= kSelectKept;
-    if (keep)
-        for (int i = tid; i < n; i += kSelectThreads) kept[i] = scores[i];
+    uint32_t low = ~0u, high = 0;
+    if (need > 0)
+        for (int i = tid; i < n; i += kPickThreads) {
+            const uint32_t x = scores[i];
+            if (keep) kept[i] = x;
+            low = min(low, x);
+            high = max(high, x);
+        }
     // (the first and the recent pages)
-    for (int i = tid; i < a.first_pages; i += kSelectThreads) out[i] = i;
-    for (int i = tid; i < a.recent_pages; i += kSelectThreads) out[a.pages - a.recent_pages + i] = have - a.recent_pages + i;
+    for (int i = tid; i < a.first_pages; i += kPickThreads) out[i] = i;
+    for (int i = tid; i < a.recent_pages; i += kPickThreads) out[a.pages - a.recent_pages + i] = have - a.recent_pages + i;
     if (need == 0) return;
     auto score = [&](int i) { return keep ? kept[i] : scores[i]; };
-    uint32_t limit = 0;
-    int rest = need;  // of the scores that share the bytes so far
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        count[tid] = 0;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        low = min(low, (uint32_t)__shfl_xor((int)low, d));
+        high = max(high, (uint32_t)__shfl_xor((int)high, d));
+    }
+    if (lane == 0) {
+        ends[0][wave] = low;
+        ends[1][wave] = high;
+    }
+    __syncthreads();
+    for (int w = 0; w < kPickWaves; ++w) {
+        low = min(low, ends[0][w]);
+        high = max(high, ends[1][w]);
+    }
+    // The need-th highest score, eight bits at a time from the first that differs: of
+    // the scores whose bits from `shift` up are `limit`, `rest` are taken.
+    int shift = low == high ? 0 : 32 - __builtin_clz(low ^ high), rest = need;
+    uint64_t limit = (uint64_t)high >> shift;
+    while (shift > 0) {
+        const int width = min(shift, 8), next = shift - width;
+        if (tid < 256) count[tid] = 0;
         __syncthreads();
-        const uint32_t above = shift == 24 ? 0u : ~0u << (shift + 8);
-        for (int i = tid; i < n; i += kSelectThreads) {
-            const uint32_t x = score(i);
-            if ((x & above) == (limit & above)) atomicAdd(&count[x >> shift & 255], 1);
+        for (int i = tid; i < n; i += kPickThreads) {
+            const uint64_t x = score(i);
+            if (x >> shift == limit) atomicAdd(&count[(x >> next) & 255 >> (8 - width)], 1);
         }
         __syncthreads();
         // of the values from the highest down: the first at which `rest` are reached
-        const int mine = count[255 - tid];
+        const int mine = tid < 256 ? count[255 - tid] : 0;
         int upto = mine;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -244,16 +309,19 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectArgs 
         if (upto >= rest && upto - mine < rest) {
             found[0] = 255 - tid;
             found[1] = rest - (upto - mine);
+            found[2] = mine;
         }
         __syncthreads();
-        limit |= (uint32_t)found[0] << shift;
+        limit = limit << width | (uint32_t)found[0];
         rest = found[1];
+        shift = next;
+        if (found[2] == rest) break;  // all of them
     }
     // all above the limit, and the first `rest` equal to it
-    const int per = (n + kSelectThreads - 1) / kSelectThreads, begin = min(n, tid * per), end = min(n, begin + per);
+    const int per = (n + kPickThreads - 1) / kPickThreads, begin = min(n, tid * per), end = min(n, begin + per);
     int above = 0, equal = 0;
     for (int i = begin; i < end; ++i) {
-        const uint32_t x = score(i);
+        const uint64_t x = (uint64_t)score(i) >> shift;
         above += x > limit;
         equal += x == limit;
     }
@@ -279,22 +347,33 @@ __global__ __launch_bounds__(kSelectThreads) void page_select_kernel(SelectArgs 
     int ties = equal_upto - equal;
     int at = a.first_pages + above_upto - above + min(ties, rest);
     for (int i = begin; i < end; ++i) {
-        const uint32_t x = score(i);
+        const uint64_t x = (uint64_t)score(i) >> shift;
         if (x > limit || (x == limit && ties++ < rest)) out[at++] = a.first_pages + i;
     }
 }
 
+// Pages of a workgroup: enough workgroups to fill the GPU a few times.
+int score_pages(const SelectArgs& a) {
+    const int64_t rows = (int64_t)a.B * a.Hkv * a.T, want = 16 * (int64_t)kComputeUnits;
+    int per = 64;
+    while (per < 1024 && rows * ((a.max_pages + 2 * per - 1) / (2 * per)) >= want) per *= 2;
+    return per;
+}
+int score_chunks(const SelectArgs& a) { return (a.max_pages + score_pages(a) - 1) / score_pages(a); }
+
 template <typename T>
-hipError_t launch_score(const SelectArgs& a, int chunks, hipStream_t s) {
-    hipLaunchKernelGGL((page_score_kernel<T>), dim3((unsigned)((int64_t)a.B * a.Hkv * a.T * chunks)), dim3(kSelectThreads), 0,
-                       s, a, chunks);
+hipError_t launch_score(const SelectArgs& a, hipStream_t s) {
+    const int words = a.D / Words<T>::W, heads = std::min(a.G, kScoreQuery / a.D), chunks = score_chunks(a);
+    int lanes = 1;
+    while (lanes * kScoreWords < words) lanes *= 2;
+    hipLaunchKernelGGL((page_score_kernel<T>), dim3((unsigned)((int64_t)a.B * a.Hkv * a.T * chunks)), dim3(kSelectThreads),
+                       heads * (a.D * (int)sizeof(double) + 16 * words), s, a, score_pages(a), lanes, heads);
     return hipGetLastError();
 }
 
 int64_t bounds_grid(const PageBoundsArgs& a) {
     return ((int64_t)a.B * a.touched * a.Hkv + kSelectWaves - 1) / kSelectWaves;
 }
-int score_chunks(const SelectArgs& a) { return (a.max_pages + kScorePages - 1) / kScorePages; }
 
 }  // namespace
 
@@ -319,14 +398,14 @@ hipError_t launch_page_select(const SelectArgs& a, int dtype, hipStream_t s) {
     if (a.max_pages > a.pages) {
         hipError_t e;
         switch (dtype) {
-            case DT_F32: e = launch_score<float>(a, score_chunks(a), s); break;
-            case DT_BF16: e = launch_score<__bf16>(a, score_chunks(a), s); break;
-            case DT_F16: e = launch_score<_Float16>(a, score_chunks(a), s); break;
+            case DT_F32: e = launch_score<float>(a, s); break;
+            case DT_BF16: e = launch_score<__bf16>(a, s); break;
+            case DT_F16: e = launch_score<_Float16>(a, s); break;
             default: return hipErrorInvalidValue;
         }
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(page_select_kernel, dim3((unsigned)((int64_t)a.B * a.Hkv * a.T)), dim3(kSelectThreads), 0, s, a);
+    hipLaunchKernelGGL(page_select_kernel, dim3((unsigned)((int64_t)a.B * a.Hkv * a.T)), dim3(kPickThreads), 0, s, a);
     return hipGetLastError();
 }
 

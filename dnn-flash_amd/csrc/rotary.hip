@@ -8,10 +8,10 @@
 // itself, 2^-31 turns at p = 2^21, where 32 bits would be off by a sixteenth of
 // a turn. Sine and cosine are then fp32, like the products; the result is rounded once.
 //
-// Both kernels are bound by reading and writing each row once. A workgroup
-// takes one token or four, so the sines and cosines of a token, one per pair, are
-// computed once for all heads and shared through LDS; the first rows are on
-// their way meanwhile.
+// Both kernels are bound by reading and writing each row once. A wavefront (or,
+// with few tokens, each of four) takes a token: its place and position are scalars,
+// its sines and cosines are computed once for all heads and kept in LDS, and the
+// first rows are on their way meanwhile. A lane keeps its columns for all rows.
 
 #include "serving_kernels.h"
 
@@ -19,7 +19,8 @@ namespace ofh {
 namespace {
 
 constexpr int kRotaryThreads = 256;
-constexpr int kInFlight = 4;  // items of a thread whose loads are issued together
+constexpr int kRotaryWaves = kRotaryThreads / 64;
+constexpr int kInFlight = 4;  // rows of a lane whose loads are issued together
 constexpr double kTurn = 0.15915494309189533577;  // 1 / (2 pi)
 
 template <int BYTES>
@@ -51,10 +52,11 @@ struct Row {
     struct Item {
         C a, b;
     };
-    // columns of the item's two words
-    static __device__ __forceinline__ void columns(const Rotation& r, int item, int& ca, int& cb) {
+    int ca, cb, pair;  // columns of the item's two words, its first pair; copied: pair -1
+    __device__ __forceinline__ Row(const Rotation& r, int item) {
         const int turned = r.R / 2 / PAIRS;
-        if (item >= turned) {
+        pair = item < turned ? item * PAIRS : -1;
+        if (pair < 0) {
             ca = cb = r.R + (item - turned) * W;
         } else if (INTERLEAVED) {
             ca = item * 2 * PAIRS;
@@ -64,25 +66,19 @@ struct Row {
             cb = ca + r.R / 2;
         }
     }
-    static __device__ __forceinline__ Item load(const Rotation& r, const T* row, int item) {
-        int ca, cb;
-        columns(r, item, ca, cb);
+    __device__ __forceinline__ Item load(const T* row) const {
         Item x;
         x.a = *(const C*)(row + ca);
         x.b = ONE ? x.a : *(const C*)(row + cb);
         return x;
     }
-    static __device__ __forceinline__ void clear(const Rotation& r, T* row, int item) {
-        int ca, cb;
-        columns(r, item, ca, cb);
+    __device__ __forceinline__ void clear(T* row) const {
         *(C*)(row + ca) = C{};
         if (!ONE) *(C*)(row + cb) = C{};
     }
     // cs: cosines and sines of the row's token
-    static __device__ __forceinline__ void store(const Rotation& r, T* row, int item, const Item& x, const float2* cs) {
-        int ca, cb;
-        columns(r, item, ca, cb);
-        if (item >= r.R / 2 / PAIRS) {
+    __device__ __forceinline__ void store(T* row, const Item& x, const float2* cs) const {
+        if (pair < 0) {
             *(C*)(row + ca) = x.a;
             return;
         }
@@ -92,7 +88,7 @@ struct Row {
         } a, b;
         a.c = x.a;
         b.c = x.b;
-        cs += item * PAIRS;
+        cs += pair;
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) {
             const float2 t = cs[i];
@@ -120,131 +116,137 @@ inline __host__ __device__ int row_items(const Rotation& r, int D, int W) {
     return r.R / 2 / pairs + (D - r.R) / W;
 }
 
-template <typename T, int W, bool INTERLEAVED, int TOKENS>
-__global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
-    using X = Row<T, W, INTERLEAVED>;
-    __shared__ float2 cs[TOKENS * (kRotaryMaxDim / 2)];
-    const int64_t first = (int64_t)blockIdx.x * TOKENS;
-    const int tokens = (int)min((int64_t)TOKENS, (int64_t)a.B * a.T - first);
-    const unsigned per_row = row_items(a.r, a.D, W), per_token = per_row * (unsigned)a.H, items = per_token * tokens;
-    for (unsigned at = threadIdx.x; at - threadIdx.x < items; at += kRotaryThreads * kInFlight) {
-        typename X::Item x[kInFlight];
-        int64_t to[kInFlight];
-        unsigned tok[kInFlight], item[kInFlight];
+// The wavefront's token and its share of the token's rows. PER_TOKEN wavefronts
+// share a token; `beside` rows of `lanes` lanes stand beside each other in one.
+template <int PER_TOKEN>
+struct Share {
+    int lanes, beside, lane, slot;
+    int64_t token;
+    __device__ __forceinline__ Share(int items) {
+        lanes = 1;
+        while (lanes < items && lanes < 64) lanes *= 2;
+        beside = 64 / lanes;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
+        token = (int64_t)blockIdx.x * (kRotaryWaves / PER_TOKEN) + wave / PER_TOKEN;
+        lane = l & (lanes - 1);
+        slot = (wave % PER_TOKEN) * beside + l / lanes;
+    }
+    __device__ __forceinline__ int stride() const { return PER_TOKEN * beside; }
+};
+
+// Cosines and sines of a position, by the wavefront for itself.
+__device__ __forceinline__ void turns(const Rotation& r, int64_t position, float2* cs) {
+    for (int n = threadIdx.x & 63; n < r.R / 2; n += 64) cs[n] = turn(r, n, position);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Turns rows 0 .. rows - 1 of a token: from(row) is a row, to(row) where it goes (null:
+// nowhere), padding(row) whether it is cleared instead. `before` runs once, when the
+// first rows are on their way, and leaves cs.
+template <typename X, typename S, typename From, typename To, typename Padding, typename Before>
+__device__ __forceinline__ void turn_rows(const Rotation& r, const S& share, int items, int rows, const float2* cs, From from,
+                                          To to, Padding padding, Before before) {
+    bool first = true;
+    for (int base = 0; base < items; base += share.lanes) {
+        const int item = base + share.lane;
+        const X x(r, min(item, items - 1));
+        for (int row0 = share.slot; row0 - share.slot < rows; row0 += kInFlight * share.stride()) {
+            typename X::Item v[kInFlight];
 #pragma unroll
-        for (int i = 0; i < kInFlight; ++i) {
-            const unsigned n = at + i * kRotaryThreads;
-            if (n >= items) continue;
-            tok[i] = n / per_token;
-            const unsigned rest = n - tok[i] * per_token, h = rest / per_row;
-            item[i] = rest - h * per_row;
-            const unsigned bt = (unsigned)first + tok[i], b = bt / (unsigned)a.T, t = bt - b * (unsigned)a.T;
-            to[i] = b * a.o_sb + h * a.o_sh + t * a.o_st;
-            x[i] = X::load(a.r, (const T*)a.x + b * a.x_sb + h * a.x_sh + t * a.x_st, (int)item[i]);
-        }
-        if (at == threadIdx.x) {
-            const int pairs = a.r.R / 2;
-            for (int n = threadIdx.x; n < tokens * pairs; n += kRotaryThreads) {
-                const int j = n / pairs, pair = n - j * pairs;
-                const unsigned bt = (unsigned)first + j, b = bt / (unsigned)a.T, t = bt - b * (unsigned)a.T;
-                const int64_t position = a.positions != nullptr ? (int64_t)a.positions[b * a.pos_sb + t]
-                                         : a.lengths != nullptr ? (int64_t)a.lengths[b] - a.T + t
-                                                                : a.offset + t;
-                cs[n] = turn(a.r, pair, position);
+            for (int i = 0; i < kInFlight; ++i) {
+                const int row = min(row0 + i * share.stride(), rows - 1);
+                if (!padding(row)) v[i] = x.load(from(row));
             }
-            __syncthreads();
-        }
+            if (first) before();
+            first = false;
 #pragma unroll
-        for (int i = 0; i < kInFlight; ++i)
-            if (at + i * kRotaryThreads < items)
-                X::store(a.r, (T*)a.o + to[i], (int)item[i], x[i], cs + tok[i] * (a.r.R / 2));
+            for (int i = 0; i < kInFlight; ++i) {
+                const int row = row0 + i * share.stride();
+                if (row >= rows || item >= items) continue;
+                auto* out = to(row);
+                if (out == nullptr) continue;
+                if (padding(row)) x.clear(out);
+                else x.store(out, v[i], cs);
+            }
+        }
     }
 }
 
-// Where the rows of a new token go.
-struct Place {
-    bool padding;      // not a token of its sequence
-    int64_t position;
-    int64_t k, v;      // elements from the pools' start; -1: no place
-};
-__device__ __forceinline__ Place place(const CacheWriteArgs& w, unsigned b, unsigned t) {
-    Place p;
-    const int count = w.counts != nullptr ? max(0, min(w.counts[b], w.T)) : w.T;
-    p.padding = (int)t >= count;
-    p.position = (int64_t)w.lengths[b] - count + t;
-    p.k = p.v = -1;
-    const int64_t slot = p.position >> w.page_shift;
-    if (p.padding || p.position < 0 || slot >= w.max_pages) return p;
-    const int page = w.table[b * w.table_stride + slot];
-    if ((unsigned)page >= (unsigned)w.num_pages) return p;
-    const int64_t row = p.position & (((int64_t)1 << w.page_shift) - 1);
-    p.k = page * w.kp_sp + row * w.kp_st;
-    p.v = page * w.vp_sp + row * w.vp_st;
-    return p;
+template <typename T, int W, bool INTERLEAVED, int PER_TOKEN>
+__global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
+    __shared__ float2 table[kRotaryWaves][kRotaryMaxDim / 2];
+    const int items = row_items(a.r, a.D, W);
+    const Share<PER_TOKEN> share(items);
+    if (share.token >= (int64_t)a.B * a.T) return;
+    const int b = (int)((unsigned)share.token / (unsigned)a.T), t = (int)share.token - b * a.T;
+    float2* cs = table[threadIdx.x >> 6];
+    const T* x = (const T*)a.x + b * a.x_sb + t * a.x_st;
+    T* o = (T*)a.o + b * a.o_sb + t * a.o_st;
+    turn_rows<Row<T, W, INTERLEAVED>>(
+        a.r, share, items, a.H, cs, [&](int h) { return x + h * a.x_sh; }, [&](int h) { return o + h * a.o_sh; },
+        [](int) { return false; },
+        [&] {
+            turns(a.r, a.positions != nullptr ? (int64_t)a.positions[b * a.pos_sb + t]
+                       : a.lengths != nullptr ? (int64_t)a.lengths[b] - a.T + t
+                                              : a.offset + t, cs);
+        });
 }
 
-// Items of a token: those of its K rows, then its Q rows, then the words of its V rows.
-template <typename T, int W, bool INTERLEAVED, int TOKENS>
+template <typename T, int W, bool INTERLEAVED, int PER_TOKEN>
 __global__ __launch_bounds__(kRotaryThreads) void cache_append_kernel(CacheAppendArgs a) {
     using X = Row<T, W, INTERLEAVED>;
-    __shared__ float2 cs[TOKENS * (kRotaryMaxDim / 2)];
-    __shared__ Place places[TOKENS];
+    using C = typename X::C;
+    __shared__ float2 table[kRotaryWaves][kRotaryMaxDim / 2];
     const CacheWriteArgs& w = a.w;
-    const int64_t first = (int64_t)blockIdx.x * TOKENS;
-    const int tokens = (int)min((int64_t)TOKENS, (int64_t)w.B * w.T - first);
-    const unsigned per_row = row_items(a.r, a.D, W), v_row = (unsigned)a.Dv / W;
-    const unsigned kq = per_row * (unsigned)(w.Hkv + a.H), per_token = kq + v_row * (unsigned)w.Hkv;
-    const unsigned items = per_token * tokens;
-    for (unsigned at = threadIdx.x; at - threadIdx.x < items; at += kRotaryThreads * kInFlight) {
-        typename X::Item x[kInFlight];
-        unsigned tok[kInFlight], row[kInFlight], item[kInFlight];  // rows: K, then Q, then V
+    const int items = row_items(a.r, a.D, W), words = a.Dv / W;
+    const Share<PER_TOKEN> share(items), v_share(words);
+    if (share.token >= (int64_t)w.B * w.T) return;
+    const int b = (int)((unsigned)share.token / (unsigned)w.T), t = (int)share.token - b * w.T;
+    const int count = w.counts != nullptr ? max(0, min(w.counts[b], w.T)) : w.T;
+    const bool padding = t >= count;
+    float2* cs = table[threadIdx.x >> 6];
+
+    const int64_t position = (int64_t)w.lengths[b] - count + t, place = position >> w.page_shift;
+    int page = -1;
+    if (!padding && position >= 0 && place < w.max_pages) page = w.table[b * w.table_stride + place];
+    const bool placed = (unsigned)page < (unsigned)w.num_pages;
+    const int64_t in_page = position & (((int64_t)1 << w.page_shift) - 1);
+    T* k_to = (T*)w.k_pages + page * w.kp_sp + in_page * w.kp_st;
+    T* v_to = (T*)w.v_pages + page * w.vp_sp + in_page * w.vp_st;
+
+    const T* k = (const T*)w.k + b * w.k_sb + t * w.k_st;
+    const T* q = (const T*)a.q + b * a.q_sb + t * a.q_st;
+    T* q_to = (T*)a.q_out + b * a.o_sb + t * a.o_st;
+    // V rows are copied, K rows and Q rows turned
+    const T* v = (const T*)w.v + b * w.v_sb + t * w.v_st;
+    if (placed)
+        for (int base = 0; base < words; base += v_share.lanes) {
+            const int word = base + v_share.lane;
+            for (int h0 = v_share.slot; h0 - v_share.slot < w.Hkv; h0 += kInFlight * v_share.stride()) {
+                C x[kInFlight];
 #pragma unroll
-        for (int i = 0; i < kInFlight; ++i) {
-            const unsigned n = at + i * kRotaryThreads;
-            if (n >= items) continue;
-            tok[i] = n / per_token;
-            const unsigned rest = n - tok[i] * per_token;
-            const bool is_v = rest >= kq;
-            const unsigned r = is_v ? (rest - kq) / v_row : rest / per_row;
-            item[i] = is_v ? rest - kq - r * v_row : rest - r * per_row;
-            row[i] = is_v ? r + w.Hkv + a.H : r;
-            const unsigned bt = (unsigned)first + tok[i], b = bt / (unsigned)w.T, t = bt - b * (unsigned)w.T;
-            if (w.counts != nullptr && (int)t >= w.counts[b]) continue;  // padding is not read
-            if (is_v)
-                x[i].a = *(const typename X::C*)((const T*)w.v + b * w.v_sb + r * w.v_sh + t * w.v_st + item[i] * W);
-            else if (r < (unsigned)w.Hkv)
-                x[i] = X::load(a.r, (const T*)w.k + b * w.k_sb + r * w.k_sh + t * w.k_st, (int)item[i]);
-            else
-                x[i] = X::load(a.r, (const T*)a.q + b * a.q_sb + (r - w.Hkv) * a.q_sh + t * a.q_st, (int)item[i]);
-        }
-        if (at == threadIdx.x) {
-            const int pairs = a.r.R / 2;
-            for (int n = threadIdx.x; n < tokens * pairs; n += kRotaryThreads) {
-                const int j = n / pairs, pair = n - j * pairs;
-                const unsigned bt = (unsigned)first + j, b = bt / (unsigned)w.T, t = bt - b * (unsigned)w.T;
-                const Place p = place(w, b, t);
-                if (pair == 0) places[j] = p;
-                cs[n] = turn(a.r, pair, p.position);
-            }
-            __syncthreads();
-        }
+                for (int i = 0; i < kInFlight; ++i)
+                    x[i] = *(const C*)(v + min(h0 + i * v_share.stride(), w.Hkv - 1) * w.v_sh + min(word, words - 1) * W);
 #pragma unroll
-        for (int i = 0; i < kInFlight; ++i) {
-            if (at + i * kRotaryThreads >= items) continue;
-            const Place& p = places[tok[i]];
-            const float2* c = cs + tok[i] * (a.r.R / 2);
-            const unsigned bt = (unsigned)first + tok[i], b = bt / (unsigned)w.T, t = bt - b * (unsigned)w.T;
-            if (row[i] < (unsigned)w.Hkv) {
-                if (p.k >= 0) X::store(a.r, (T*)w.k_pages + p.k + row[i] * w.kp_sh, (int)item[i], x[i], c);
-            } else if (row[i] < (unsigned)(w.Hkv + a.H)) {
-                T* to = (T*)a.q_out + b * a.o_sb + (row[i] - w.Hkv) * a.o_sh + t * a.o_st;
-                if (p.padding) X::clear(a.r, to, (int)item[i]);
-                else X::store(a.r, to, (int)item[i], x[i], c);
-            } else if (p.v >= 0) {
-                *(typename X::C*)((T*)w.v_pages + p.v + (row[i] - w.Hkv - a.H) * w.vp_sh + item[i] * W) = x[i].a;
+                for (int i = 0; i < kInFlight; ++i) {
+                    const int h = h0 + i * v_share.stride();
+                    if (h < w.Hkv && word < words) *(C*)(v_to + h * w.vp_sh + word * W) = x[i];
+                }
             }
         }
-    }
+    turn_rows<X>(
+        a.r, share, items, w.Hkv + a.H, cs,
+        [&](int row) { return row < w.Hkv ? k + row * w.k_sh : q + (row - w.Hkv) * a.q_sh; },
+        [&](int row) -> T* {
+            if (row >= w.Hkv) return q_to + (row - w.Hkv) * a.o_sh;
+            return placed ? k_to + row * w.kp_sh : nullptr;
+        },
+        [&](int) { return padding; },
+        [&] {
+            if (!padding) turns(a.r, position, cs);
+        });
 }
 
 bool turns_in_words(const Rotation& r, int D, int elem) {
@@ -270,23 +272,20 @@ bool append_in_words(const CacheAppendArgs& a, int elem) {
     return turns_in_words(a.r, a.D, elem) && a.Dv % (16 / elem) == 0 && aligned(all, strides, elem);
 }
 
-int elem_of(int dtype) { return dtype == DT_F32 ? 4 : 2; }
+// A wavefront per token once that fills the GPU, a workgroup before.
+bool many_tokens(int64_t tokens) { return tokens >= 16 * (int64_t)kComputeUnits; }
+int64_t rotary_grid(int64_t tokens) { return many_tokens(tokens) ? (tokens + kRotaryWaves - 1) / kRotaryWaves : tokens; }
 
-// Four tokens per workgroup once that leaves enough workgroups to fill the GPU.
-bool four_tokens(int64_t tokens) { return tokens >= 16 * (int64_t)kComputeUnits; }
-
-// Items of a workgroup and tokens are 32-bit in the kernels.
-bool fits(int64_t tokens, int64_t per_token) {
-    return tokens < ((int64_t)1 << 31) && per_token < ((int64_t)1 << 28) &&
-           grid_fits(four_tokens(tokens) ? (tokens + 3) / 4 : tokens, kRotaryThreads);
+// Tokens and rows of a token are 32-bit in the kernels.
+bool fits(int64_t tokens, int64_t rows) {
+    return tokens < ((int64_t)1 << 31) && rows < ((int64_t)1 << 30) && grid_fits(rotary_grid(tokens), kRotaryThreads);
 }
 
-#define OFH_ROTARY_LAUNCH(KERNEL, T, W, INTER)                                                                      \
-    do {                                                                                                            \
-        if (four_tokens(tokens))                                                                                    \
-            hipLaunchKernelGGL((KERNEL<T, W, INTER, 4>), dim3((unsigned)((tokens + 3) / 4)), dim3(kRotaryThreads), 0, s, a); \
-        else                                                                                                        \
-            hipLaunchKernelGGL((KERNEL<T, W, INTER, 1>), dim3((unsigned)tokens), dim3(kRotaryThreads), 0, s, a);     \
+#define OFH_ROTARY_LAUNCH(KERNEL, T, W, INTER)                                                          \
+    do {                                                                                                \
+        const dim3 grid((unsigned)rotary_grid(tokens)), block(kRotaryThreads);                          \
+        if (many_tokens(tokens)) hipLaunchKernelGGL((KERNEL<T, W, INTER, 1>), grid, block, 0, s, a);    \
+        else hipLaunchKernelGGL((KERNEL<T, W, INTER, kRotaryWaves>), grid, block, 0, s, a);             \
     } while (0)
 
 template <typename T>
@@ -314,15 +313,8 @@ hipError_t launch_append_type(const CacheAppendArgs& a, hipStream_t s) {
 
 }  // namespace
 
-bool rotary_fits(const RotaryArgs& a, int dtype) {
-    const int elem = elem_of(dtype), w = rotary_in_words(a, elem) ? 16 / elem : 1;
-    return fits((int64_t)a.B * a.T, (int64_t)a.H * row_items(a.r, a.D, w));
-}
-bool cache_append_fits(const CacheAppendArgs& a, int dtype) {
-    const int elem = elem_of(dtype), w = append_in_words(a, elem) ? 16 / elem : 1;
-    return fits((int64_t)a.w.B * a.w.T,
-                ((int64_t)a.w.Hkv + a.H) * row_items(a.r, a.D, w) + (int64_t)a.w.Hkv * (a.Dv / w));
-}
+bool rotary_fits(const RotaryArgs& a) { return fits((int64_t)a.B * a.T, a.H); }
+bool cache_append_fits(const CacheAppendArgs& a) { return fits((int64_t)a.w.B * a.w.T, (int64_t)a.w.Hkv + a.H); }
 
 hipError_t launch_rotary(const RotaryArgs& a, int dtype, hipStream_t s) {
     switch (dtype) {

@@ -408,6 +408,7 @@ size_t select_bytes(const ofh::SelectArgs& a) {
 // A batch in groups that share pages.
 struct PrefixPlan {
     Split tail;
+    ofh::PrefixKernel kernel;
     int tiles, splits, min_steps;
     size_t tail_o, tail_ml, prefix_o, prefix_ml;  // bytes
     size_t bytes() const { return tail_o + tail_ml + prefix_o + prefix_ml; }
@@ -439,9 +440,10 @@ PrefixPlan plan_prefix(const ofh::StreamArgs& a, int dtype, const ofh_prefix_gro
     ofh::StreamArgs own = a;
     own.capacity = std::max(a.capacity - (int)g->least_shared, 1);
     plan.tail = plan_split(own, dtype, max_key_splits);
-    const int dk = ofh::stream_kernel_dim(a.D, a.Dv);
-    const int rows = ofh::prefix_tile_rows(a, dtype), step = ofh::stream_step_keys(dtype, dk);
-    plan.min_steps = ofh::kStreamThreads / 64;
+    plan.kernel = ofh::prefix_kernel(a, dtype);
+    const int rows = plan.kernel.rows, step = plan.kernel.step_keys;
+    // (a wavefront of the streaming kernel takes a step, a workgroup of the other)
+    plan.min_steps = plan.kernel.key_splits == 0 ? ofh::kStreamThreads / 64 : 2;
     plan.tiles = (int)(((int64_t)a.B * a.T * a.G + (int64_t)a.groups * (rows - 1)) / rows);
     const int64_t units = (int64_t)a.Hkv * plan.tiles, steps = ((int64_t)g->most_shared + step - 1) / step;
     const int64_t n = std::min<int64_t>({(2 * ofh::kComputeUnits + units - 1) / units, steps / plan.min_steps,
@@ -459,7 +461,7 @@ PrefixPlan plan_prefix(const ofh::StreamArgs& a, int dtype, const ofh_prefix_gro
 int run_prefix(ofh::StreamArgs& a, int dtype, const PrefixPlan& plan, void* workspace, size_t workspace_bytes,
                hipStream_t stream) {
     if (!ofh::grid_fits(plan.tail.units * plan.tail.splits, ofh::kStreamThreads) ||
-        !ofh::grid_fits((int64_t)a.Hkv * plan.tiles * plan.splits, ofh::kStreamThreads) ||
+        !ofh::grid_fits(((int64_t)a.Hkv * plan.splits + 8) * plan.tiles, ofh::kStreamThreads) ||
         !ofh::grid_fits((int64_t)a.B * a.Hkv * a.T * a.G * ((a.Dv + 31) / 32), 64))
         return unsupported("attention call exceeds the launch range");
     ofh::ScratchLease lease;
@@ -475,7 +477,8 @@ int run_prefix(ofh::StreamArgs& a, int dtype, const PrefixPlan& plan, void* work
     a.part_ml = reinterpret_cast<float*>(at += plan.tail_o);
     a.prefix_o = reinterpret_cast<float*>(at += plan.tail_ml);
     a.prefix_ml = reinterpret_cast<float*>(at += plan.prefix_o);
-    OFH_HIP_CHECK(ofh::launch_stream_prefix(a, dtype, stream));
+    if (plan.kernel.key_splits > 0) OFH_HIP_CHECK(ofh::launch_prefix(a, dtype, plan.kernel.key_splits, stream));
+    else OFH_HIP_CHECK(ofh::launch_stream_prefix(a, dtype, stream));
     OFH_HIP_CHECK(ofh::launch_stream_tail(a, dtype, stream));
     return lease.release();
 }

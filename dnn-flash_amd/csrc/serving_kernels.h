@@ -90,8 +90,16 @@ hipError_t launch_stream(const StreamArgs& a, int dtype, hipStream_t s);
 // Attention over groups of sequences that share pages, and over selected pages.
 // The prefix writes its partial rows (prefix_*); the tail's launch reads the rest
 // and joins both.
-int prefix_tile_rows(const StreamArgs& a, int dtype);
+// A prefix tile's rows, its keys' steps (of how many keys), and its workgroups.
+struct PrefixKernel {
+    int rows, step_keys, key_splits;  // key_splits: of prefix_fwd.hip's kernel, 0: the streaming kernel
+};
+PrefixKernel prefix_kernel(const StreamArgs& a, int dtype);
+inline int64_t prefix_grid(const StreamArgs& a) {
+    return ((int64_t)a.Hkv * a.prefix_splits + 7) / 8 * 8 * a.prefix_tiles;
+}
 hipError_t launch_stream_prefix(const StreamArgs& a, int dtype, hipStream_t s);
+hipError_t launch_prefix(const StreamArgs& a, int dtype, int key_splits, hipStream_t s);
 hipError_t launch_stream_tail(const StreamArgs& a, int dtype, hipStream_t s);
 hipError_t launch_stream_selected(const StreamArgs& a, int dtype, hipStream_t s);
 
@@ -190,7 +198,7 @@ struct RotaryArgs {
     const int32_t* lengths;
     int64_t offset;
 };
-bool rotary_fits(const RotaryArgs& a, int dtype);  // in one launch
+bool rotary_fits(const RotaryArgs& a);  // in one launch
 hipError_t launch_rotary(const RotaryArgs& a, int dtype, hipStream_t s);
 
 // New rows into pages with K turned on the way, and Q turned into q_out (H 0: no Q).
@@ -203,7 +211,7 @@ struct CacheAppendArgs {
     int H, D, Dv;
     Rotation r;
 };
-bool cache_append_fits(const CacheAppendArgs& a, int dtype);
+bool cache_append_fits(const CacheAppendArgs& a);
 hipError_t launch_cache_append(const CacheAppendArgs& a, int dtype, hipStream_t s);
 
 // Whole pages src -> dst in several pools of one geometry. The words of a

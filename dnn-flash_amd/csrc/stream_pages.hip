@@ -14,7 +14,7 @@ namespace {
 
 template <typename T, int DK, int RT>
 hipError_t launch_prefix_rt(const StreamArgs& a, hipStream_t s) {
-    const dim3 grid((unsigned)((int64_t)a.Hkv * a.prefix_tiles * a.prefix_splits)), block(kStreamThreads);
+    const dim3 grid((unsigned)prefix_grid(a)), block(kStreamThreads);
     hipLaunchKernelGGL((stream_fwd_kernel<T, DK, RT, kPrefix, kPart>), grid, block, 0, s, a);
     return hipGetLastError();
 }
@@ -79,13 +79,18 @@ hipError_t launch(const StreamArgs& a, int dtype, int rows, hipStream_t s) {
 
 }  // namespace
 
-// (groups of different sizes have one kernel: that of their average)
-static int group_rows(const StreamArgs& a) { return a.B / a.groups * a.T * a.G; }
-int prefix_tile_rows(const StreamArgs& a, int dtype) {
-    return stream_tile_rows(dtype, stream_kernel_dim(a.D, a.Dv), group_rows(a));
+// Groups of different sizes have one kernel: that of their average rows.
+PrefixKernel prefix_kernel(const StreamArgs& a, int dtype) {
+    const int dk = stream_kernel_dim(a.D, a.Dv), rows = a.B / a.groups * a.T * a.G;
+    // (a lane of prefix_fwd.hip adds the bytes of up to 16 rows in 32 bits, as here)
+    if (dtype != DT_F32 && rows > 32) {
+        const int key_splits = dk <= 128 && rows <= window_rows(2) ? 2 : 1;
+        return PrefixKernel{window_rows(key_splits), 64, key_splits};
+    }
+    return PrefixKernel{stream_tile_rows(dtype, dk, rows), stream_step_keys(dtype, dk), 0};
 }
 hipError_t launch_stream_prefix(const StreamArgs& a, int dtype, hipStream_t s) {
-    return launch<kLaunchPrefix>(a, dtype, group_rows(a), s);
+    return launch<kLaunchPrefix>(a, dtype, a.B / a.groups * a.T * a.G, s);
 }
 hipError_t launch_stream_tail(const StreamArgs& a, int dtype, hipStream_t s) {
     return launch<kLaunchTail>(a, dtype, a.T * a.G, s);

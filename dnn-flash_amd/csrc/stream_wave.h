@@ -257,25 +257,16 @@ __device__ __forceinline__ StreamPart stream_part(const StreamArgs& a, int id, i
 }
 
 // Prefix tiles: the tiles of all groups (rt) of a key-value head, and their parts.
-// A key-value head's run on one XCD where the heads can be dealt out evenly: its
-// tiles read the same keys.
-__device__ __forceinline__ StreamPart prefix_part(const StreamArgs& a, int id) {
-    const int per = a.prefix_tiles * a.prefix_splits;
-    StreamPart p;
-    int rest;
+// The tiles that read the same keys, those of a part of a head, run on one XCD, side
+// by side: what one reads the others find in its cache. Parts and heads are dealt
+// out to the eight XCDs in turn (the grid is filled up to eights: false past the last).
+__device__ __forceinline__ bool prefix_part(const StreamArgs& a, int id, StreamPart& p) {
+    const int j = id >> 3, round = j / a.prefix_tiles, unit = 8 * round + (id & 7);
     p.b = 0;
-    if ((a.Hkv & 7) == 0) {
-        const int j = id >> 3;
-        p.hk = j / per * 8 + (id & 7);
-        rest = j % per;
-    } else {
-        p.hk = id / per;
-        rest = id % per;
-    }
-    // (the tiles of a part side by side: what one reads the others find in the cache)
-    p.part = rest / a.prefix_tiles;
-    p.rt = rest - p.part * a.prefix_tiles;
-    return p;
+    p.rt = j - round * a.prefix_tiles;
+    p.part = unit / a.Hkv;
+    p.hk = unit - p.part * a.Hkv;
+    return p.part < a.prefix_splits;
 }
 
 // Parts of a tile of `steps` steps (at most `splits`, of min_steps each), and the steps of each.
@@ -840,8 +831,7 @@ void stream_fwd_kernel(StreamArgs a) {
     StreamPart at;
     PrefixTile pt{};
     if constexpr (SRC == kPrefix) {
-        at = prefix_part(a, blockIdx.x);
-        if (!prefix_tile(a, at.rt, W::ROWS, pt)) return;
+        if (!prefix_part(a, blockIdx.x, at) || !prefix_tile(a, at.rt, W::ROWS, pt)) return;
     } else {
         at = stream_part(a, blockIdx.x, MODE == kOwn ? (a.row_tiles + kWaves - 1) / kWaves : a.row_tiles);
     }
