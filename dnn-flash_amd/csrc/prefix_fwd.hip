@@ -4,8 +4,14 @@
 // sequence, so that a tile goes on from one to the next, and leave partial rows (max,
 // sum, unnormalised O) that the join folds with each sequence's own keys.
 //
-// A page's 16 rows are 16 KB or less of consecutive copies with one scalar base, so
-// pages cost a table entry per 16 keys (loaded a tile ahead) and nothing per lane.
+// A copy of a wavefront stays within 16 keys, which are one page's: its base is a
+// scalar, read from the lane that holds the place of these keys.
+//
+// One workgroup of a CU is a prefix's while another reads a sequence's own keys, so
+// a workgroup by itself has to keep enough loads in flight: K and V of a step are
+// halves of their own in a ring of 80 KB, each waited for by count, and a barrier
+// before a half is used frees the one used before it. (With two stages of K and V
+// together, 64 KB, a step waited for its memory.)
 
 #include "stream_wave.h"
 #include "window_wave.h"
@@ -13,9 +19,46 @@
 namespace ofh {
 namespace {
 
+// dma16s of COUNT copies that are `step` bytes of LDS apart, M0 saved once.
+template <int COUNT>
+__device__ __forceinline__ void dma16s_row(const char* const (&base)[COUNT], unsigned off, unsigned lds, unsigned step);
+template <>
+__device__ __forceinline__ void dma16s_row<2>(const char* const (&base)[2], unsigned off, unsigned lds, unsigned step) {
+    unsigned save;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
+        "s_add_u32 m0, m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
+        : "=&s"(save) : "v"(off), "s"(base[0]), "s"(base[1]), "s"(lds), "s"(step) : "memory", "scc");
+}
+template <>
+__device__ __forceinline__ void dma16s_row<4>(const char* const (&base)[4], unsigned off, unsigned lds, unsigned step) {
+    unsigned save;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
+        "s_add_u32 m0, m0, %7\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
+        "s_add_u32 m0, m0, %7\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %4\n\t"
+        "s_add_u32 m0, m0, %7\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %5\n\ts_mov_b32 m0, %0"
+        : "=&s"(save)
+        : "v"(off), "s"(base[0]), "s"(base[1]), "s"(base[2]), "s"(base[3]), "s"(lds), "s"(step)
+        : "memory", "scc");
+}
+
+// Steps of SN keys, which KS groups of wavefronts share in BN, and a ring of HALVES.
+template <int D, int KS>
+struct PrefixTiles {
+    static constexpr int THREADS = 256, WAVES = THREADS / 64;
+    static constexpr int R = WAVES / KS;
+    static constexpr int BN = D == 256 || KS == 2 ? 32 : 64;
+    static constexpr int SN = D == 256 ? 32 : 64;
+    static constexpr int SB = SN / BN;
+    static constexpr int WAVES_PER_SIMD = D <= 128 ? 2 : 1;
+    static constexpr int HALVES = D == 128 ? 5 : 9;
+    static_assert(SB % KS == 0, "the groups share a step");
+};
+
 template <typename T, int D, int KS>
-struct PrefixWave : WindowWave<T, D, KS> {
-    using Base = WindowWave<T, D, KS>;
+struct PrefixWave : WindowWave<T, D, KS, PrefixTiles<D, KS>> {
+    using Base = WindowWave<T, D, KS, PrefixTiles<D, KS>>;
     using Tiles = typename Base::Tiles;
     using typename Base::L;
     using typename Base::v8;
@@ -25,13 +68,14 @@ struct PrefixWave : WindowWave<T, D, KS> {
     using Base::smem;
     using Base::wave;
     static constexpr int SN = Base::SN, BLOCKS = SN / kStreamKeys, NW = Tiles::THREADS / 64;
-    struct Pages {
-        int id[BLOCKS];    // of each 16 keys; 0 where there is none
-        unsigned missing;  // one bit each
+    // Where the 16-key blocks of some steps stand, a block per lane.
+    struct Places {
+        uint64_t k, v;     // addresses of the first rows; of page 0's where there is no page
+        uint64_t missing;  // a bit for each block without one
     };
+    static constexpr int KEPT = 64 / BLOCKS;  // steps
 
     const StreamArgs& sa;
-    const int32_t* table;
     PrefixRow at;
     bool in;  // a row of the group
     int hk;
@@ -60,53 +104,51 @@ struct PrefixWave : WindowWave<T, D, KS> {
         this->lo_min = wave_min(this->lo);
         this->lo_max = wave_max(this->lo);
         if (pt.rt * Tiles::R * kQueriesPerWave + slice * kQueriesPerWave >= rows) this->hi_max = 0;  // no rows of its own
-        table = sa.table + pt.start * sa.table_stride;
         const int place = (64 * wave + lane) % L::CPR;
         koff = 2u * (unsigned)((dma_row0 & 15) * (int)sa.k_st + 8 * Base::src_chunk(place ^ L::kswz(dma_row0), a.D));
         voff = 2u * (unsigned)((dma_row0 & 15) * (int)sa.v_st + 8 * Base::src_chunk(place ^ L::vswz(dma_row0), a.Dv));
     }
 
-    // Pages of a staged tile; blocks past the last repeat it.
-    __device__ __forceinline__ Pages pages(int tile) const {
-        Pages p;
-        p.missing = 0;
-#pragma unroll
-        for (int j = 0; j < BLOCKS; ++j) {
-            const int key = min(tile * BLOCKS + j, a.N / kStreamKeys - 1) * kStreamKeys;
-            const int id = uniform(table[key >> sa.page_shift]);
-            const bool ok = (unsigned)id < (unsigned)sa.num_pages;
-            p.id[j] = ok ? id : 0;
-            p.missing |= ok ? 0u : 1u << j;
-        }
+    // Places of a lane's block: of step tile number `tile`, block j of it (blocks past the
+    // keys repeat the last). Formed by 64 lanes at once: as scalars, four of a step's
+    // blocks took 250 instructions of each step's time.
+    __device__ __forceinline__ Places places(int first, int tile, int j) const {
+        const int key = min(tile * BLOCKS + j, a.N / kStreamKeys - 1) * kStreamKeys;
+        const int id = sa.table[first * sa.table_stride + (key >> sa.page_shift)];
+        const bool ok = (unsigned)id < (unsigned)sa.num_pages;
+        const int64_t page = ok ? id : 0, row = key & ((1 << sa.page_shift) - 1);
+        Places p;
+        p.k = (uint64_t)sa.k + 2 * (page * sa.k_sp + hk * sa.k_sh + row * sa.k_st);
+        p.v = (uint64_t)sa.v + 2 * (page * sa.v_sp + hk * sa.v_sh + row * sa.v_st);
+        p.missing = __builtin_amdgcn_ballot_w64(!ok);
         return p;
     }
-
-    // Global -> LDS copies of a staged tile (asynchronous): copy u of a wavefront covers
-    // rows of one block.
-    static constexpr int COPY_ROWS = 64 / L::CPR;  // of a wavefront's copy: 8, 4 or 2
-    __device__ __forceinline__ void copy_pages(int tile, int stage, const Pages& p) const {
-        const unsigned lds0 = (unsigned)(uintptr_t)smem + stage + 1024 * wave;
+    static __device__ __forceinline__ uint64_t of_lane(uint64_t x, int lane) {
+        const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)x, lane);
+        const unsigned hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(x >> 32), lane);
+        return (uint64_t)hi << 32 | lo;
+    }
+    // Global -> LDS copies of a step's K or V (asynchronous) to `to`.
+    // x: K or V of the blocks; `lane` holds the step's first.
+    __device__ __forceinline__ void copy_half(uint64_t x, int lane, int64_t row_stride, unsigned off, int to) const {
+        constexpr int COPY_ROWS = 64 / L::CPR;  // of a wavefront's copy: 8, 4 or 2
+        constexpr int PER = Base::DSTEP;        // of the workgroup's: 32, 16 or 8
+        const char* base[Base::CPT];
 #pragma unroll
         for (int u = 0; u < Base::CPT; ++u) {
-            constexpr int PER = Base::DSTEP;  // rows of the workgroup's copy
-            const int block = PER >= 32 ? 2 * u + (wave * COPY_ROWS >> 4) : PER * u >> 4;
-            const int id = PER >= 32 ? (wave * COPY_ROWS >> 4 ? p.id[(2 * u + 1) % BLOCKS] : p.id[2 * u % BLOCKS]) : p.id[block];
-            const int key = min(tile * BLOCKS + block, a.N / kStreamKeys - 1) * kStreamKeys;
-            const int row = (key & ((1 << sa.page_shift) - 1)) + (PER < 16 ? PER * u & 15 : 0);
-            const T* k = (const T*)sa.k + id * sa.k_sp + hk * sa.k_sh + row * sa.k_st;
-            const T* v = (const T*)sa.v + id * sa.v_sp + hk * sa.v_sh + row * sa.v_st;
-            dma16s(k, koff, lds0 + 1024 * NW * u);
-            dma16s(v, voff, lds0 + L::KTILE + 1024 * NW * u);
+            const int block = PER >= 32 ? 2 * u + uniform(wave * COPY_ROWS >> 4) : PER * u >> 4;
+            base[u] = (const char*)(of_lane(x, lane + block) + (PER < 16 ? (PER * u & 15) * 2 * row_stride : 0));
         }
+        dma16s_row<Base::CPT>(base, off, (unsigned)(uintptr_t)smem + to + 1024 * wave, 1024 * NW);
     }
-    // V rows of a landed tile that count for nothing -> 0: past the keys, or without a page.
-    __device__ __forceinline__ void clear_rows(int tile, int stage, unsigned missing) const {
+    // V rows of a landed step that count for nothing -> 0: past the keys, or without a page.
+    __device__ __forceinline__ void clear_rows(int tile, int at_lds, unsigned missing) const {
         if (missing == 0 && tile * SN + SN <= a.N) return;
 #pragma unroll
         for (int u = 0; u < Base::CPT; ++u) {
             const int row = dma_row0 + u * Base::DSTEP;
             if (tile * SN + row >= a.N || (missing >> (row >> 4) & 1))
-                *(u32x4*)(smem + stage + L::KTILE + 1024 * wave + 1024 * NW * u + 16 * (threadIdx.x & 63)) =
+                *(u32x4*)(smem + at_lds + 1024 * wave + 1024 * NW * u + 16 * (threadIdx.x & 63)) =
                     u32x4{0u, 0u, 0u, 0u};
         }
     }
@@ -136,17 +178,23 @@ struct PrefixWave : WindowWave<T, D, KS> {
     }
 };
 
-template <typename T, int D, int KS, WindowScores SCORES>
-__global__ __launch_bounds__((WindowTiles<D, KS>::THREADS), (WindowTiles<D, KS>::WAVES_PER_SIMD))
-void prefix_fwd_kernel(StreamArgs sa) {
+// LDS of a workgroup: the ring, or the states that key groups fold.
+template <typename T, int D, int KS>
+constexpr int prefix_lds() {
     using W = PrefixWave<T, D, KS>;
-    using L = typename W::L;
+    constexpr int FOLD = KS > 1 ? (KS - 1) * W::Tiles::R * group_state_bytes(D) : 0, RING = W::Tiles::HALVES * W::L::KTILE;
+    return FOLD > RING ? FOLD : RING;
+}
+
+// Workgroup `id` of the prefix's.
+template <typename T, int D, int KS, WindowScores SCORES>
+__device__ __forceinline__ void prefix_workgroup(const StreamArgs& sa, int id, unsigned char* smem) {
+    using W = PrefixWave<T, D, KS>;
     constexpr int R = W::Tiles::R, ROWS = R * kQueriesPerWave, SN = W::SN, SB = SN / W::BN;
-    constexpr int FOLD = KS > 1 ? (KS - 1) * R * group_state_bytes(D) : 0;
-    __shared__ __attribute__((aligned(16))) unsigned char smem[FOLD > 2 * L::STAGE ? FOLD : 2 * L::STAGE];
+    constexpr int HALF = W::L::KTILE, HALVES = W::Tiles::HALVES;
     StreamPart part;
     PrefixTile pt;
-    if (!prefix_part(sa, (int)blockIdx.x, part) || !prefix_tile(sa, part.rt, ROWS, pt)) return;
+    if (!prefix_part(sa, id, part) || !prefix_tile(sa, part.rt, ROWS, pt)) return;
     FwdArgs a{};
     a.q = sa.q;
     a.k = sa.k;
@@ -161,18 +209,25 @@ void prefix_fwd_kernel(StreamArgs sa) {
     a.inv_softcap = sa.softcap > 0.0f ? 1.0f / sa.softcap : 0.0f;
     const int wave = uniform(threadIdx.x >> 6), slice = wave % R, kg = wave / R;
     W w(a, sa, smem, pt, part.hk, wave, slice);
-    // the tiles that some row of the workgroup sees: [0, sink_tiles) and [first, end)
-    __shared__ int seen[2][4];
-    if ((threadIdx.x & 63) == 0) {
-        seen[0][wave] = w.hi_max;
-        seen[1][wave] = w.lo_min;
-    }
-    __syncthreads();
-    int hi_max = 0, lo_min = 0x7fffffff;
+    // The tiles that some row of the workgroup sees: [0, sink_tiles) and [first, end).
+    // (Without a window all shared ones: where sequences end within them, masked; the
+    // lengths, a memory round trip, are then on their way beside the first keys.)
+    int* seen = (int*)smem;
+    int hi_max = pt.shared, lo_min = 0;
+    if (sa.window > 0) {
+        if ((threadIdx.x & 63) == 0) {
+            seen[wave] = w.hi_max;
+            seen[4 + wave] = w.lo_min;
+        }
+        __syncthreads();
+        hi_max = 0;
+        lo_min = 0x7fffffff;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        hi_max = max(hi_max, uniform(seen[0][i]));
-        lo_min = min(lo_min, uniform(seen[1][i]));
+        for (int i = 0; i < 4; ++i) {
+            hi_max = max(hi_max, uniform(seen[i]));
+            lo_min = min(lo_min, uniform(seen[4 + i]));
+        }
+        __syncthreads();  // (the ring takes its place)
     }
     const int end = (hi_max + SN - 1) / SN;
     int sink_tiles = 0, first = 0;
@@ -186,37 +241,83 @@ void prefix_fwd_kernel(StreamArgs sa) {
     const int begin = part.part < parts ? min(steps, part.part * per) : steps, stop = min(steps, begin + per);
     auto tile = [&](int st) { return st < sink_tiles ? st : st - sink_tiles + first; };
     auto run = [&](auto redo) {
-        auto p = w.pages(tile(begin));
-        w.copy_pages(tile(begin), 0, p);
-        auto next = w.pages(tile(min(begin + 1, stop - 1)));
-        wait_vm_loads();
-        w.clear_rows(tile(begin), 0, p.missing);
-        if (a.D < D) w.zero_pad(0);
-        __syncthreads();
+        constexpr bool REDO = decltype(redo)::value;
+        // Half h is K (even) or V (odd) of step begin + h / 2, at place h % HALVES of the
+        // ring; HALVES - 1 of them, of AHEAD steps, are on their way or in use.
+        constexpr int AHEAD = (HALVES - 1) / 2;
+        static_assert(HALVES % 2 == 1, "a step's halves are copied where those of an earlier one are used");
+        const int halves = 2 * (stop - begin);
+        auto forward = [](int x) { return x == (HALVES - 1) * HALF ? 0 : x + HALF; };
+        int to = 0, at = 0;     // places to copy to, and in use
+        uint64_t missing = 0;   // of the steps copied, four bits each, the last lowest
+        typename W::Places p;
+        int lane0 = 0;          // of the step copied last
+        auto copy_k = [&](int st) {
+            const int n = st - begin, lane = threadIdx.x & 63;
+            if (n % W::KEPT == 0)
+                p = w.places(pt.start, tile(min(st + lane / W::BLOCKS, stop - 1)), lane % W::BLOCKS);
+            lane0 = n % W::KEPT * W::BLOCKS;
+            missing = missing << 4 | (p.missing >> lane0 & ((1u << W::BLOCKS) - 1));
+            w.copy_half(p.k, lane0, sa.k_st, w.koff, to);
+            to = forward(to);
+        };
+        auto copy_v = [&] {
+            w.copy_half(p.v, lane0, sa.v_st, w.voff, to);
+            to = forward(to);
+        };
+        // Half h has landed for every wavefront, and the one before it is used up.
+        auto await = [&](int h) {
+            if (h + HALVES - 1 <= halves) wait_vm<W::CPT * (HALVES - 2)>();
+            else wait_vm_loads();
+        };
+        for (int i = 0; i < AHEAD; ++i)
+            if (begin + i < stop) {
+                copy_k(begin + i);
+                copy_v();
+            }
         for (int st = begin; st < stop; ++st) {
-            const int stage = (st - begin & 1) * L::STAGE, other = L::STAGE - stage;
-            if (st + 1 < stop) w.copy_pages(tile(st + 1), other, next);
-            const auto after = w.pages(tile(min(st + 2, stop - 1)));
-#pragma unroll
-            for (int i = 0; i < SB / KS; ++i) {
-                const int sub = i * KS + kg, k0 = tile(st) * SN + sub * W::BN;
-                if (w.sees(k0))
-                    w.template step<SCORES, decltype(redo)::value>(stage, sub, k0,
-                                                                   p.missing >> (sub * W::BN / kStreamKeys) & ((1u << W::BN / kStreamKeys) - 1));
-            }
-            wait_vm_loads();
-            if (st + 1 < stop) {
-                w.clear_rows(tile(st + 1), other, next.missing);
-                if (a.D < D) w.zero_pad(other);
-            }
-            p = next;
-            next = after;
+            const int h = 2 * (st - begin), t = tile(st), ahead = min(AHEAD, stop - st);  // steps copied from this one on
+            const unsigned gone = (unsigned)(missing >> 4 * (ahead - 1)) & 15u;
+            await(h);
+            if (a.D < D) w.zero_pad(at);
             __syncthreads();
+            if (st + AHEAD < stop) copy_k(st + AHEAD);
+            const int sub = kg, k0 = t * SN + sub * W::BN;
+            const unsigned no = gone >> (sub * W::BN / kStreamKeys) & ((1u << W::BN / kStreamKeys) - 1);
+            const bool some = w.sees(k0), partly = w.partly(k0) || no != 0;
+            if (some) {
+                __builtin_amdgcn_s_setprio(1);
+                w.qk(at, sub);
+                __builtin_amdgcn_s_setprio(0);
+                w.template softmax_window<SCORES>(k0, partly, no);
+            }
+            at = forward(at);
+            await(h + 1);
+            w.clear_rows(t, at, gone);
+            __syncthreads();
+            if (st + AHEAD < stop) copy_v();
+            const int stage = at - HALF;  // (V stands behind K there)
+            if (some && REDO && partly) {
+                w.pv_seen(stage, sub, k0);
+            } else if (some) {
+                __builtin_amdgcn_s_setprio(1);
+                w.pv(stage, sub);
+                __builtin_amdgcn_s_setprio(0);
+            }
+            at = forward(at);
         }
+        __syncthreads();
     };
+    static_assert(SB == KS, "a group has one step's scores at a time");
     if (begin < stop) {
         run(Bool<false>{});
-        if (__syncthreads_or(w.nan_in_o())) {
+        // (by hand: __syncthreads_or has LDS of its own, and two rings fill the CU's)
+        const uint64_t mine = __builtin_amdgcn_ballot_w64(w.nan_in_o());
+        if ((threadIdx.x & 63) == 0) seen[wave] = mine != 0;
+        __syncthreads();
+        const bool bad = seen[0] | seen[1] | seen[2] | seen[3];
+        __syncthreads();
+        if (uniform(bad)) {
             w.restart();
             run(Bool<true>{});
         }
@@ -226,31 +327,65 @@ void prefix_fwd_kernel(StreamArgs sa) {
         w.store_part((int64_t)part.part * sa.B * sa.Hkv * sa.T * sa.G + row_of_all(sa, w.at.b, part.hk, w.at.t, w.at.g));
 }
 
+template <typename T, int D, int KS, WindowScores SCORES>
+__global__ __launch_bounds__((PrefixTiles<D, KS>::THREADS), (PrefixTiles<D, KS>::WAVES_PER_SIMD))
+void prefix_fwd_kernel(StreamArgs a) {
+    __shared__ __attribute__((aligned(16))) unsigned char smem[prefix_lds<T, D, KS>()];
+    prefix_workgroup<T, D, KS, SCORES>(a, blockIdx.x, smem);
+}
+
+// With the plain scale, beside the sequences' own keys in one launch: the matrix cores
+// are busy with the ones while the others wait for memory.
+template <typename T, int D, int KS, int RT>
+__global__ __launch_bounds__(kStreamThreads, (PrefixTiles<D, KS>::WAVES_PER_SIMD))
+void prefix_shared_kernel(StreamArgs a) {
+    constexpr int TAIL = (kWaves - 1) * stream_state<T, D, RT>() * 4, PREFIX = prefix_lds<T, D, KS>();
+    __shared__ __attribute__((aligned(16))) unsigned char smem[PREFIX > TAIL ? PREFIX : TAIL];
+    int id;
+    if (shared_workgroup(a, blockIdx.x, id)) prefix_workgroup<T, D, KS, kScoresPlain>(a, id, smem);
+    else if (id < tail_grid(a)) stream_workgroup<T, D, RT, kTail, kPart>(a, id, (float*)smem);
+}
+
 template <typename T, int D, int KS>
-hipError_t launch_prefix_groups(const StreamArgs& a, hipStream_t s) {
-    const dim3 grid((unsigned)prefix_grid(a)), block(WindowTiles<D, KS>::THREADS);
+hipError_t launch_prefix_groups(const StreamArgs& a, int dtype, hipStream_t s) {
+    const dim3 block(kStreamThreads);
+    static_assert(PrefixTiles<D, KS>::THREADS == kStreamThreads, "both parts of a launch have its workgroup");
+    const bool plain = a.alibi == nullptr && a.softcap <= 0.0f;
+    const bool wide = D <= 128 && stream_tile_rows(dtype, D, a.T * a.G) == 32;
+    // (at D = 128 the registers of 32-row tiles leave room for one workgroup per CU: with
+    // two, 115 would spill)
+    if (plain && !(wide && D == 128)) {
+        const dim3 grid((unsigned)shared_grid(a));
+        if constexpr (D == 64)
+            if (wide) hipLaunchKernelGGL((prefix_shared_kernel<T, D, KS, 2>), grid, block, 0, s, a);
+        if (!wide) hipLaunchKernelGGL((prefix_shared_kernel<T, D, KS, 1>), grid, block, 0, s, a);
+        if (hipError_t e = hipGetLastError()) return e;
+        return launch_stream_join(a, dtype, s);
+    }
+    const dim3 grid((unsigned)prefix_grid(a));
     if (a.softcap > kCapExp) hipLaunchKernelGGL((prefix_fwd_kernel<T, D, KS, kScoresWideCap>), grid, block, 0, s, a);
-    else if (a.alibi != nullptr || a.softcap > 0.0f)
-        hipLaunchKernelGGL((prefix_fwd_kernel<T, D, KS, kScoresMod>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((prefix_fwd_kernel<T, D, KS, kScoresPlain>), grid, block, 0, s, a);
-    return hipGetLastError();
+    else if (!plain) hipLaunchKernelGGL((prefix_fwd_kernel<T, D, KS, kScoresMod>), grid, block, 0, s, a);
+    else if constexpr (D == 128) hipLaunchKernelGGL((prefix_fwd_kernel<T, D, KS, kScoresPlain>), grid, block, 0, s, a);
+    if (hipError_t e = hipGetLastError()) return e;
+    return launch_stream_tail(a, dtype, s);
 }
 template <typename T>
-hipError_t launch_prefix_type(const StreamArgs& a, int key_splits, hipStream_t s) {
+hipError_t launch_prefix_type(const StreamArgs& a, int dtype, int key_splits, hipStream_t s) {
+    const bool two = key_splits == 2;
     switch (stream_kernel_dim(a.D, a.Dv)) {
-        case 64: return key_splits == 2 ? launch_prefix_groups<T, 64, 2>(a, s) : launch_prefix_groups<T, 64, 1>(a, s);
-        case 128: return key_splits == 2 ? launch_prefix_groups<T, 128, 2>(a, s) : launch_prefix_groups<T, 128, 1>(a, s);
-        case 256: return launch_prefix_groups<T, 256, 1>(a, s);
+        case 64: return two ? launch_prefix_groups<T, 64, 2>(a, dtype, s) : launch_prefix_groups<T, 64, 1>(a, dtype, s);
+        case 128: return two ? launch_prefix_groups<T, 128, 2>(a, dtype, s) : launch_prefix_groups<T, 128, 1>(a, dtype, s);
+        case 256: return launch_prefix_groups<T, 256, 1>(a, dtype, s);
         default: return hipErrorInvalidValue;
     }
 }
 
 }  // namespace
 
-hipError_t launch_prefix(const StreamArgs& a, int dtype, int key_splits, hipStream_t s) {
+hipError_t launch_prefix_shared(const StreamArgs& a, int dtype, int key_splits, hipStream_t s) {
     switch (dtype) {
-        case DT_BF16: return launch_prefix_type<__bf16>(a, key_splits, s);
-        case DT_F16: return launch_prefix_type<_Float16>(a, key_splits, s);
+        case DT_BF16: return launch_prefix_type<__bf16>(a, dtype, key_splits, s);
+        case DT_F16: return launch_prefix_type<_Float16>(a, dtype, key_splits, s);
         default: return hipErrorInvalidValue;
     }
 }

@@ -446,7 +446,7 @@ PrefixPlan plan_prefix(const ofh::StreamArgs& a, int dtype, const ofh_prefix_gro
     plan.min_steps = plan.kernel.key_splits == 0 ? ofh::kStreamThreads / 64 : 2;
     plan.tiles = (int)(((int64_t)a.B * a.T * a.G + (int64_t)a.groups * (rows - 1)) / rows);
     const int64_t units = (int64_t)a.Hkv * plan.tiles, steps = ((int64_t)g->most_shared + step - 1) / step;
-    const int64_t n = std::min<int64_t>({(2 * ofh::kComputeUnits + units - 1) / units, steps / plan.min_steps,
+    const int64_t n = std::min<int64_t>({(plan.kernel.workgroups + units - 1) / units, steps / plan.min_steps,
                                          max_key_splits > 0 ? max_key_splits : 128});
     plan.splits = (int)std::max<int64_t>(1, n);
     const size_t tail_rows = (size_t)plan.tail.units * plan.tail.splits * plan.tail.tile_rows;
@@ -461,7 +461,8 @@ PrefixPlan plan_prefix(const ofh::StreamArgs& a, int dtype, const ofh_prefix_gro
 int run_prefix(ofh::StreamArgs& a, int dtype, const PrefixPlan& plan, void* workspace, size_t workspace_bytes,
                hipStream_t stream) {
     if (!ofh::grid_fits(plan.tail.units * plan.tail.splits, ofh::kStreamThreads) ||
-        !ofh::grid_fits(((int64_t)a.Hkv * plan.splits + 8) * plan.tiles, ofh::kStreamThreads) ||
+        !ofh::grid_fits(((int64_t)a.Hkv * plan.splits + 8) * plan.tiles + plan.tail.units * plan.tail.splits + 8,
+                        ofh::kStreamThreads) ||
         !ofh::grid_fits((int64_t)a.B * a.Hkv * a.T * a.G * ((a.Dv + 31) / 32), 64))
         return unsupported("attention call exceeds the launch range");
     ofh::ScratchLease lease;
@@ -477,9 +478,8 @@ int run_prefix(ofh::StreamArgs& a, int dtype, const PrefixPlan& plan, void* work
     a.part_ml = reinterpret_cast<float*>(at += plan.tail_o);
     a.prefix_o = reinterpret_cast<float*>(at += plan.tail_ml);
     a.prefix_ml = reinterpret_cast<float*>(at += plan.prefix_o);
-    if (plan.kernel.key_splits > 0) OFH_HIP_CHECK(ofh::launch_prefix(a, dtype, plan.kernel.key_splits, stream));
-    else OFH_HIP_CHECK(ofh::launch_stream_prefix(a, dtype, stream));
-    OFH_HIP_CHECK(ofh::launch_stream_tail(a, dtype, stream));
+    if (plan.kernel.key_splits > 0) OFH_HIP_CHECK(ofh::launch_prefix_shared(a, dtype, plan.kernel.key_splits, stream));
+    else OFH_HIP_CHECK(ofh::launch_stream_shared(a, dtype, plan.kernel.rows, stream));
     return lease.release();
 }
 

@@ -90,17 +90,24 @@ hipError_t launch_stream(const StreamArgs& a, int dtype, hipStream_t s);
 // Attention over groups of sequences that share pages, and over selected pages.
 // The prefix writes its partial rows (prefix_*); the tail's launch reads the rest
 // and joins both.
-// A prefix tile's rows, its keys' steps (of how many keys), and its workgroups.
+// How the shared keys are read: rows of a tile, keys of a step, workgroups to divide
+// them over.
 struct PrefixKernel {
     int rows, step_keys, key_splits;  // key_splits: of prefix_fwd.hip's kernel, 0: the streaming kernel
+    int workgroups;
 };
 PrefixKernel prefix_kernel(const StreamArgs& a, int dtype);
-inline int64_t prefix_grid(const StreamArgs& a) {
+__host__ __device__ inline int64_t prefix_grid(const StreamArgs& a) {  // (filled up to eights)
     return ((int64_t)a.Hkv * a.prefix_splits + 7) / 8 * 8 * a.prefix_tiles;
 }
-hipError_t launch_stream_prefix(const StreamArgs& a, int dtype, hipStream_t s);
-hipError_t launch_prefix(const StreamArgs& a, int dtype, int key_splits, hipStream_t s);
+__host__ __device__ inline int64_t tail_grid(const StreamArgs& a) { return (int64_t)a.B * a.Hkv * a.row_tiles * a.splits; }
+inline int64_t shared_grid(const StreamArgs& a) { return prefix_grid(a) + (tail_grid(a) + 7) / 8 * 8; }
+// All of a call: the streaming kernel, and the other (kernel.key_splits > 0).
+hipError_t launch_stream_shared(const StreamArgs& a, int dtype, int prefix_rows, hipStream_t s);
+hipError_t launch_prefix_shared(const StreamArgs& a, int dtype, int key_splits, hipStream_t s);
+// Parts of it: the sequences' own keys and the join, the join.
 hipError_t launch_stream_tail(const StreamArgs& a, int dtype, hipStream_t s);
+hipError_t launch_stream_join(const StreamArgs& a, int dtype, hipStream_t s);
 hipError_t launch_stream_selected(const StreamArgs& a, int dtype, hipStream_t s);
 
 // Bounds of the keys of pages: the pages that hold the last counts[b] tokens of each

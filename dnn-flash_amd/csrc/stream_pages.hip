@@ -12,13 +12,6 @@
 namespace ofh {
 namespace {
 
-template <typename T, int DK, int RT>
-hipError_t launch_prefix_rt(const StreamArgs& a, hipStream_t s) {
-    const dim3 grid((unsigned)prefix_grid(a)), block(kStreamThreads);
-    hipLaunchKernelGGL((stream_fwd_kernel<T, DK, RT, kPrefix, kPart>), grid, block, 0, s, a);
-    return hipGetLastError();
-}
-
 template <typename T, int SRC>
 hipError_t launch_join(const StreamArgs& a, int tile_rows, hipStream_t s) {
     const int64_t items = (int64_t)a.B * a.Hkv * a.T * a.G * ((a.Dv + 31) / 32);
@@ -27,9 +20,35 @@ hipError_t launch_join(const StreamArgs& a, int tile_rows, hipStream_t s) {
     return hipGetLastError();
 }
 
+// The shared part and the sequences' own in one launch (RTP: of the prefix's tiles).
+template <typename T, int DK, int RTP, int RT>
+__global__ __launch_bounds__(kStreamThreads, (RTP > RT ? stream_per_cu<T, DK, RTP>() : stream_per_cu<T, DK, RT>()))
+void stream_shared_kernel(StreamArgs a) {
+    __shared__ __attribute__((aligned(16))) float lds[(kWaves - 1) * stream_state<T, DK, (RTP > RT ? RTP : RT)>()];
+    int id;
+    if (shared_workgroup(a, blockIdx.x, id)) stream_workgroup<T, DK, RTP, kPrefix, kPart>(a, id, lds);
+    else if (id < tail_grid(a)) stream_workgroup<T, DK, RT, kTail, kPart>(a, id, lds);
+}
+template <typename T, int DK, int RTP, int RT>
+hipError_t launch_shared_rt(const StreamArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((stream_shared_kernel<T, DK, RTP, RT>), dim3((unsigned)shared_grid(a)), dim3(kStreamThreads), 0, s, a);
+    if (hipError_t e = hipGetLastError()) return e;
+    return launch_join<T, kTail>(a, 16 * RT, s);
+}
+template <typename T, int DK, int RT>
+hipError_t launch_shared(const StreamArgs& a, int prefix_rows, hipStream_t s) {
+    if (prefix_rows == 16) {
+        // (a tile of 16 rows for a group of which each sequence has more: fp32 alone)
+        if constexpr (RT == 1 || sizeof(T) == 4) return launch_shared_rt<T, DK, 1, RT>(a, s);
+    } else if constexpr (DK <= 128) {
+        return launch_shared_rt<T, DK, 2, RT>(a, s);
+    }
+    return hipErrorInvalidValue;
+}
+
 template <typename T, int DK, int RT>
 hipError_t launch_tail_rt(const StreamArgs& a, hipStream_t s) {
-    const dim3 grid((unsigned)((int64_t)a.B * a.Hkv * a.row_tiles * a.splits)), block(kStreamThreads);
+    const dim3 grid((unsigned)tail_grid(a)), block(kStreamThreads);
     hipLaunchKernelGGL((stream_fwd_kernel<T, DK, RT, kTail, kPart>), grid, block, 0, s, a);
     if (hipError_t e = hipGetLastError()) return e;
     return launch_join<T, kTail>(a, 16 * RT, s);
@@ -48,31 +67,32 @@ hipError_t launch_selected_rt(const StreamArgs& a, hipStream_t s) {
 }
 
 // What to launch: a call's dtype, kernel head dim and rows of a tile.
-enum What { kLaunchPrefix, kLaunchTail, kLaunchSelected };
+enum What { kLaunchShared, kLaunchTail, kLaunchJoin, kLaunchSelected };
 
 template <What W, typename T, int DK, int RT>
-hipError_t launch_rt(const StreamArgs& a, hipStream_t s) {
-    if constexpr (W == kLaunchPrefix) return launch_prefix_rt<T, DK, RT>(a, s);
+hipError_t launch_rt(const StreamArgs& a, int prefix_rows, hipStream_t s) {
+    if constexpr (W == kLaunchShared) return launch_shared<T, DK, RT>(a, prefix_rows, s);
     else if constexpr (W == kLaunchTail) return launch_tail_rt<T, DK, RT>(a, s);
+    else if constexpr (W == kLaunchJoin) return launch_join<T, kTail>(a, 16 * RT, s);
     else return launch_selected_rt<T, DK, RT>(a, s);
 }
 template <What W, typename T>
-hipError_t launch_type(const StreamArgs& a, int rows, hipStream_t s) {
+hipError_t launch_type(const StreamArgs& a, int rows, int prefix_rows, hipStream_t s) {
     const int dk = stream_kernel_dim(a.D, a.Dv);
     const bool wide = stream_tile_rows(sizeof(T) == 4 ? DT_F32 : DT_BF16, dk, rows) == 32;
     switch (dk) {
-        case 64: return wide ? launch_rt<W, T, 64, 2>(a, s) : launch_rt<W, T, 64, 1>(a, s);
-        case 128: return wide ? launch_rt<W, T, 128, 2>(a, s) : launch_rt<W, T, 128, 1>(a, s);
-        case 256: return launch_rt<W, T, 256, 1>(a, s);
+        case 64: return wide ? launch_rt<W, T, 64, 2>(a, prefix_rows, s) : launch_rt<W, T, 64, 1>(a, prefix_rows, s);
+        case 128: return wide ? launch_rt<W, T, 128, 2>(a, prefix_rows, s) : launch_rt<W, T, 128, 1>(a, prefix_rows, s);
+        case 256: return launch_rt<W, T, 256, 1>(a, prefix_rows, s);
         default: return hipErrorInvalidValue;
     }
 }
 template <What W>
-hipError_t launch(const StreamArgs& a, int dtype, int rows, hipStream_t s) {
+hipError_t launch(const StreamArgs& a, int dtype, int rows, int prefix_rows, hipStream_t s) {
     switch (dtype) {
-        case DT_F32: return launch_type<W, float>(a, rows, s);
-        case DT_BF16: return launch_type<W, __bf16>(a, rows, s);
-        case DT_F16: return launch_type<W, _Float16>(a, rows, s);
+        case DT_F32: return launch_type<W, float>(a, rows, prefix_rows, s);
+        case DT_BF16: return launch_type<W, __bf16>(a, rows, prefix_rows, s);
+        case DT_F16: return launch_type<W, _Float16>(a, rows, prefix_rows, s);
         default: return hipErrorInvalidValue;
     }
 }
@@ -80,23 +100,34 @@ hipError_t launch(const StreamArgs& a, int dtype, int rows, hipStream_t s) {
 }  // namespace
 
 // Groups of different sizes have one kernel: that of their average rows.
+//
+// Through LDS (16 bits, more than 32 rows): a workgroup per CU, whose other place a
+// sequence's own keys have (us, bf16 H32/8 D128, 16384 shared keys, 33-1024 of each
+// sequence's own, 256 / 512 workgroups: 64 sequences 66 / 76, 32 49 / 58, 16 31 / 40).
+// Streaming: as many as the registers let run at once, the shared part being most
+// of the work (f32 D64 B15 H8, 4000 shared, 3 tokens, two per CU: 256 27.5, 512 25.2;
+// bf16 D128 B8 H32/8 16384 shared, 32 rows, one per CU: 256 32.7, 512 40.8).
 PrefixKernel prefix_kernel(const StreamArgs& a, int dtype) {
     const int dk = stream_kernel_dim(a.D, a.Dv), rows = a.B / a.groups * a.T * a.G;
-    // (a lane of prefix_fwd.hip adds the bytes of up to 16 rows in 32 bits, as here)
     if (dtype != DT_F32 && rows > 32) {
         const int key_splits = dk <= 128 && rows <= window_rows(2) ? 2 : 1;
-        return PrefixKernel{window_rows(key_splits), 64, key_splits};
+        return PrefixKernel{window_rows(key_splits), dk == 256 ? 32 : 64, key_splits, kComputeUnits};
     }
-    return PrefixKernel{stream_tile_rows(dtype, dk, rows), stream_step_keys(dtype, dk), 0};
+    const int tile = stream_tile_rows(dtype, dk, rows);
+    const bool one = dk == 256 || (dk == 128 && tile == 32);
+    return PrefixKernel{tile, stream_step_keys(dtype, dk), 0, (one ? 1 : 2) * kComputeUnits};
 }
-hipError_t launch_stream_prefix(const StreamArgs& a, int dtype, hipStream_t s) {
-    return launch<kLaunchPrefix>(a, dtype, a.B / a.groups * a.T * a.G, s);
+hipError_t launch_stream_shared(const StreamArgs& a, int dtype, int prefix_rows, hipStream_t s) {
+    return launch<kLaunchShared>(a, dtype, a.T * a.G, prefix_rows, s);
 }
 hipError_t launch_stream_tail(const StreamArgs& a, int dtype, hipStream_t s) {
-    return launch<kLaunchTail>(a, dtype, a.T * a.G, s);
+    return launch<kLaunchTail>(a, dtype, a.T * a.G, 0, s);
+}
+hipError_t launch_stream_join(const StreamArgs& a, int dtype, hipStream_t s) {
+    return launch<kLaunchJoin>(a, dtype, a.T * a.G, 0, s);
 }
 hipError_t launch_stream_selected(const StreamArgs& a, int dtype, hipStream_t s) {
-    return launch<kLaunchSelected>(a, dtype, a.G, s);
+    return launch<kLaunchSelected>(a, dtype, a.G, 0, s);
 }
 
 }  // namespace ofh

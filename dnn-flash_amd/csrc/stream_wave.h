@@ -154,6 +154,10 @@ struct PrefixTile {
 };
 __device__ __forceinline__ bool prefix_tile(const StreamArgs& a, int tile, int rows, PrefixTile& p) {
     const int lane = threadIdx.x & 63;
+    if (a.groups == 1) {
+        p = PrefixTile{0, a.B, stream_shared(a, 0), tile};
+        return p.shared > 0 && (int64_t)tile * rows < (int64_t)a.B * a.T * a.G;
+    }
     for (int base = 0; base < a.groups; base += 64) {
         const int g = base + lane;
         int start = 0, end = 0, shared = 0;
@@ -267,6 +271,24 @@ __device__ __forceinline__ bool prefix_part(const StreamArgs& a, int id, StreamP
     p.part = unit / a.Hkv;
     p.hk = unit - p.part * a.Hkv;
     return p.part < a.prefix_splits;
+}
+
+// One launch of prefix workgroups and of the sequences' own (kTail): by turns one of
+// each per CU while both last, since the ones compute and the others read. (Eight and
+// eight, one per XCD, puts each kind on every other CU.) True for a prefix workgroup;
+// id is its number, or the other's.
+__device__ __forceinline__ bool shared_workgroup(const StreamArgs& a, int block, int& id) {
+    const int prefix = (int)prefix_grid(a), tail = (int)((tail_grid(a) + 7) / 8 * 8);
+    const int turns = min(prefix, tail) / kComputeUnits, turn = block / (2 * kComputeUnits);
+    const int rest = block - turn * 2 * kComputeUnits;
+    if (turn < turns) {
+        id = turn * kComputeUnits + rest % kComputeUnits;
+        return rest < kComputeUnits;
+    }
+    // what is left: the prefix's, then the others
+    const int left = block - turns * 2 * kComputeUnits, prefix_left = prefix - turns * kComputeUnits;
+    id = turns * kComputeUnits + (left < prefix_left ? left : left - prefix_left);
+    return left < prefix_left;
 }
 
 // Parts of a tile of `steps` steps (at most `splits`, of min_steps each), and the steps of each.
@@ -818,139 +840,29 @@ __global__ __launch_bounds__(kStreamThreads) void stream_join_kernel(StreamArgs 
     }
 }
 
-template <typename T, int DK, int RT, int SRC, int MODE>
-__global__
-__launch_bounds__(kStreamThreads, DK > 128 || (RT == 2 && DK * sizeof(T) >= 256) ? 1 : 2)
-void stream_fwd_kernel(StreamArgs a) {
-    using W = StreamWave<T, DK, RT, SRC, MODE == kOwn ? 1 : kWaves>;
-    constexpr bool SPLIT = MODE == kPart;
-    using S = typename W::S;
-    constexpr int STATE = 64 * (4 * S::NO * RT + 2 * RT);  // floats of a wavefront's state
-    __shared__ __attribute__((aligned(16))) float lds[MODE == kOwn ? 1 : (kWaves - 1) * STATE];
-    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    StreamPart at;
-    PrefixTile pt{};
-    if constexpr (SRC == kPrefix) {
-        if (!prefix_part(a, blockIdx.x, at) || !prefix_tile(a, at.rt, W::ROWS, pt)) return;
-    } else {
-        at = stream_part(a, blockIdx.x, MODE == kOwn ? (a.row_tiles + kWaves - 1) / kWaves : a.row_tiles);
-    }
-    if (MODE == kOwn) {
-        at.rt = at.rt * kWaves + wave;
-        if (at.rt >= a.row_tiles) return;
-    }
-    const StreamRange r = SRC == kPrefix ? prefix_range(a, pt, W::ROWS) : stream_range<SRC>(a, at.b, at.rt, W::ROWS);
-    const int steps = (r.blocks + S::NB - 1) / S::NB;
-    const int64_t slot = (((int64_t)at.b * a.Hkv + at.hk) * a.row_tiles + at.rt) * a.splits + at.part;
-    const int64_t total = (int64_t)a.B * a.Hkv * a.T * a.G;  // rows of all heads
-    int per = steps;
-    if constexpr (SRC == kPrefix) {
-        if (at.part >= stream_parts(a.prefix_splits, a.prefix_min_steps, steps, per)) {
-            const int row = pt.rt * W::ROWS + (int)threadIdx.x;
-            if ((int)threadIdx.x < W::ROWS && row < r.rows) {
-                const PrefixRow x = prefix_row(a, pt, row);
-                const int64_t prow = at.part * total + row_of_all(a, x.b, at.hk, x.t, x.g);
-                a.prefix_ml[2 * prow] = kNegInf;
-                a.prefix_ml[2 * prow + 1] = 0.0f;
-            }
-            return;
-        }
-    } else if (SPLIT && at.part >= stream_parts(a.splits, a.min_steps, steps, per)) {
-        // no steps: what the join reads of this part
-        if ((int)threadIdx.x < W::ROWS) {
-            a.part_ml[2 * (slot * W::ROWS + threadIdx.x)] = kNegInf;
-            a.part_ml[2 * (slot * W::ROWS + threadIdx.x) + 1] = 0.0f;
-        }
-        return;
-    }
-    W w(a, r, at, pt);
-    w.run(at.part * per + (MODE == kOwn ? 0 : wave), min(steps, (at.part + 1) * per));
-
-    // fold the wavefronts' states into wavefront 0's
-#pragma unroll
-    for (int i = 0; i < RT; ++i) w.l[i] = sum4(w.l[i]);
-    if (MODE != kOwn && wave > 0) {
-        float* st = lds + (wave - 1) * STATE;
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-#pragma unroll
-            for (int c = 0; c < S::NO; ++c) *(f32x4*)(st + 4 * (64 * (i * S::NO + c) + lane)) = w.o[i][c];
-            st[64 * 4 * S::NO * RT + 64 * (2 * i) + lane] = w.m[i];
-            st[64 * 4 * S::NO * RT + 64 * (2 * i + 1) + lane] = w.l[i];
-        }
-    }
-    if (MODE != kOwn) {
-        __syncthreads();
-        if (wave != 0) return;
-    }
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        float top = w.m[i], sum = w.l[i];
-        if constexpr (MODE != kOwn) {
-            float ms[kWaves], ls[kWaves];
-            ms[0] = w.m[i];
-            ls[0] = w.l[i];
-#pragma unroll
-            for (int k = 1; k < kWaves; ++k) {
-                const float* st = lds + (k - 1) * STATE + 64 * 4 * S::NO * RT;
-                ms[k] = st[64 * (2 * i) + lane];
-                ls[k] = st[64 * (2 * i + 1) + lane];
-                top = fmaxf(top, ms[k]);
-            }
-            const float mu = top == kNegInf ? 0.0f : top;
-            const float keep = __builtin_amdgcn_exp2f(w.m[i] - mu);
-            sum = ls[0] * keep;
-#pragma unroll
-            for (int c = 0; c < S::NO; ++c) w.o[i][c] *= keep;
-#pragma unroll
-            for (int k = 1; k < kWaves; ++k) {
-                const float f = __builtin_amdgcn_exp2f(ms[k] - mu);
-                sum += f * ls[k];
-#pragma unroll
-                for (int c = 0; c < S::NO; ++c) {
-                    const f32x4 v = *(const f32x4*)(lds + (k - 1) * STATE + 4 * (64 * (i * S::NO + c) + lane));
-                    w.o[i][c] += f * v;
-                }
-            }
-        }
-        // row n, columns 16 VW c + VW (4 g + e) + 0 .. VW - 1
-        const int row = (SRC == kPrefix ? pt.rt : at.rt) * W::ROWS + 16 * i + w.n;
-        if (row >= (SRC == kPrefix ? r.rows : a.T * a.G)) continue;
-        const int t = row / a.G, h = w.hk * a.G + row - t * a.G;
-        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-        int64_t off = w.b * a.o_sb + h * a.o_sh + t * a.o_st;
-        if constexpr (SRC == kSelected) off = w.b / a.tokens * a.o_sb + h * a.o_sh + w.b % a.tokens * a.o_st;
-        int64_t prow = slot * W::ROWS + 16 * i + w.n;
-        float* part_o = a.part_o;
-        float* part_ml = a.part_ml;
-        if constexpr (SRC == kPrefix) {
-            const PrefixRow x = prefix_row(a, pt, row);
-            prow = at.part * total + row_of_all(a, x.b, w.hk, x.t, x.g);
-            part_o = a.prefix_o;
-            part_ml = a.prefix_ml;
-        }
-#pragma unroll
-        for (int c = 0; c < S::VC; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int col = 16 * S::VW * c + S::VW * (4 * w.g + e);
-                if (col >= a.Dv) continue;
-                float x[S::VW];
-#pragma unroll
-                for (int k = 0; k < S::VW; ++k) x[k] = w.o[i][c * S::VW + k][e];
-                if (!SPLIT) {
-                    put_out<T, S::VW>(a, off + col, x, inv);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < S::VW; k += 4)
-                        *(f32x4*)(part_o + prow * a.Dv + col + k) = f32x4{x[k], x[k + 1], x[k + 2], x[k + 3]};
-                }
-            }
-        if (SPLIT && w.g == 0) {
-            part_ml[2 * prow] = top;
-            part_ml[2 * prow + 1] = sum;
-        }
-    }
+// Workgroups of a CU that the registers leave room for.
+template <typename T, int DK, int RT>
+constexpr int stream_per_cu() {
+    return DK > 128 || (RT == 2 && DK * sizeof(T) >= 256) ? 1 : 2;
 }
+// Floats of a wavefront's state.
+template <typename T, int DK, int RT>
+constexpr int stream_state() {
+    return 64 * (4 * StreamTile<T, DK>::NO * RT + 2 * RT);
+}
+
+template <typename T, int DK, int RT, int SRC, int MODE>
+__device__ __forceinline__ void stream_workgroup(const StreamArgs& a, int id, float* lds) {
+#include "stream_workgroup.inc"
+}
+
+template <typename T, int DK, int RT, int SRC, int MODE>
+__global__ __launch_bounds__(kStreamThreads, (stream_per_cu<T, DK, RT>()))
+void stream_fwd_kernel(StreamArgs a) {
+    __shared__ __attribute__((aligned(16))) float lds[MODE == kOwn ? 1 : (kWaves - 1) * stream_state<T, DK, RT>()];
+    const int id = blockIdx.x;
+#include "stream_workgroup.inc"
+}
+
 }  // namespace
 }  // namespace ofh

@@ -39,10 +39,9 @@ struct Bool {
     static constexpr bool value = B;
 };
 
-template <typename T, int D, int KS>
-struct WindowWave : Wave32<T, D, MOD_PLAIN, false, WindowTiles<D, KS>::THREADS, WindowTiles<D, KS>::BN,
-                           WindowTiles<D, KS>::SB> {
-    using Tiles = WindowTiles<D, KS>;
+template <typename T, int D, int KS, typename Tiles_ = WindowTiles<D, KS>>
+struct WindowWave : Wave32<T, D, MOD_PLAIN, false, Tiles_::THREADS, Tiles_::BN, Tiles_::SB> {
+    using Tiles = Tiles_;
     using Base = Wave32<T, D, MOD_PLAIN, false, Tiles::THREADS, Tiles::BN, Tiles::SB>;
     using typename Base::L;
     using typename Base::M16;
@@ -277,12 +276,12 @@ struct WindowWave : Wave32<T, D, MOD_PLAIN, false, WindowTiles<D, KS>::THREADS, 
 
     // SEEN: partly masked tiles are added key by key.
     template <WindowScores SCORES, bool SEEN>
-    __device__ __forceinline__ void step(int stage, int sub, int k0, unsigned missing = 0) {
-        const bool mask = partly(k0) || missing != 0;
+    __device__ __forceinline__ void step(int stage, int sub, int k0) {
+        const bool mask = partly(k0);
         __builtin_amdgcn_s_setprio(1);
         this->qk(stage, sub);
         __builtin_amdgcn_s_setprio(0);
-        softmax_window<SCORES>(k0, mask, missing);
+        softmax_window<SCORES>(k0, mask);
         if (SEEN && mask) {
             pv_seen(stage, sub, k0);
             return;
