@@ -36,6 +36,11 @@ struct Words {
     }
 };
 
+template <int N>
+struct Number {
+    static constexpr int value = N;
+};
+
 // A NaN stays.
 __device__ __forceinline__ float lower(float a, float b) { return b < a || b != b ? b : a; }
 __device__ __forceinline__ float upper(float a, float b) { return b > a || b != b ? b : a; }
@@ -44,12 +49,12 @@ __device__ __forceinline__ float upper(float a, float b) { return b > a || b != 
 __device__ __forceinline__ int row_lanes(int words) { return words <= 1 ? 1 : 1 << (32 - __builtin_clz(words - 1)); }
 
 // A wavefront per touched page and key-value head: its lanes take the words of a
-// row and, beside each other, several rows, four of which are in flight per lane.
+// row and, beside each other, several rows, four or eight of which are in flight per lane.
 // Bound by reading the page's keys once; a decode step's few pages by the launch.
 template <typename T>
 __global__ __launch_bounds__(kSelectThreads) void page_bounds_kernel(PageBoundsArgs a) {
     using X = Words<T>;
-    constexpr int W = X::W, AHEAD = 4;
+    constexpr int W = X::W;
     const int lane = threadIdx.x & 63;
     const int64_t item = (int64_t)blockIdx.x * kSelectWaves + (threadIdx.x >> 6);
     const int64_t bi = item / a.Hkv;
@@ -72,21 +77,26 @@ __global__ __launch_bounds__(kSelectThreads) void page_bounds_kernel(PageBoundsA
         lo[j] = __builtin_huge_valf();
         hi[j] = kNegInf;
     }
-    for (int r = group; r < rows; r += AHEAD * groups) {
-        u32x4 x[AHEAD];
+    auto read = [&](auto ahead) {  // rows of a lane in flight
+        constexpr int AHEAD = decltype(ahead)::value;
+        for (int r = group; r < rows; r += AHEAD * groups) {
+            u32x4 x[AHEAD];
 #pragma unroll
-        for (int n = 0; n < AHEAD; ++n) x[n] = *(const u32x4*)(keys + (int64_t)min(r + n * groups, rows - 1) * a.k_st);
+            for (int n = 0; n < AHEAD; ++n) x[n] = *(const u32x4*)(keys + (int64_t)min(r + n * groups, rows - 1) * a.k_st);
 #pragma unroll
-        for (int n = 0; n < AHEAD; ++n) {
-            float f[W];
-            X::get(x[n], f);
+            for (int n = 0; n < AHEAD; ++n) {
+                float f[W];
+                X::get(x[n], f);
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-                lo[j] = lower(lo[j], f[j]);
-                hi[j] = upper(hi[j], f[j]);
+                for (int j = 0; j < W; ++j) {
+                    lo[j] = lower(lo[j], f[j]);
+                    hi[j] = upper(hi[j], f[j]);
+                }
             }
         }
-    }
+    };
+    if (rows > 4 * groups) read(Number<8>{});
+    else read(Number<4>{});
     for (int d = lanes; d < 64; d *= 2)
 #pragma unroll
         for (int j = 0; j < W; ++j) {
@@ -161,12 +171,14 @@ __global__ __launch_bounds__(kSelectThreads) void page_score_kernel(SelectArgs a
     const int rows = a.B * a.Hkv * a.T, chunk = blockIdx.x / rows;
     const int64_t row = blockIdx.x - (int64_t)chunk * rows;  // (b, hk, t)
     const int t = (int)(row % a.T), hk = (int)(row / a.T % a.Hkv), b = (int)(row / a.T / a.Hkv);
-    const int have = candidates(a, b, t);
-    const int page0 = chunk * per, page1 = min(have, page0 + per);
-    if (have <= a.pages || page0 >= have) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int words = a.D / W, beside = 64 / lanes;
     const int sub = lane & (lanes - 1), slot = lane / lanes;
+    // (the first page's table entry is read beside the length, not after it)
+    const int page0 = chunk * per, start = page0 + wave * beside + slot;
+    const int first_page = a.table[b * a.table_stride + min(start, a.max_pages - 1)];
+    const int have = candidates(a, b, t), page1 = min(have, page0 + per);
+    if (have <= a.pages || page0 >= have) return;
     for (int g0 = 0; g0 < a.G; g0 += heads_kept) {
         const int heads = min(heads_kept, a.G - g0);
         __syncthreads();
@@ -186,8 +198,9 @@ __global__ __launch_bounds__(kSelectThreads) void page_score_kernel(SelectArgs a
             masks[n] = m;
         }
         __syncthreads();
-        for (int p = page0 + wave * beside + slot; p - slot < page1; p += kSelectWaves * beside) {
-            const int page = a.table[b * a.table_stride + min(p, page1 - 1)];
+        for (int p = start; p - slot < page1; p += kSelectWaves * beside) {
+            // (lanes past the last page score some page of the table, for nothing)
+            const int page = p == start ? first_page : a.table[b * a.table_stride + min(p, page1 - 1)];
             const bool ok = (unsigned)page < (unsigned)a.num_pages;
             const T* at = (const T*)a.bounds + (ok ? page : 0) * a.b_sp + hk * a.b_sh;
             u32x4 lo[kScoreWords], hi[kScoreWords];
@@ -243,11 +256,19 @@ __global__ __launch_bounds__(kPickThreads) void page_select_kernel(SelectArgs a)
     __shared__ int found[3];
     __shared__ int sums[2][kPickWaves];
     __shared__ uint32_t ends[2][kPickWaves];
+    constexpr int EARLY = 4;
     const int64_t row = blockIdx.x;
     const int t = (int)(row % a.T), b = (int)(row / a.T / a.Hkv);
-    const int have = candidates(a, b, t);
     int32_t* out = a.selected + row * a.pages;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // the first scores are read beside the length (what is there past the candidates is
+    // not used; no scores are there when every sequence of the table may take all)
+    uint32_t early[EARLY] = {};
+    if (a.max_pages > a.pages)
+#pragma unroll
+        for (int i = 0; i < EARLY; ++i)
+            early[i] = a.scores[row * a.max_pages + min(a.first_pages + tid + i * kPickThreads, a.max_pages - 1)];
+    const int have = candidates(a, b, t);
     if (have <= a.pages) {
         for (int i = tid; i < a.pages; i += kPickThreads) out[i] = i < have ? i : -1;
         return;
@@ -256,13 +277,17 @@ __global__ __launch_bounds__(kPickThreads) void page_select_kernel(SelectArgs a)
     const int n = have - a.first_pages - a.recent_pages, need = a.pages - a.first_pages - a.recent_pages;
     const bool keep = n <= kSelectKept;
     uint32_t low = ~0u, high = 0;
-    if (need > 0)
-        for (int i = tid; i < n; i += kPickThreads) {
-            const uint32_t x = scores[i];
+    if (need > 0) {
+        auto take = [&](int i, uint32_t x) {
             if (keep) kept[i] = x;
             low = min(low, x);
             high = max(high, x);
-        }
+        };
+#pragma unroll
+        for (int i = 0; i < EARLY; ++i)
+            if (tid + i * kPickThreads < n) take(tid + i * kPickThreads, early[i]);
+        for (int i = tid + EARLY * kPickThreads; i < n; i += kPickThreads) take(i, scores[i]);
+    }
     // (the first and the recent pages)
     for (int i = tid; i < a.first_pages; i += kPickThreads) out[i] = i;
     for (int i = tid; i < a.recent_pages; i += kPickThreads) out[a.pages - a.recent_pages + i] = have - a.recent_pages + i;

@@ -352,6 +352,10 @@ struct StreamWave {
     const char* kbase;
     const char* vbase;
     unsigned koff, voff[4];
+    // kSelected: entries listed + lane of the row's list: the entry's first key, and its
+    // page (-1: selects nothing). 64 lanes look them up at once; one after the other,
+    // list and table were two memory round trips for every step.
+    int listed, listed_key, listed_page;
 
     __device__ __forceinline__ StreamWave(const StreamArgs& args, const StreamRange& range, const StreamPart& at,
                                           const PrefixTile& pt)
@@ -393,6 +397,7 @@ struct StreamWave {
             pos[i] = (int)(r.first_pos + t);
             slope[i] = a.alibi != nullptr ? a.alibi[h] : 0.0f;
         }
+        if constexpr (SRC == kSelected) look_up(0);
         limits(r.t0, hi_min, lo_min);
         limits(r.t1, hi_max, lo_max);
         // (with padding rows in the tile the last token sees none: the rows before it set the range)
@@ -442,21 +447,27 @@ struct StreamWave {
         if (SRC == kSelected) return p.key[j];
         return uniform(kStreamKeys * r.template block<SRC>(min(step * S::NB + j, r.blocks - 1)));
     }
-    __device__ __forceinline__ Pages pages(int step) const {
+    // An entry outside the table's row, or not above the one before it, selects nothing.
+    __device__ __forceinline__ void look_up(int first) {
+        listed = first;
+        const int e = min(first + (int)(threadIdx.x & 63), a.num_selected - 1), seq = b / a.tokens;
+        const int32_t* list = a.selected + (((int64_t)seq * a.Hkv + hk) * a.tokens + b - seq * a.tokens) * a.num_selected;
+        const int page = list[e], before = e > 0 ? list[e - 1] : -1;
+        const bool ok = page > before && page < a.capacity >> a.page_shift;
+        listed_key = ok ? page << a.page_shift : 0;
+        const int id = a.table[seq * a.table_stride + (listed_key >> a.page_shift)];
+        listed_page = ok ? id : -1;
+    }
+    __device__ __forceinline__ Pages pages(int step) {
         Pages p;
         if constexpr (SRC == kSelected) {
-            // An entry outside the table's row, or not above the one before it, selects nothing.
-            const int seq = b / a.tokens;
-            const int32_t* list = a.selected + (((int64_t)seq * a.Hkv + hk) * a.tokens + b - seq * a.tokens) * a.num_selected;
             const int shift = a.page_shift - 4;
 #pragma unroll
             for (int j = 0; j < S::NB; ++j) {
                 const int i = uniform(min(step * S::NB + j, r.blocks - 1)), e = i >> shift;
-                const int page = list[e], before = e > 0 ? list[e - 1] : -1;
-                const bool ok = page > before && page < a.capacity >> a.page_shift;
-                p.key[j] = uniform(ok ? (page << a.page_shift) + kStreamKeys * (i - (e << shift)) : 0);
-                const int id = a.table[seq * a.table_stride + (p.key[j] >> a.page_shift)];
-                p.id[j] = ok ? id : -1;
+                if (e < listed || e >= listed + 64) look_up(e);
+                p.key[j] = __builtin_amdgcn_readlane(listed_key, e - listed) + kStreamKeys * (i - (e << shift));
+                p.id[j] = __builtin_amdgcn_readlane(listed_page, e - listed);
             }
             return p;
         }

@@ -1412,6 +1412,7 @@ class Rotary:
         p.head_dim = head_dim
         self._fields(p.rotary)
         self._params = bytes(p)
+        self._held = None  # (layout of the last call, its parameters): calls are laid out alike
 
     def _fields(self, r: RotaryFields) -> None:
         r.frequencies, r.rotary_dim = self.frequencies.data_ptr(), self.rotary_dim
@@ -1425,30 +1426,28 @@ class Rotary:
         T of lengths[b] tokens). `transpose` turns back: the gradient of x from
         that of the result. out: x itself, or a tensor like it. Returns out."""
         torch, dev = self._torch, self._device
-        if not (isinstance(x, torch.Tensor) and x.dtype in _DTYPE_CODES and _is_rows(torch, x, x.dtype, dev)):
-            _check_rows(torch, "x", x, 4, None, dev)
+        layout = (x.shape, x.stride(), x.dtype, x.device) if isinstance(x, torch.Tensor) else None
+        held = self._held
+        if held is None or layout != held[0]:
+            held = self._held = (layout, self._lay_out(x))
         B, H, T, D = x.shape
-        if D != self.head_dim:
-            raise ValueError(f"x must have rows of {self.head_dim} columns")
-        if type(offset) is not int or not -(1 << 31) <= offset < 1 << 31:
-            raise ValueError("offset must be an integer within 32 bits")
+        p = RotaryParams.from_buffer_copy(held[1])
+        if offset != 0 or type(offset) is not int:
+            if type(offset) is not int or not -(1 << 31) <= offset < 1 << 31:
+                raise ValueError("offset must be an integer within 32 bits")
+            p.offset = offset
+        if transpose:
+            p.transpose = 1
         if (positions is not None) + (lengths is not None) + (offset != 0) > 1:
             raise ValueError("pass one of offset, positions and lengths")
-        p = RotaryParams.from_buffer_copy(self._params)
-        p.batch, p.heads, p.tokens, p.dtype, p.offset = B, H, T, _DTYPE_CODES[x.dtype], offset
-        p.transpose = int(bool(transpose))
         if positions is not None:
             _check_ints(torch, "positions", positions, (T,) if isinstance(positions, torch.Tensor) and positions.dim() == 1
                         else (B, T), dev)
-            if min(positions.stride()) < 0:
-                raise ValueError("positions: strides must be non-negative")
             p.positions = positions.data_ptr()
             p.position_stride = positions.stride(0) if positions.dim() == 2 and B > 1 else 0
         elif lengths is not None:
             _check_ints(torch, "lengths", lengths, (B,), dev)
             p.lengths = lengths.data_ptr()
-        if not x.is_contiguous():
-            p.x_strides[:] = _axis_strides("x", x)
         if out is None:
             out = torch.empty((B, H, T, D), dtype=x.dtype, device=dev)
         else:
@@ -1456,17 +1455,30 @@ class Rotary:
             if out.shape != x.shape:
                 raise ValueError(f"out must have shape {tuple(x.shape)}")
             _check_written("out", out)
-        if not out.is_contiguous():
-            p.o_strides[:] = _axis_strides("out", out)
-        if out.data_ptr() == x.data_ptr():
-            # (axes of one element have any stride)
-            if _axis_strides("out", out) != _axis_strides("x", x):
-                raise ValueError("x turned in place must keep its strides")
-            p.o_strides[:] = p.x_strides[:]
+            if not out.is_contiguous():
+                p.o_strides[:] = _axis_strides("out", out)
+            if out.data_ptr() == x.data_ptr():
+                # (axes of one element have any stride)
+                if _axis_strides("out", out) != _axis_strides("x", x):
+                    raise ValueError("x turned in place must keep its strides")
+                p.o_strides[:] = p.x_strides[:]
         rc = _launch(torch, dev, stream, self._lib.ofh_rotary_fwd, ctypes.addressof(p), x.data_ptr(), out.data_ptr())
         if rc != OFH_SUCCESS:
             check(rc)
         return out
+
+    def _lay_out(self, x) -> bytes:
+        """Checks x and its layout; the parameters of a call with a contiguous result."""
+        torch, dev = self._torch, self._device
+        if not (isinstance(x, torch.Tensor) and x.dtype in _DTYPE_CODES and _is_rows(torch, x, x.dtype, dev)):
+            _check_rows(torch, "x", x, 4, None, dev)
+        if x.shape[3] != self.head_dim:
+            raise ValueError(f"x must have rows of {self.head_dim} columns")
+        p = RotaryParams.from_buffer_copy(self._params)
+        p.batch, p.heads, p.tokens, p.dtype = *x.shape[:3], _DTYPE_CODES[x.dtype]
+        if not x.is_contiguous():
+            p.x_strides[:] = _axis_strides("x", x)
+        return bytes(p)
 
 
 class CacheAppender:
@@ -1488,13 +1500,44 @@ class CacheAppender:
         rotary._fields(p.rotary)
         self._params = bytes(p)
         self._append = L.ofh_cache_append
+        self._held = None  # (layout of the last call, its parameters): steps are laid out alike
 
     def __call__(self, k, v, q=None, *, q_out=None, stream=None):
         """k: [B,Hkv,T,D], v: [B,Hkv,T,Dv], the (padded) new rows; q: [B,H,T,D].
         Returns the turned q (q_out: q itself, or a tensor like it), whose rows at
         t >= counts[b] are 0; None without q."""
         w = self._writer
-        torch, dev, dtype = w._torch, w._device, w._dtype
+        torch, dev = w._torch, w._device
+        tensor = torch.Tensor
+        layout = None
+        if isinstance(k, tensor) and isinstance(v, tensor) and (q is None or isinstance(q, tensor)):
+            layout = (k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device)
+            if q is not None:
+                layout += (q.shape, q.stride(), q.dtype, q.device)
+        held = self._held
+        if held is not None and layout == held[0]:
+            p = held[1]
+        else:
+            p = self._lay_out(k, v, q)
+            self._held = (layout, p)
+        q_ptr = out_ptr = None
+        if q is not None:
+            q_ptr = q.data_ptr()
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            else:
+                p = self._lay_out_result(p, q, q_out)
+            out_ptr = q_out.data_ptr()
+        elif q_out is not None:
+            raise ValueError("q_out needs q")
+        rc = _launch(torch, dev, stream, self._append, p, k.data_ptr(), v.data_ptr(), q_ptr, *w._ptrs, out_ptr)
+        if rc != OFH_SUCCESS:
+            check(rc)
+        return q_out
+
+    def _lay_out(self, k, v, q) -> bytes:
+        """Checks the rows and their layout; the parameters of a call with a contiguous q_out."""
+        w = self._writer
         T = w._check_new(k, v)
         B, _, D, _ = w._row
         p = CacheAppendParams.from_buffer_copy(self._params)
@@ -1503,37 +1546,31 @@ class CacheAppender:
             p.cache.k_strides[:] = _axis_strides("k", k)
         if not v.is_contiguous():
             p.cache.v_strides[:] = _axis_strides("v", v)
-        q_ptr = out_ptr = None
         if q is not None:
-            if not _is_rows(torch, q, dtype, dev):
-                _check_rows(torch, "q", q, 4, dtype, dev)
-            H = q.shape[1]
-            if q.shape != (B, H, T, D):
+            if not _is_rows(w._torch, q, w._dtype, w._device):
+                _check_rows(w._torch, "q", q, 4, w._dtype, w._device)
+            if q.shape != (B, q.shape[1], T, D):
                 raise ValueError(f"q must be {(B, 'H', T, D)}")
-            p.heads = H
+            p.heads = q.shape[1]
             if not q.is_contiguous():
                 p.q_strides[:] = _axis_strides("q", q)
-            if q_out is None:
-                q_out = torch.empty((B, H, T, D), dtype=dtype, device=dev)
-            else:
-                _check_rows(torch, "q_out", q_out, 4, dtype, dev)
-                if q_out.shape != q.shape:
-                    raise ValueError(f"q_out must have shape {tuple(q.shape)}")
-                _check_written("q_out", q_out)
-            if not q_out.is_contiguous():
-                p.o_strides[:] = _axis_strides("q_out", q_out)
-            q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
-            if q_ptr == out_ptr:
-                if _axis_strides("q_out", q_out) != _axis_strides("q", q):
-                    raise ValueError("q turned in place must keep its strides")
-                p.o_strides[:] = p.q_strides[:]
-        elif q_out is not None:
-            raise ValueError("q_out needs q")
-        rc = _launch(torch, dev, stream, self._append, ctypes.addressof(p), k.data_ptr(), v.data_ptr(), q_ptr, *w._ptrs,
-                     out_ptr)
-        if rc != OFH_SUCCESS:
-            check(rc)
-        return q_out
+        return bytes(p)
+
+    def _lay_out_result(self, params: bytes, q, q_out) -> bytes:
+        w = self._writer
+        _check_rows(w._torch, "q_out", q_out, 4, w._dtype, w._device)
+        if q_out.shape != q.shape:
+            raise ValueError(f"q_out must have shape {tuple(q.shape)}")
+        _check_written("q_out", q_out)
+        p = CacheAppendParams.from_buffer_copy(params)
+        if not q_out.is_contiguous():
+            p.o_strides[:] = _axis_strides("q_out", q_out)
+        if q_out.data_ptr() == q.data_ptr():
+            # (axes of one element have any stride)
+            if _axis_strides("q_out", q_out) != _axis_strides("q", q):
+                raise ValueError("q turned in place must keep its strides")
+            p.o_strides[:] = p.q_strides[:]
+        return bytes(p)
 
 
 def cache_append(k, v, k_pages, v_pages, page_table, lengths, rotary: Rotary, *, q=None, q_out=None, counts=None,
