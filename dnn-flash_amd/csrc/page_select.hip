@@ -416,7 +416,8 @@ hipError_t launch_page_bounds(const PageBoundsArgs& a, int dtype, hipStream_t s)
 }
 
 bool page_select_fits(const SelectArgs& a) {
-    return grid_fits((int64_t)a.B * a.Hkv * a.T * score_chunks(a), kSelectThreads);
+    const int64_t rows = (int64_t)a.B * a.Hkv * a.T;
+    return grid_fits(rows * score_chunks(a), kSelectThreads) && grid_fits(rows, kPickThreads);
 }
 
 hipError_t launch_page_select(const SelectArgs& a, int dtype, hipStream_t s) {

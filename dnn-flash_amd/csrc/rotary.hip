@@ -6,7 +6,8 @@
 // The angle is formed in 64 bits in turns and brought within half a turn
 // there, so that far positions keep their digits: p f_i / 2 pi is off by 2^-52 of
 // itself, 2^-31 turns at p = 2^21, where 32 bits would be off by a sixteenth of
-// a turn. Sine and cosine are then fp32, like the products; the result is rounded once.
+// a turn. Sine and cosine are then fp32, with what the angle's rounding to fp32 takes
+// off put back to first order, and so are the products; the result is rounded once.
 //
 // Both kernels are bound by reading and writing each row once. A wavefront (or,
 // with few tokens, each of four) takes a token: its place and position are scalars,
@@ -22,6 +23,7 @@ constexpr int kRotaryThreads = 256;
 constexpr int kRotaryWaves = kRotaryThreads / 64;
 constexpr int kInFlight = 4;  // rows of a lane whose loads are issued together
 constexpr double kTurn = 0.15915494309189533577;  // 1 / (2 pi)
+constexpr double kHalfTurn = 3.14159265358979323846;
 
 template <int BYTES>
 struct Word;
@@ -104,10 +106,12 @@ struct Row {
 };
 
 __device__ __forceinline__ float2 turn(const Rotation& r, int pair, int64_t position) {
-    const double turns = (double)position * (r.freq[pair] * kTurn);
+    const double turns = (double)position * (r.freq[pair] * kTurn), halves = 2.0 * (turns - __builtin_rint(turns));
+    const float x = (float)halves, off = (float)((halves - (double)x) * kHalfTurn);
     float s, c;
-    sincospif((float)(2.0 * (turns - __builtin_rint(turns))), &s, &c);
-    return float2{c * r.magnitude, (r.transpose ? -s : s) * r.magnitude};
+    sincospif(x, &s, &c);
+    const float s1 = __builtin_fmaf(c, off, s), c1 = __builtin_fmaf(-s, off, c);
+    return float2{c1 * r.magnitude, (r.transpose ? -s1 : s1) * r.magnitude};
 }
 
 // Items of a row.

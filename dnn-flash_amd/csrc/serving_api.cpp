@@ -425,13 +425,14 @@ int prefix_args(const ofh_paged_params* p, const ofh_prefix_groups* g, bool chec
         return invalid("starts and shared_tokens must be non-null");
     if (g->least_shared > g->most_shared || g->most_shared > p->max_pages * p->page_size)
         return invalid("least_shared and most_shared must be within the table's tokens, in this order");
+    if (g->sharing_groups > g->groups || g->sharing_sequences > p->batch || g->most_sequences > p->batch)
+        return invalid("sharing groups and sequences must be within the batch's");
     // (rows of all sequences are numbered in 32 bits)
     if ((uint64_t)p->batch * p->heads * p->query_tokens > (uint64_t)kMaxTokens)
         return unsupported("attention dimensions exceed the 32-bit index range");
     a.group_starts = g->starts;
     a.shared = g->shared_tokens;
     a.groups = (int)g->groups;
-    a.max_shared = (int)g->most_shared;
     return OFH_SUCCESS;
 }
 
@@ -440,11 +441,14 @@ PrefixPlan plan_prefix(const ofh::StreamArgs& a, int dtype, const ofh_prefix_gro
     ofh::StreamArgs own = a;
     own.capacity = std::max(a.capacity - (int)g->least_shared, 1);
     plan.tail = plan_split(own, dtype, max_key_splits);
-    plan.kernel = ofh::prefix_kernel(a, dtype);
+    const int64_t groups = g->sharing_groups > 0 ? (int64_t)g->sharing_groups : a.groups;
+    const int64_t sequences = g->sharing_sequences > 0 ? (int64_t)g->sharing_sequences : a.B;
+    const int64_t largest = g->most_sequences > 0 ? (int64_t)g->most_sequences : (sequences + groups - 1) / groups;
+    plan.kernel = ofh::prefix_kernel(a, dtype, (int)(largest * a.T * a.G));
     const int rows = plan.kernel.rows, step = plan.kernel.step_keys;
     // (a wavefront of the streaming kernel takes a step, a workgroup of the other)
     plan.min_steps = plan.kernel.key_splits == 0 ? ofh::kStreamThreads / 64 : 2;
-    plan.tiles = (int)(((int64_t)a.B * a.T * a.G + (int64_t)a.groups * (rows - 1)) / rows);
+    plan.tiles = (int)((sequences * a.T * a.G + groups * (rows - 1)) / rows);
     const int64_t units = (int64_t)a.Hkv * plan.tiles, steps = ((int64_t)g->most_shared + step - 1) / step;
     const int64_t n = std::min<int64_t>({(plan.kernel.workgroups + units - 1) / units, steps / plan.min_steps,
                                          max_key_splits > 0 ? max_key_splits : 128});

@@ -55,7 +55,7 @@ struct StreamArgs {
     // group's first sequence.
     const int32_t* group_starts;
     const int32_t* shared;
-    int groups, max_shared;
+    int groups;
     int prefix_tiles, prefix_splits, prefix_min_steps;
     float* prefix_o;   // [prefix_splits][B Hkv T G][Dv]
     float* prefix_ml;  // [prefix_splits][B Hkv T G][2]
@@ -96,7 +96,7 @@ struct PrefixKernel {
     int rows, step_keys, key_splits;  // key_splits: of prefix_fwd.hip's kernel, 0: the streaming kernel
     int workgroups;
 };
-PrefixKernel prefix_kernel(const StreamArgs& a, int dtype);
+PrefixKernel prefix_kernel(const StreamArgs& a, int dtype, int rows);  // of the largest group
 __host__ __device__ inline int64_t prefix_grid(const StreamArgs& a) {  // (filled up to eights)
     return ((int64_t)a.Hkv * a.prefix_splits + 7) / 8 * 8 * a.prefix_tiles;
 }

@@ -99,7 +99,7 @@ hipError_t launch(const StreamArgs& a, int dtype, int rows, int prefix_rows, hip
 
 }  // namespace
 
-// Groups of different sizes have one kernel: that of their average rows.
+// Groups of different sizes have one kernel: the largest one's.
 //
 // Through LDS (16 bits, more than 32 rows): a workgroup per CU, whose other place a
 // sequence's own keys have (us, bf16 H32/8 D128, 16384 shared keys, 33-1024 of each
@@ -107,8 +107,8 @@ hipError_t launch(const StreamArgs& a, int dtype, int rows, int prefix_rows, hip
 // Streaming: as many as the registers let run at once, the shared part being most
 // of the work (f32 D64 B15 H8, 4000 shared, 3 tokens, two per CU: 256 27.5, 512 25.2;
 // bf16 D128 B8 H32/8 16384 shared, 32 rows, one per CU: 256 32.7, 512 40.8).
-PrefixKernel prefix_kernel(const StreamArgs& a, int dtype) {
-    const int dk = stream_kernel_dim(a.D, a.Dv), rows = a.B / a.groups * a.T * a.G;
+PrefixKernel prefix_kernel(const StreamArgs& a, int dtype, int rows) {
+    const int dk = stream_kernel_dim(a.D, a.Dv);
     if (dtype != DT_F32 && rows > 32) {
         const int key_splits = dk <= 128 && rows <= window_rows(2) ? 2 : 1;
         return PrefixKernel{window_rows(key_splits), dk == 256 ? 32 : 64, key_splits, kComputeUnits};

@@ -270,6 +270,9 @@ class PrefixGroupsParams(ctypes.Structure):
         ("shared_tokens", ctypes.c_void_p),
         ("least_shared", ctypes.c_size_t),
         ("most_shared", ctypes.c_size_t),
+        ("most_sequences", ctypes.c_size_t),
+        ("sharing_groups", ctypes.c_size_t),
+        ("sharing_sequences", ctypes.c_size_t),
     ]
 
 
@@ -1075,6 +1078,8 @@ class PrefixGroups:
         lib().ofh_prefix_groups_init(ctypes.addressof(p))
         p.groups, p.starts, p.shared_tokens = len(groups), *(t.data_ptr() for t in self._held)
         p.least_shared, p.most_shared = min(shared), max(shared)
+        sharing = [n for n, tokens in groups if tokens > 0]
+        p.most_sequences, p.sharing_groups, p.sharing_sequences = max(sharing, default=0), len(sharing), sum(sharing)
         self._params = p
 
 

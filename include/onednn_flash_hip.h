@@ -376,9 +376,13 @@ typedef struct ofh_prefix_groups {
      * sequence has them in. Taken down to whole pages; 0 shares nothing. (Numbers
      * that differ within a group leave its rows undefined, inside their memory.) */
     const int32_t* shared_tokens;
-    /* The least and the most of them, as the host knows them: how the work is
+    /* The least and the most of them, and the sequences of the largest group that
+     * shares any (0: an average group's), as the host knows them: how the work is
      * divided goes by these, the result does not. */
-    size_t least_shared, most_shared;
+    size_t least_shared, most_shared, most_sequences;
+    /* At most so many groups share tokens, with so many sequences together (0: all
+     * groups, the whole batch): rows of groups past these are undefined. */
+    size_t sharing_groups, sharing_sequences;
 } ofh_prefix_groups;
 
 void ofh_prefix_groups_init(ofh_prefix_groups* g);

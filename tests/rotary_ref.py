@@ -3,10 +3,11 @@ allows, from the arithmetic alone.
 
 With u = 2^-24 (fp32): the angle in turns is off by 2 2^-53 of itself (two
 roundings in 64 bits); brought within half a turn and doubled, it is rounded to
-fp32, off by 2^-25, which is pi 2^-25 < 1.6 u radians. Sine and cosine are right
-to 2 ulp (2 u), their product with the magnitude to u, the products with x and y
-and their sum to u each: with (|x| + |y|) m in front,
-    (1.6 + 2 + 1 + 1 + 1) u + the 64-bit angle's own error.
+fp32, off by 2^-25, which is d = pi 2^-25 < 1.6 u radians; put back to first order
+with one rounding, d^2 is left, nothing here, and that rounding, u. Sine and cosine
+are right to 2 ulp (2 u), their product with the magnitude to u, the products with
+x and y and their sum to u each: with (|x| + |y|) m in front,
+    (1 + 2 + 1 + 1 + 1) u + the 64-bit angle's own error.
 The result is rounded to its type (half a step)."""
 
 from __future__ import annotations
@@ -30,7 +31,7 @@ def rotate(x, position, frequencies, *, interleaved=False, magnitude=1.0, transp
     out, bound = x.copy(), np.zeros(x.shape)
     p, q = x[..., a], x[..., b]
     out[..., a], out[..., b] = p * c - q * s, q * c + p * s
-    e = (6.6 * 2.0 ** -24 + 4.0 * 2.0 ** -53 * np.abs(angle)) * abs(magnitude) * (np.abs(p) + np.abs(q))
+    e = (6.0 * 2.0 ** -24 + 4.0 * 2.0 ** -53 * np.abs(angle)) * abs(magnitude) * (np.abs(p) + np.abs(q))
     half = 2.0 ** -25 if dtype == "f16" else 2.0 ** -134 if dtype == "bf16" else 2.0 ** -150  # subnormals
     bound[..., a] = e + HALF[dtype] * (np.abs(out[..., a]) + e) + half
     bound[..., b] = e + HALF[dtype] * (np.abs(out[..., b]) + e) + half

@@ -148,6 +148,21 @@ def test_prefix_scores(ofh, dt):
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("size", [16, 32, 64, 256])
+def test_prefix_page_sizes(ofh, dt, D, size):
+    """Pages within, of and past the keys of a step; pools with strides; a last step that
+    is not full."""
+    shared = max(size, 1200 // size * size)
+    lengths = [shared + 1 + 11 * b for b in range(21)]
+    k, v, table = make(D, dt, [(21, shared)], lengths, 4, D, D, size)
+    wide = torch.zeros((k.shape[0], size, 4, D + 8), dtype=k.dtype)[..., :D].transpose(1, 2)  # token-major pages
+    wide.copy_(k)
+    check(ofh, dt, [(21, shared)], lengths, 16, 4, 1, D, pools=(wide, v, table), size=size, seed=size)
+    check(ofh, dt, [(21, shared)], lengths, 16, 4, 1, D, pools=(k, v, table), size=size, seed=size, softcap=20.0, slopes=True)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
 def test_prefix_many_rows(ofh, dt, D):
     """Several tiles of rows, several parts of keys, tiles that end inside a sequence."""
     rng = np.random.default_rng(D)
@@ -165,6 +180,32 @@ def test_prefix_many_groups(ofh, dt):
     shared = [t for n, t in groups for _ in range(n)]
     check(ofh, dt, groups, [s + 1 + b % 20 for b, s in enumerate(shared)], 4, 2, 1, 64, rows=200)
     check(ofh, dt, groups, [s + 2 + b % 40 for b, s in enumerate(shared)], 16, 1, 2, 128, rows=200, seed=1)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_prefix_beside_single_sequences(ofh, dt):
+    """A large group and small ones among sequences that share nothing."""
+    groups = [(1, 0)] * 20 + [(40, 512)] + [(1, 0)] * 9 + [(2, 1024)] + [(3, 0)]
+    shared = [t for n, t in groups for _ in range(n)]
+    check(ofh, dt, groups, [s + 1 + 5 * (b % 13) for b, s in enumerate(shared)], 8, 2, 1, 128, rows=150)
+    check(ofh, dt, groups, [s + 2 + 5 * (b % 13) for b, s in enumerate(shared)], 4, 4, 2, 64, rows=150, seed=1)
+    check(ofh, dt, [(1, 0)] * 70, [1 + 5 * b for b in range(70)], 4, 2, 1, 64, rows=100, seed=2)  # nothing is shared
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [3, 12, 40])
+def test_prefix_workspace_contents(ofh, dt, n):
+    """What the workspace held before does not matter: NaN in all of it."""
+    F = ofh
+    groups = [(n, 400), (2, 0)]
+    lengths = [3 if b % 5 == 4 else 401 + 30 * b for b in range(n)] + [50, 0]
+    k, v, table = make(4, dt, groups, [max(x, 401) for x in lengths], 2, 64, 64, 16)
+    q = randn(5, (n + 2, 8, 1, 64), dt).cuda()
+    for options in (dict(), dict(window=100, sink_tokens=20), dict(softcap=10.0)):
+        a = F.SharedPrefixAttention(k.cuda(), v.cuda(), torch.from_numpy(table).cuda(), i32(lengths), groups=groups, heads=8,
+                                    **options)
+        outs = [a(q, workspace=torch.full((a.workspace_bytes,), x, dtype=torch.uint8, device="cuda")) for x in (0, 255, 127)]
+        assert all(torch.equal(o, outs[0]) for o in outs) and torch.isfinite(outs[0]).all()
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])

@@ -320,6 +320,41 @@ def test_selected_hidden_values(ofh, dt, bad):
     assert torch.equal(run(), clean)
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_select_workspace_contents(ofh, dt):
+    """What the workspaces held before does not matter."""
+    F = ofh
+    lengths = [900, 0, 16, 500, 3000]
+    table, total = make_table(9, lengths, 16)
+    k, v, q = randn(0, (total, 2, 16, 64), dt).cuda(), randn(1, (total, 2, 16, 64), dt).cuda(), randn(2, (5, 8, 2, 64), dt).cuda()
+    bounds = torch.zeros((total, 2, 2, 64), dtype=TYPES[dt], device="cuda")
+    F.page_bounds(k, bounds, i32(table), i32(lengths))
+    a = F.SelectedAttention(k, v, bounds, i32(table), i32(lengths), heads=8, pages=70, query_tokens=2)
+    assert a.workspace_bytes > 0 and a.select_workspace_bytes > 0
+    fill = lambda n, x: torch.full((n,), x, dtype=torch.uint8, device="cuda")
+    lists = [a.select(q, workspace=fill(a.select_workspace_bytes, x)) for x in (0, 255, 127)]
+    assert all(torch.equal(x, lists[0]) for x in lists)
+    outs = [a(q, selected=lists[0], workspace=fill(a.workspace_bytes, x)) for x in (0, 255, 127)]
+    assert all(torch.equal(x, outs[0]) for x in outs) and torch.isfinite(outs[0]).all()
+
+
+def test_selected_long_lists(ofh):
+    """Lists longer than the 64 entries that are looked up at once, with gaps."""
+    F = ofh
+    lengths, size = [16 * 400 - 3, 16 * 250], 16
+    table, total = make_table(5, lengths, size)
+    k, v, q = randn(0, (total, 2, size, 64), "bf16"), randn(1, (total, 2, size, 64), "bf16"), randn(2, (2, 4, 1, 64), "bf16")
+    bounds = torch.zeros((total, 2, 2, 64), dtype=torch.bfloat16, device="cuda")
+    lists = np.full((2, 2, 1, 200), -1, np.int32)
+    for b in range(2):
+        for h in range(2):
+            pick = np.sort(np.random.default_rng(2 * b + h).permutation(-(-lengths[b] // size))[:200 - 30 * h])
+            lists[b, h, 0, :pick.size] = pick
+    for splits in (0, 1, 5):
+        a = F.SelectedAttention(k.cuda(), v.cuda(), bounds, i32(table), i32(lengths), heads=4, pages=200, max_key_splits=splits)
+        check_rows(f"long lists {splits}", a(q.cuda(), selected=i32(lists)), q, k, v, table, lengths, lists, size, "bf16")
+
+
 def test_select_refusals(ofh):
     F = ofh
     k = torch.zeros((9, 2, 16, 64), dtype=torch.bfloat16, device="cuda")

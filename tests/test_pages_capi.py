@@ -58,6 +58,9 @@ def test_paged_refusals(ofh, fields, code, text):
     (dict(groups=3), 1, "groups must be 1 to batch"),
     (dict(least_shared=48), 1, "in this order"),
     (dict(most_shared=96), 1, "within the table's tokens"),
+    (dict(sharing_groups=2), 1, "within the batch's"),
+    (dict(sharing_sequences=3), 1, "within the batch's"),
+    (dict(most_sequences=3), 1, "within the batch's"),
 ])
 def test_group_refusals(ofh, fields, code, text):
     L, n = ofh.lib(), ctypes.c_size_t()
