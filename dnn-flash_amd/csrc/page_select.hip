@@ -8,6 +8,7 @@
 // formed in 64 bits and rounded to fp32: its order then decides no rank.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "flash_wave32.h"
 #include "serving_kernels.h"
@@ -34,11 +35,6 @@ struct Words {
         for (int i = 0; i < W; ++i) v[i] = (T)f[i];
         return __builtin_bit_cast(u32x4, v);
     }
-};
-
-template <int N>
-struct Number {
-    static constexpr int value = N;
 };
 
 // A NaN stays.
@@ -95,8 +91,8 @@ __global__ __launch_bounds__(kSelectThreads) void page_bounds_kernel(PageBoundsA
             }
         }
     };
-    if (rows > 4 * groups) read(Number<8>{});
-    else read(Number<4>{});
+    if (rows > 4 * groups) read(std::integral_constant<int, 8>{});
+    else read(std::integral_constant<int, 4>{});
     for (int d = lanes; d < 64; d *= 2)
 #pragma unroll
         for (int j = 0; j < W; ++j) {

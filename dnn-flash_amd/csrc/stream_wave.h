@@ -5,6 +5,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "flash_wave32.h"
 #include "serving_kernels.h"
@@ -786,8 +787,10 @@ __global__ __launch_bounds__(kStreamThreads) void stream_join_kernel(StreamArgs 
     constexpr int G = 4;
     const int lane = threadIdx.x & 63, grp = lane >> 3;
     const int chunks = a.Dv / 4, blocks = (chunks + 7) / 8, rows = a.T * a.G;
-    const int64_t item = (int64_t)blockIdx.x * (kStreamThreads / 64) + uniform(threadIdx.x >> 6);
-    const int64_t at = item / blocks;  // row of all heads
+    // (below 2^26 by the launch's limit; the older two keep their code)
+    using Item = typename std::conditional<SRC == kTail || SRC == kSelected, unsigned, int64_t>::type;
+    const Item item = (Item)blockIdx.x * (kStreamThreads / 64) + uniform(threadIdx.x >> 6);
+    const Item at = item / blocks;  // row of all heads
     const int bh = (int)(at / rows), row = (int)(at - (int64_t)bh * rows);
     if (bh >= a.B * a.Hkv) return;
     const int c = 8 * (int)(item - at * blocks) + (lane & 7), cc = min(c, chunks - 1);
@@ -795,27 +798,41 @@ __global__ __launch_bounds__(kStreamThreads) void stream_join_kernel(StreamArgs 
     const int64_t first = ((int64_t)bh * a.row_tiles + rt) * a.splits * tile_rows + row - rt * tile_rows;
     float m = kNegInf, l = 0.0f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (SRC == kTail) {
+    if constexpr (SRC == kTail || SRC == kSelected) {
+        // one list of parts, whose loads do not wait for each other or for the group's keys
+        const int before = SRC == kTail ? a.prefix_splits : 0;
         const int64_t total = (int64_t)a.B * a.Hkv * rows;
-        const int parts = stream_shared(a, bh / a.Hkv) > 0 ? a.prefix_splits : 0;
-        for (int s = grp; s < parts; s += 8 * G) {
-            float ms[G], ls[G];
-            f32x4 os[G];
+        const int n = before + a.splits;
+        const bool shares = SRC == kTail && stream_shared(a, bh / a.Hkv) > 0;
+        auto take = [&](int s0, auto count) {
+            constexpr int C = decltype(count)::value;
+            typedef float f32x2 __attribute__((ext_vector_type(2)));
+            f32x2 ml[C];
+            f32x4 os[C];
 #pragma unroll
-            for (int j = 0; j < G; ++j) {
-                const int64_t p = (int64_t)(s + 8 * j < parts ? s + 8 * j : s) * total + at;
-                ms[j] = a.prefix_ml[2 * p];
-                ls[j] = a.prefix_ml[2 * p + 1];
-                os[j] = *(const f32x4*)(a.prefix_o + p * a.Dv + 4 * cc);
+            for (int j = 0; j < C; ++j) {
+                const int s = min(s0 + 8 * j + grp, n - 1), own = s - before;
+                const int64_t p = own < 0 ? s * total + at : first + (int64_t)own * tile_rows;
+                ml[j] = *(const f32x2*)((own < 0 ? a.prefix_ml : a.part_ml) + 2 * p);
+                os[j] = *(const f32x4*)((own < 0 ? a.prefix_o : a.part_o) + p * a.Dv + 4 * cc);
             }
 #pragma unroll
-            for (int j = 0; j < G; ++j) {
-                if (s + 8 * j >= parts) ms[j] = kNegInf;
-                const bool none = ms[j] == kNegInf && !(ls[j] != ls[j]);
-                lse_fold(m, l, acc, ms[j], none ? 0.0f : ls[j], none ? f32x4{0.f, 0.f, 0.f, 0.f} : os[j]);
+            for (int j = 0; j < C; ++j) {
+                const int s = s0 + 8 * j + grp;
+                const bool skip = s >= n || (s < before && !shares);
+                const float mj = skip ? kNegInf : ml[j][0];
+                const bool none = skip || (mj == kNegInf && !(ml[j][1] != ml[j][1]));
+                lse_fold(m, l, acc, mj, none ? 0.0f : ml[j][1], none ? f32x4{0.f, 0.f, 0.f, 0.f} : os[j]);
             }
+        };
+        for (int s0 = 0; s0 < n; s0 += 32) {
+            if (n - s0 <= 8) take(s0, std::integral_constant<int, 1>{});
+            else if (n - s0 <= 16) take(s0, std::integral_constant<int, 2>{});
+            else if (n - s0 <= 24) take(s0, std::integral_constant<int, 3>{});
+            else take(s0, std::integral_constant<int, 4>{});
         }
     }
+    if constexpr (SRC != kTail && SRC != kSelected)
     for (int s = grp; s < a.splits; s += 8 * G) {
         float ms[G], ls[G];
         f32x4 os[G];
