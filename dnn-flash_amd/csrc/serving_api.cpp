@@ -449,9 +449,13 @@ PrefixPlan plan_prefix(const ofh::StreamArgs& a, int dtype, const ofh_prefix_gro
     // (a wavefront of the streaming kernel takes a step, a workgroup of the other)
     plan.min_steps = plan.kernel.key_splits == 0 ? ofh::kStreamThreads / 64 : 2;
     plan.tiles = (int)((sequences * a.T * a.G + groups * (rows - 1)) / rows);
-    const int64_t units = (int64_t)a.Hkv * plan.tiles, steps = ((int64_t)g->most_shared + step - 1) / step;
-    const int64_t n = std::min<int64_t>({(plan.kernel.workgroups + units - 1) / units, steps / plan.min_steps,
-                                         max_key_splits > 0 ? max_key_splits : 128});
+    const int64_t steps = ((int64_t)g->most_shared + step - 1) / step;
+    // (groups of a tile each at most have no more tiles than groups)
+    const bool one_each = largest * a.T * a.G <= rows;
+    const int64_t units = (int64_t)a.Hkv * (one_each ? std::min<int64_t>(plan.tiles, groups) : plan.tiles);
+    const int64_t parts =
+        ofh::prefix_parts(plan.kernel, units, plan.tail.units, plan.tail.units * plan.tail.splits);
+    const int64_t n = std::min<int64_t>({parts, steps / plan.min_steps, max_key_splits > 0 ? max_key_splits : 128});
     plan.splits = (int)std::max<int64_t>(1, n);
     const size_t tail_rows = (size_t)plan.tail.units * plan.tail.splits * plan.tail.tile_rows;
     const size_t prefix_rows = (size_t)a.B * a.Hkv * a.T * a.G * plan.splits;

@@ -90,12 +90,15 @@ hipError_t launch_stream(const StreamArgs& a, int dtype, hipStream_t s);
 // Attention over groups of sequences that share pages, and over selected pages.
 // The prefix writes its partial rows (prefix_*); the tail's launch reads the rest
 // and joins both.
-// How the shared keys are read: rows of a tile, keys of a step, workgroups to divide
-// them over.
+// How the shared keys are read: rows of a tile, keys of a step, workgroups that a CU
+// runs at once.
 struct PrefixKernel {
     int rows, step_keys, key_splits;  // key_splits: of prefix_fwd.hip's kernel, 0: the streaming kernel
-    int workgroups;
+    int per_cu;
 };
+// Parts to divide the shared keys of `units` tiles and heads into, beside `own` tiles
+// and heads of the sequences' own keys in `own_parts` workgroups.
+int64_t prefix_parts(const PrefixKernel& k, int64_t units, int64_t own, int64_t own_parts);
 PrefixKernel prefix_kernel(const StreamArgs& a, int dtype, int rows);  // of the largest group
 __host__ __device__ inline int64_t prefix_grid(const StreamArgs& a) {  // (filled up to eights)
     return ((int64_t)a.Hkv * a.prefix_splits + 7) / 8 * 8 * a.prefix_tiles;

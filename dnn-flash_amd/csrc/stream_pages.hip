@@ -101,21 +101,37 @@ hipError_t launch(const StreamArgs& a, int dtype, int rows, int prefix_rows, hip
 
 // Groups of different sizes have one kernel: the largest one's.
 //
-// Through LDS (16 bits, more than 32 rows): a workgroup per CU, whose other place a
-// sequence's own keys have (us, bf16 H32/8 D128, 16384 shared keys, 33-1024 of each
-// sequence's own, 256 / 512 workgroups: 64 sequences 66 / 76, 32 49 / 58, 16 31 / 40).
-// Streaming: as many as the registers let run at once, the shared part being most
-// of the work (f32 D64 B15 H8, 4000 shared, 3 tokens, two per CU: 256 27.5, 512 25.2;
-// bf16 D128 B8 H32/8 16384 shared, 32 rows, one per CU: 256 32.7, 512 40.8).
+// Through LDS (16 bits, more than 32 rows) or streaming.
 PrefixKernel prefix_kernel(const StreamArgs& a, int dtype, int rows) {
     const int dk = stream_kernel_dim(a.D, a.Dv);
     if (dtype != DT_F32 && rows > 32) {
         const int key_splits = dk <= 128 && rows <= window_rows(2) ? 2 : 1;
-        return PrefixKernel{window_rows(key_splits), dk == 256 ? 32 : 64, key_splits, kComputeUnits};
+        return PrefixKernel{window_rows(key_splits), dk == 256 ? 32 : 64, key_splits, 1};
     }
     const int tile = stream_tile_rows(dtype, dk, rows);
     const bool one = dk == 256 || (dk == 128 && tile == 32);
-    return PrefixKernel{tile, stream_step_keys(dtype, dk), 0, (one ? 1 : 2) * kComputeUnits};
+    return PrefixKernel{tile, stream_step_keys(dtype, dk), 0, one ? 1 : 2};
+}
+
+// Through LDS: a workgroup per CU, whose other place the sequences' own keys have (us,
+// bf16 H32/8 D128, 16384 shared keys, 33-1024 of each sequence's own, 256 / 512
+// workgroups: 64 sequences 66 / 76, 32 49 / 58, 16 31 / 40).
+//
+// Streaming: shared and own together no more than run at once, since what waits for a
+// place then costs a whole pass (us, 512 / 624 workgroups at two per CU: f32 D64, 3 groups
+// of 5 sequences with 3 tokens, H8, 4000 shared 24.9 / 29.9; f16 D64, 4 groups of 4,
+// H16/8, 8192 shared 23.0 / 28.2; 256 / 324 at one: f16 D256, one group of 5, H16/4,
+// 6000 shared 21.5 / 29.5). A second one of a CU only up to 16 parts (16 against 6 of those
+// f32 groups 24.9 / 26.9, 12 against 4 of the f16 ones 23.0 / 29.3; but 24 against 56 of
+// one group of 8, f32 D64 H8, 16000 shared 24.7 / 33.9), where the parts of an own
+// tile, mostly short, count as one (f32 D128, one group of 4, H32/8, 16000 shared, 28
+// parts 37.9, 16 44.8).
+int64_t prefix_parts(const PrefixKernel& k, int64_t units, int64_t own, int64_t own_parts) {
+    constexpr int64_t kCus = kComputeUnits, kFew = 16;
+    if (k.key_splits > 0) return (kCus + units - 1) / units;
+    const int64_t at_once = std::max(k.per_cu * kCus - own_parts, kCus / 2) / units;
+    const int64_t first = (kCus - own) / units;
+    return std::min(at_once, std::max(first, kFew));
 }
 hipError_t launch_stream_shared(const StreamArgs& a, int dtype, int prefix_rows, hipStream_t s) {
     return launch<kLaunchShared>(a, dtype, a.T * a.G, prefix_rows, s);
