@@ -46,7 +46,10 @@ __device__ __forceinline__ int row_lanes(int words) { return words <= 1 ? 1 : 1 
 
 // A wavefront per touched page and key-value head: its lanes take the words of a
 // row and, beside each other, several rows, four or eight of which are in flight per lane.
-// Bound by reading the page's keys once; a decode step's few pages by the launch.
+// Bound by reading the page's keys once (us: fp16, 8 prompts of 1500 new tokens up to 2048
+// long, H8 D128, pages of 32, 26 MB, 8.7, 3.0 TB/s; as many wavefronts as pages and
+// heads, 3072, are one round of the GPU, so a wavefront's own loads in flight count);
+// a decode step's few pages by the launch (64 sequences 4.2).
 template <typename T>
 __global__ __launch_bounds__(kSelectThreads) void page_bounds_kernel(PageBoundsArgs a) {
     using X = Words<T>;
@@ -245,7 +248,8 @@ constexpr int kPickThreads = 512, kPickWaves = kPickThreads / 64;
 // candidates between the first and the recent ones is found from counts of the
 // scores' bits; then each thread takes a stretch of the candidates, counts what is
 // above and what is equal to it, and after a sum over the threads before writes its
-// share: ascending, ties to the lower page.
+// share: ascending, ties to the lower page. Bound by its barriers, 7-7.5 us with the
+// launch: eight bits a round take four rounds at most.
 __global__ __launch_bounds__(kPickThreads) void page_select_kernel(SelectArgs a) {
     __shared__ uint32_t kept[kSelectKept];
     __shared__ int count[256];

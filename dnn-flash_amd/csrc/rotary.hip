@@ -13,6 +13,10 @@
 // with few tokens, each of four) takes a token: its place and position are scalars,
 // its sines and cosines are computed once for all heads and kept in LDS, and the
 // first rows are on their way meanwhile. A lane keeps its columns for all rows.
+// Measured (us): rows by themselves, bf16 B4 H32 T2048 D128, 134 MB, 26.2, which is 5.1
+// TB/s, a copy's rate (kernel 23.4); into the cache, fp16 B8 H16/8 T2048 of which 700-2048
+// count, 207 MB, 48.8 (kernel 43.8, 4.7 TB/s); one token of 64 sequences, bf16 H32/8 D128,
+// 7.9 (kernel 4.9): the launch, then length, place in the table, page and store in turn.
 
 #include "serving_kernels.h"
 
@@ -276,7 +280,8 @@ bool append_in_words(const CacheAppendArgs& a, int elem) {
     return turns_in_words(a.r, a.D, elem) && a.Dv % (16 / elem) == 0 && aligned(all, strides, elem);
 }
 
-// A wavefront per token once that fills the GPU, a workgroup before.
+// A wavefront per token once that fills the GPU, a workgroup before (us, a workgroup /
+// a wavefront: the 8192 tokens of 32 heads above 29.3 / 26.2, the prompts 62.7 / 48.8).
 bool many_tokens(int64_t tokens) { return tokens >= 16 * (int64_t)kComputeUnits; }
 int64_t rotary_grid(int64_t tokens) { return many_tokens(tokens) ? (tokens + kRotaryWaves - 1) / kRotaryWaves : tokens; }
 

@@ -1,5 +1,6 @@
-// C ABI of the serving operators (include/onednn_flash_hip.h): windowed and
-// paged attention, writing and copying of cache pages. Argument checks, layout
+// C ABI of the serving operators (include/onednn_flash_hip.h): windowed and paged
+// attention, also over shared prefixes and selected pages, bounds and selection of
+// pages, writing and copying of cache pages. Argument checks, layout
 // resolution, the split of a call's keys over workgroups, scratch.
 
 #include "onednn_flash_hip.h"
@@ -511,10 +512,11 @@ int selected_args(const ofh_paged_params* p, size_t pages, bool check_ptrs, cons
 }
 
 // Tokens take equally many keys, so a workgroup per CU is enough, and parts of eight
-// steps, four at kernel dim 256 (us, parts per tile: bf16 B32 H32/8 D128, 64 pages of 32, 256 tiles 1 52, 2 59; B8,
-// 64 tiles, 2 22.8, 4 20.2; f16 B1, 64 pages of 64, 8 tiles, 8 16.3, 16 13.8, 32 14.7; bf16
-// D256, 64 pages of 32, 8 tiles, 8 18.7, 16 16.3); with less than 32 steps the join costs what they save (f32 B4 H8 3 tokens D64, 20 steps,
-// 96 tiles 1 15.2, 2 16.4, 3 18.7).
+// steps, four at kernel dim 256 (us, parts per tile: bf16 B32 H32/8 D128, 64 pages of
+// 32, 256 tiles 1 52, 2 59; B8, 64 tiles, 2 22.8, 4 20.2; f16 B1, 64 pages of 64, 8 tiles,
+// 8 16.3, 16 13.8, 32 14.7; bf16 D256, 64 pages of 32, 8 tiles, 8 18.7, 16 16.3); with less
+// than 32 steps the join costs what they save (f32 B4 H8 3 tokens D64, 20 steps, 96
+// tiles 1 15.2, 2 16.4, 3 18.7).
 Split plan_selected(const ofh::StreamArgs& a, int dtype, int max_key_splits) {
     ofh::StreamArgs seen = a;
     seen.capacity = (int)std::min<int64_t>(a.capacity, (int64_t)a.num_selected << a.page_shift);
@@ -523,7 +525,8 @@ Split plan_selected(const ofh::StreamArgs& a, int dtype, int max_key_splits) {
     const int64_t steps = ((int64_t)seen.capacity + step - 1) / step;
     if (steps < 32) return s;
     const int64_t least = dk == 256 ? 4 : 8;
-    const int64_t n = std::min<int64_t>({ofh::kComputeUnits / s.units, steps / least, max_key_splits > 0 ? max_key_splits : 128});
+    const int64_t n =
+        std::min<int64_t>({ofh::kComputeUnits / s.units, steps / least, max_key_splits > 0 ? max_key_splits : 128});
     if (n <= 1) return s;
     s.splits = (int)n;
     const size_t rows = (size_t)s.units * s.splits * s.tile_rows;
