@@ -377,22 +377,33 @@ __global__ __launch_bounds__(kPickThreads) void page_select_kernel(SelectArgs a)
     }
 }
 
-// Pages of a workgroup: enough workgroups to fill the GPU a few times.
-int score_pages(const SelectArgs& a) {
+// Lanes that share a page's bounds of `words` words.
+int score_lanes(int words) {
+    int lanes = 1;
+    while (lanes * kScoreWords < words) lanes *= 2;
+    return lanes;
+}
+
+// Pages of a workgroup: one round of its lanes, more where the workgroups then still
+// fill the GPU a few times (us of a selection, 64 pages / one round: f32 D256 B2 H64/4, 512
+// pages 35.2 / 16.3; f16 D64 B32 H32/8, 1875 pages 34.2 / 30.3).
+int score_pages(const SelectArgs& a, int lanes) {
     const int64_t rows = (int64_t)a.B * a.Hkv * a.T, want = 16 * (int64_t)kComputeUnits;
-    int per = 64;
+    int per = kSelectWaves * (64 / lanes);
     while (per < 1024 && rows * ((a.max_pages + 2 * per - 1) / (2 * per)) >= want) per *= 2;
     return per;
 }
-int score_chunks(const SelectArgs& a) { return (a.max_pages + score_pages(a) - 1) / score_pages(a); }
+int score_chunks(const SelectArgs& a, int lanes) {
+    const int per = score_pages(a, lanes);
+    return (a.max_pages + per - 1) / per;
+}
 
 template <typename T>
 hipError_t launch_score(const SelectArgs& a, hipStream_t s) {
-    const int words = a.D / Words<T>::W, heads = std::min(a.G, kScoreQuery / a.D), chunks = score_chunks(a);
-    int lanes = 1;
-    while (lanes * kScoreWords < words) lanes *= 2;
+    const int words = a.D / Words<T>::W, heads = std::min(a.G, kScoreQuery / a.D), lanes = score_lanes(words);
+    const int chunks = score_chunks(a, lanes);
     hipLaunchKernelGGL((page_score_kernel<T>), dim3((unsigned)((int64_t)a.B * a.Hkv * a.T * chunks)), dim3(kSelectThreads),
-                       heads * (a.D * (int)sizeof(double) + 16 * words), s, a, score_pages(a), lanes, heads);
+                       heads * (a.D * (int)sizeof(double) + 16 * words), s, a, score_pages(a, lanes), lanes, heads);
     return hipGetLastError();
 }
 
@@ -415,9 +426,10 @@ hipError_t launch_page_bounds(const PageBoundsArgs& a, int dtype, hipStream_t s)
     return hipGetLastError();
 }
 
-bool page_select_fits(const SelectArgs& a) {
+bool page_select_fits(const SelectArgs& a, int dtype) {
     const int64_t rows = (int64_t)a.B * a.Hkv * a.T;
-    return grid_fits(rows * score_chunks(a), kSelectThreads) && grid_fits(rows, kPickThreads);
+    const int lanes = score_lanes(a.D * (dtype == DT_F32 ? 4 : 2) / 16);
+    return grid_fits(rows * score_chunks(a, lanes), kSelectThreads) && grid_fits(rows, kPickThreads);
 }
 
 hipError_t launch_page_select(const SelectArgs& a, int dtype, hipStream_t s) {

@@ -708,7 +708,7 @@ int ofh_select_pages(const ofh_select_params* p, const void* q, const void* boun
     return guarded([&]() -> int {
         ofh::SelectArgs a;
         if (int rc = select_args(p, true, q, bounds, selected, a)) return rc;
-        if (!ofh::page_select_fits(a)) return unsupported("selection exceeds the launch range");
+        if (!ofh::page_select_fits(a, p->dtype)) return unsupported("selection exceeds the launch range");
         ofh::ScratchLease lease;
         if (int rc = take_workspace(select_bytes(a), workspace, workspace_bytes, static_cast<hipStream_t>(stream), lease))
             return rc;

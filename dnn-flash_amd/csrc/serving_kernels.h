@@ -147,7 +147,7 @@ struct SelectArgs {
     int pages, first_pages, recent_pages;
     int negative;  // scores of -q
 };
-bool page_select_fits(const SelectArgs& a);
+bool page_select_fits(const SelectArgs& a, int dtype);
 hipError_t launch_page_select(const SelectArgs& a, int dtype, hipStream_t s);
 
 // Prompts on the matrix cores with K and V staged through LDS (window_fwd.hip).
