@@ -200,7 +200,7 @@ __device__ __forceinline__ PrefixRow prefix_row(const StreamArgs& a, const Prefi
 __device__ __forceinline__ int prefix_limits(const StreamArgs& a, const PrefixTile& p, const PrefixRow& x, int& hi, int& lo) {
     const int pos = max(0, min(a.lengths[x.b], a.capacity)) - a.T + x.t;
     hi = max(0, min(p.shared, pos + 1));
-    lo = a.window > 0 ? pos + 1 - a.window : -0x7fffffff;
+    lo = a.window > 0 ? max(pos, -1) + 1 - a.window : -0x7fffffff;  // (before -1 none is seen: hi)
     return pos;
 }
 // Row of all heads, in which the prefix's partial rows are kept.
@@ -387,11 +387,26 @@ struct StreamWave {
         for (int i = 0; i < RT; ++i) {
             const int row = min(rt * ROWS + 16 * i + n, a.T * a.G - 1);
             const int t = row / a.G, h = hk * a.G + row - t * a.G;
+            const T* qrow = (const T*)a.q + b * a.q_sb + h * a.q_sh + t * a.q_st;
             if constexpr (SRC == kSelected) {
                 const int seq = b / a.tokens;
                 load_q(i, (const T*)a.q + seq * a.q_sb + h * a.q_sh + (b - seq * a.tokens) * a.q_st);
+            } else if constexpr (PAGED) {
+                load_q(i, qrow);
             } else {
-                load_q(i, (const T*)a.q + b * a.q_sb + h * a.q_sh + t * a.q_st);
+                // (load_q written out: the call moves the registers of the kernels that
+                // spill; f32 B2 H16/4 N1500 D256 710 us, 755 with it. Written out for
+                // pages too, those spill 95 times instead of 71.)
+#pragma unroll
+                for (int c = 0; c < S::KF; ++c) {
+                    const int d = S::KW * (4 * c + g);
+                    q[i][c] = u32x4{0u, 0u, 0u, 0u};
+                    if (d < a.D) q[i][c] = *(const u32x4*)(qrow + d);
+                }
+#pragma unroll
+                for (int j = 0; j < S::NO; ++j) o[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                m[i] = kNegInf;
+                l[i] = 0.0f;
             }
             tok[i] = t;
             limits(t, hi[i], lo[i]);
