@@ -47,8 +47,8 @@ __device__ __forceinline__ int row_lanes(int words) { return words <= 1 ? 1 : 1 
 // A wavefront per touched page and key-value head: its lanes take the words of a
 // row and, beside each other, several rows, four or eight of which are in flight per lane.
 // Bound by reading the page's keys once (us: fp16, 8 prompts of 1500 new tokens up to 2048
-// long, H8 D128, pages of 32, 26 MB, 8.7, 3.0 TB/s; as many wavefronts as pages and
-// heads, 3072, are one round of the GPU, so a wavefront's own loads in flight count);
+// long, H8 D128, pages of 32, 26 MB, 8.7, 3.0 TB/s; a wavefront per page and
+// head is 12 per CU, one round of the GPU, so a wavefront's own loads in flight count);
 // a decode step's few pages by the launch (64 sequences 4.2).
 template <typename T>
 __global__ __launch_bounds__(kSelectThreads) void page_bounds_kernel(PageBoundsArgs a) {
