@@ -192,6 +192,23 @@ def test_prefix_beside_single_sequences(ofh, dt):
     check(ofh, dt, [(1, 0)] * 70, [1 + 5 * b for b in range(70)], 4, 2, 1, 64, rows=100, seed=2)  # nothing is shared
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_prefix_parts(ofh, dt, D):
+    """The shared keys in as many parts as the call's own tiles leave room for: none
+    (own tiles for every place), few, and the most."""
+    check(ofh, dt, [(72, 512)], [513 + 7 * i for i in range(72)], 8, 8, 1, D, rows=32, seed=D)
+    check(ofh, dt, [(6, 512), (5, 256)], [600 + 3 * i for i in range(11)], 8, 4, 2, D, rows=32, seed=D + 1)
+    check(ofh, dt, [(3, 4096)], [4097, 4300, 4096], 2, 1, 1, D, rows=6, seed=D + 2)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_prefix_widest_window(ofh, dt):
+    """Positions before the sequence, and a window wider than any of them."""
+    for n in (1, 5):
+        check(ofh, dt, [(3 * n, 64)], [0, 2, 80] * n, 4, 2, 5, 64, window=(1 << 30) - 1, sink_tokens=1, rows=60, seed=n)
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("n", [3, 12, 40])
 def test_prefix_workspace_contents(ofh, dt, n):
