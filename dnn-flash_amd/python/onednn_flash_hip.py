@@ -13,6 +13,7 @@ with the same keyword names and validation, on device tensors.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import operator
@@ -840,12 +841,46 @@ def _given_workspace(torch, workspace, out):
 def _new_workspace(torch, need, device, stream):
     """Scratch of one call on `stream` (a handle or a torch stream; None: the current
     one). It is freed when the call returns, so it belongs to the stream that uses it."""
-    if stream is None:
+    with _on_stream(torch, device, stream):
         return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def _on_stream(torch, device, stream):
+    """Context in which tensors are allocated on `stream` (as _new_workspace takes it)."""
+    if stream is None or device.type != "cuda":
+        return contextlib.nullcontext()
     if not isinstance(stream, torch.cuda.Stream):
         stream = torch.cuda.ExternalStream(stream, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(need, dtype=torch.uint8, device=device)
+    return torch.cuda.stream(stream)
+
+
+class _Kept:
+    """Device tensors of the library's own that kernels read, on whichever stream an
+    object is called. When nothing holds them their memory goes to the next tensor of
+    the stream that they were made on, so a call on another torch stream tells the
+    allocator, which then waits for it. (Not for a stream given by its handle, which
+    may be gone by then: such a call's object is kept until it has run.)"""
+
+    def __init__(self, torch, *tensors):
+        self._torch, self.tensors, self._index = torch, tensors, tensors[0].device.index
+        self._told = set()
+        if self._index is not None:  # (None: on the CPU)
+            self._told.add(torch._C._cuda_getCurrentRawStream(self._index))
+
+    def used(self, stream) -> None:
+        """A call on `stream` (as _launch takes it) reads the tensors."""
+        if self._index is None:
+            return
+        if stream is None:
+            if self._torch._C._cuda_getCurrentRawStream(self._index) in self._told:
+                return
+            stream = self._torch.cuda.current_stream(self._index)
+        elif not isinstance(stream, self._torch.cuda.Stream):
+            return
+        if stream.cuda_stream not in self._told:
+            for t in self.tensors:
+                t.record_stream(stream)
+            self._told.add(stream.cuda_stream)
 
 
 def _workspace_need(query, p, *more) -> int:
@@ -1073,10 +1108,10 @@ class PrefixGroups:
         for n, tokens in groups:
             starts.append(starts[-1] + n)
             shared += [tokens] * n
-        self._held = tuple(torch.tensor(x, dtype=torch.int32, device=device) for x in (starts, shared))
+        self._kept = _Kept(torch, *(torch.tensor(x, dtype=torch.int32, device=device) for x in (starts, shared)))
         p = PrefixGroupsParams()
         lib().ofh_prefix_groups_init(ctypes.addressof(p))
-        p.groups, p.starts, p.shared_tokens = len(groups), *(t.data_ptr() for t in self._held)
+        p.groups, p.starts, p.shared_tokens = len(groups), *(t.data_ptr() for t in self._kept.tensors)
         p.least_shared, p.most_shared = min(shared), max(shared)
         sharing = [n for n, tokens in groups if tokens > 0]
         p.most_sequences, p.sharing_groups, p.sharing_sequences = max(sharing, default=0), len(sharing), sum(sharing)
@@ -1099,13 +1134,17 @@ class SharedPrefixAttention(PagedAttention):
             groups = PrefixGroups(groups, page_size=p.page_size, device=self._device)
         if groups.batch != p.batch:
             raise ValueError(f"groups must have the batch's {p.batch} sequences together")
-        if groups._held[0].device != self._device:
+        if groups._kept.tensors[0].device != self._device:
             raise ValueError(f"groups must be on {self._device}")
         if any(tokens % p.page_size or tokens > p.max_pages * p.page_size for _, tokens in groups.groups):
             raise ValueError("shared tokens must be whole pages of the table's rows")
         self._groups = groups
         self._fwd, self._more = L.ofh_shared_prefix_attention_fwd, (ctypes.addressof(groups._params),)
         self._need = _workspace_need(L.ofh_shared_prefix_workspace_bytes, p, *self._more)
+
+    def _attend(self, q, more, out, workspace, stream):
+        self._groups._kept.used(stream)
+        return super()._attend(q, more, out, workspace, stream)
 
 
 def shared_prefix_attention(q, k_pages, v_pages, page_table, lengths, *, groups, out=None, out_dtype=None, workspace=None,
@@ -1115,9 +1154,11 @@ def shared_prefix_attention(q, k_pages, v_pages, page_table, lengths, *, groups,
         raise ValueError("q must be a rank-4 tensor")
     if out is not None and out_dtype is not None and out.dtype != out_dtype:
         raise ValueError("out and out_dtype disagree")
-    return SharedPrefixAttention(k_pages, v_pages, page_table, lengths, groups=groups, heads=q.shape[1],
-                                 query_tokens=q.shape[2], out_dtype=out_dtype, **options)(
-                                     q, out=out, workspace=workspace, stream=stream)
+    # (the groups of a list are freed when the call returns, as its scratch is)
+    with _on_stream(_torch(), q.device, stream):
+        attend = SharedPrefixAttention(k_pages, v_pages, page_table, lengths, groups=groups, heads=q.shape[1],
+                                       query_tokens=q.shape[2], out_dtype=out_dtype, **options)
+    return attend(q, out=out, workspace=workspace, stream=stream)
 
 
 def _check_bounds(torch, k_pages, k_bounds):
