@@ -166,7 +166,9 @@ __global__ __launch_bounds__(kSelectThreads) void page_score_kernel(SelectArgs a
     using X = Words<T>;
     constexpr int W = X::W;
     extern __shared__ __attribute__((aligned(16))) double q[];
-    u32x4* masks = (u32x4*)(q + heads_kept * a.D);
+    // rows of Q in the layout of the lanes: `slots` words, 0 past the row
+    const int slots = lanes * kScoreWords;
+    u32x4* masks = (u32x4*)(q + heads_kept * slots * W);
     const int rows = a.B * a.Hkv * a.T, chunk = blockIdx.x / rows;
     const int64_t row = blockIdx.x - (int64_t)chunk * rows;  // (b, hk, t)
     const int t = (int)(row % a.T), hk = (int)(row / a.T % a.Hkv), b = (int)(row / a.T / a.Hkv);
@@ -181,9 +183,15 @@ __global__ __launch_bounds__(kSelectThreads) void page_score_kernel(SelectArgs a
     for (int g0 = 0; g0 < a.G; g0 += heads_kept) {
         const int heads = min(heads_kept, a.G - g0);
         __syncthreads();
-        for (int n = threadIdx.x; n < heads * words; n += kSelectThreads) {
-            const int g = n / words, w = n - g * words;
+        for (int n = threadIdx.x; n < heads * slots; n += kSelectThreads) {
+            const int g = n >> __builtin_ctz(slots), w = n & (slots - 1);
             const T* at = (const T*)a.q + b * a.q_sb + (int64_t)(hk * a.G + g0 + g) * a.q_sh + t * a.q_st + w * W;
+            if (w >= words) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) q[n * W + j] = 0.0;
+                masks[n] = u32x4{0u, 0u, 0u, 0u};
+                continue;
+            }
             unsigned on[W];
 #pragma unroll
             for (int j = 0; j < W; ++j) {
@@ -210,14 +218,14 @@ __global__ __launch_bounds__(kSelectThreads) void page_score_kernel(SelectArgs a
                 hi[c] = *(const u32x4*)(at + a.b_st + word * W);
             }
 #pragma unroll
-            for (int c = 0; c < kScoreWords; ++c)  // a word past the row counts as 0
+            for (int c = 0; c < kScoreWords; ++c)  // a word past the row is 0, as Q's is
                 if (sub + lanes * c >= words) lo[c] = hi[c] = u32x4{0u, 0u, 0u, 0u};
             unsigned best = 0;
             for (int g = 0; g < heads; ++g) {
                 double sum[2] = {0.0, 0.0};
 #pragma unroll
                 for (int c = 0; c < kScoreWords; ++c) {
-                    const int word = g * words + min(sub + lanes * c, words - 1);
+                    const int word = g * slots + sub + lanes * c;
                     const u32x4 m = masks[word];
                     u32x4 bound;
 #pragma unroll
@@ -400,10 +408,10 @@ int score_chunks(const SelectArgs& a, int lanes) {
 
 template <typename T>
 hipError_t launch_score(const SelectArgs& a, hipStream_t s) {
-    const int words = a.D / Words<T>::W, heads = std::min(a.G, kScoreQuery / a.D), lanes = score_lanes(words);
-    const int chunks = score_chunks(a, lanes);
+    const int words = a.D / Words<T>::W, lanes = score_lanes(words), slots = lanes * kScoreWords;
+    const int heads = std::min(a.G, kScoreQuery / (slots * Words<T>::W)), chunks = score_chunks(a, lanes);
     hipLaunchKernelGGL((page_score_kernel<T>), dim3((unsigned)((int64_t)a.B * a.Hkv * a.T * chunks)), dim3(kSelectThreads),
-                       heads * (a.D * (int)sizeof(double) + 16 * words), s, a, score_pages(a, lanes), lanes, heads);
+                       heads * slots * (Words<T>::W * (int)sizeof(double) + 16), s, a, score_pages(a, lanes), lanes, heads);
     return hipGetLastError();
 }
 
