@@ -1447,11 +1447,10 @@ class Rotary:
         device = torch.device(device)
         if device.type != "cuda":
             raise ValueError("device must be a GPU")
-        self.head_dim, self.rotary_dim, self.interleaved = head_dim, rotary_dim, bool(interleaved)
-        self.magnitude = float(magnitude)
+        self._shape, self._interleaved, self._magnitude = (head_dim, rotary_dim), bool(interleaved), float(magnitude)
         # (its own copy: a program may go on with its tensor)
-        self.frequencies = frequencies.detach().to(device, copy=True).contiguous()
-        self._torch, self._device = torch, self.frequencies.device
+        self._frequencies = frequencies.detach().to(device, copy=True).contiguous()
+        self._torch, self._device = torch, self._frequencies.device
         p = RotaryParams()
         self._lib = lib()
         self._lib.ofh_rotary_params_init(ctypes.addressof(p))
@@ -1460,8 +1459,15 @@ class Rotary:
         self._params = bytes(p)
         self._held = None  # (layout of the last call, its parameters): calls are laid out alike
 
+    # (not to be assigned: calls, also of a CacheAppender, go by what they were when it was made)
+    head_dim = property(lambda self: self._shape[0])
+    rotary_dim = property(lambda self: self._shape[1])
+    interleaved = property(lambda self: self._interleaved)
+    magnitude = property(lambda self: self._magnitude)
+    frequencies = property(lambda self: self._frequencies, doc="float64 on the device: the tensor that calls read")
+
     def _fields(self, r: RotaryFields) -> None:
-        r.frequencies, r.rotary_dim = self.frequencies.data_ptr(), self.rotary_dim
+        r.frequencies, r.rotary_dim = self._frequencies.data_ptr(), self.rotary_dim
         r.interleaved, r.magnitude = int(self.interleaved), self.magnitude
 
     def __call__(self, x, *, offset: int = 0, positions=None, lengths=None, transpose: bool = False, out=None,
