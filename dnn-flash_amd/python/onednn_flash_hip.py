@@ -1450,6 +1450,7 @@ class Rotary:
         self._shape, self._interleaved, self._magnitude = (head_dim, rotary_dim), bool(interleaved), float(magnitude)
         # (its own copy: a program may go on with its tensor)
         self._frequencies = frequencies.detach().to(device, copy=True).contiguous()
+        self._kept = _Kept(torch, self._frequencies)
         self._torch, self._device = torch, self._frequencies.device
         p = RotaryParams()
         self._lib = lib()
@@ -1514,6 +1515,7 @@ class Rotary:
                 if _axis_strides("out", out) != _axis_strides("x", x):
                     raise ValueError("x turned in place must keep its strides")
                 p.o_strides[:] = p.x_strides[:]
+        self._kept.used(stream)
         rc = _launch(torch, dev, stream, self._lib.ofh_rotary_fwd, ctypes.addressof(p), x.data_ptr(), out.data_ptr())
         if rc != OFH_SUCCESS:
             check(rc)
@@ -1582,6 +1584,7 @@ class CacheAppender:
             out_ptr = q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out needs q")
+        self._rotary._kept.used(stream)
         rc = _launch(torch, dev, stream, self._append, p, k.data_ptr(), v.data_ptr(), q_ptr, *w._ptrs, out_ptr)
         if rc != OFH_SUCCESS:
             check(rc)

@@ -17,13 +17,13 @@ def _need_gpu():
         pytest.skip("no GPU")
 
 
-@pytest.fixture
-def busy():
-    """A side stream with work ahead of the calls, a few tens of milliseconds."""
+def busy_stream():
+    """A side stream with work ahead of the calls, 40 ms. (Copies to the device may wait
+    for it: objects are made before.)"""
+    torch.cuda.current_stream().synchronize()
     side = torch.cuda.Stream()
-    side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        torch.cuda._sleep(50_000_000)
+        torch.cuda._sleep(100_000_000)
     return side
 
 
@@ -53,12 +53,11 @@ def spy(monkeypatch, F):
 
 
 @pytest.mark.parametrize("handle", [False, True])
-def test_groups_of_one_call(ofh, monkeypatch, busy, handle):
+def test_groups_of_one_call(ofh, monkeypatch, handle):
     k, v, table, lengths = pools()
     q = torch.randn(8, 8, 1, 64, device="cuda", dtype=torch.bfloat16)
     want = ofh.shared_prefix_attention(q, k, v, table, lengths, groups=[(8, 48)])
-    torch.cuda.current_stream().synchronize()
-    ptrs = spy(monkeypatch, ofh)
+    ptrs, busy = spy(monkeypatch, ofh), busy_stream()
     out = ofh.shared_prefix_attention(q, k, v, table, lengths, groups=[(8, 48)], stream=busy.cuda_stream if handle else busy)
     assert len(ptrs) == 2 and not reused(ptrs, 64)
     busy.synchronize()
@@ -66,19 +65,52 @@ def test_groups_of_one_call(ofh, monkeypatch, busy, handle):
 
 
 @pytest.mark.parametrize("current", [False, True])
-def test_groups_of_a_dropped_object(ofh, monkeypatch, busy, current):
+def test_groups_of_a_dropped_object(ofh, monkeypatch, current):
     k, v, table, lengths = pools()
     q = torch.randn(8, 8, 1, 64, device="cuda", dtype=torch.bfloat16)
     want = ofh.shared_prefix_attention(q, k, v, table, lengths, groups=[(8, 48)])
-    torch.cuda.current_stream().synchronize()
     ptrs = spy(monkeypatch, ofh)
     attend = ofh.SharedPrefixAttention(k, v, table, lengths, groups=[(8, 48)], heads=8)
+    busy = busy_stream()
     if current:
         with torch.cuda.stream(busy):
             out = attend(q)
     else:
         out = attend(q, stream=busy)
     del attend
-    assert len(ptrs) == 2 and not busy.query() and not reused(ptrs, 64)
+    assert len(ptrs) == 2 and not reused(ptrs, 64) and not busy.query()
+    busy.synchronize()
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("current", [False, True])
+def test_frequencies_of_a_dropped_rotary(ofh, monkeypatch, current):
+    x = torch.randn(2, 4, 5, 64, device="cuda")
+    want = ofh.Rotary(64)(x, offset=9)
+    ptrs = spy(monkeypatch, ofh)
+    rotary = ofh.Rotary(64)
+    busy = busy_stream()
+    if current:
+        with torch.cuda.stream(busy):
+            out = rotary(x, offset=9)
+    else:
+        out = rotary(x, offset=9, stream=busy)
+    del rotary
+    assert len(ptrs) == 1 and not reused(ptrs, 256) and not busy.query()
+    busy.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_frequencies_of_a_dropped_appender(ofh, monkeypatch):
+    k_pages, v_pages, table, lengths = pools()
+    table = torch.arange(32, dtype=torch.int32, device="cuda").reshape(8, 4)
+    k, q = (torch.randn(8, h, 1, 64, device="cuda", dtype=torch.bfloat16) for h in (2, 8))
+    want = ofh.cache_append(k, k, k_pages, v_pages, table, lengths, ofh.Rotary(64), q=q)
+    ptrs = spy(monkeypatch, ofh)
+    append = ofh.CacheAppender(k_pages, v_pages, table, lengths, ofh.Rotary(64))
+    busy = busy_stream()
+    out = append(k, k, q, stream=busy)
+    del append
+    assert len(ptrs) == 1 and not reused(ptrs, 256) and not busy.query()
     busy.synchronize()
     assert torch.equal(out, want)
