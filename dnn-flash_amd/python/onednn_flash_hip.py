@@ -1442,7 +1442,8 @@ class Rotary:
         frequencies = torch.as_tensor(frequencies, dtype=torch.float64)
         if tuple(frequencies.shape) != (rotary_dim // 2,):
             raise ValueError("frequencies must be rotary_dim / 2 numbers")
-        if not bool(torch.isfinite(frequencies).all()):
+        on_host = frequencies.device.type == "cpu"
+        if on_host and not bool(torch.isfinite(frequencies).all()):
             raise ValueError("frequencies must be finite")
         device = torch.device(device)
         if device.type != "cuda":
@@ -1450,6 +1451,9 @@ class Rotary:
         self._shape, self._interleaved, self._magnitude = (head_dim, rotary_dim), bool(interleaved), float(magnitude)
         # (its own copy: a program may go on with its tensor)
         self._frequencies = frequencies.detach().to(device, copy=True).contiguous()
+        # (a copy from a device has ended when what was copied is looked at: calls may run on any stream)
+        if not on_host and not bool(torch.isfinite(self._frequencies).all()):
+            raise ValueError("frequencies must be finite")
         self._kept = _Kept(torch, self._frequencies)
         self._torch, self._device = torch, self._frequencies.device
         p = RotaryParams()

@@ -114,3 +114,16 @@ def test_frequencies_of_a_dropped_appender(ofh, monkeypatch):
     assert len(ptrs) == 1 and not reused(ptrs, 256) and not busy.query()
     busy.synchronize()
     assert torch.equal(out, want)
+
+
+def test_frequencies_from_a_device_are_there(ofh, monkeypatch):
+    """A Rotary made from a device tensor is ready when its constructor returns: what
+    was looked at last is its own copy, not the tensor before it was copied."""
+    seen, plain = [], torch.isfinite
+    monkeypatch.setattr(torch, "isfinite", lambda t: seen.append(t.data_ptr()) or plain(t))
+    given = torch.rand(32, dtype=torch.float64, device="cuda")
+    rotary = ofh.Rotary(64, frequencies=given)
+    assert seen == [rotary.frequencies.data_ptr()] and rotary.frequencies.data_ptr() != given.data_ptr()
+    given[3] = float("nan")
+    with pytest.raises(ValueError, match="finite"):
+        ofh.Rotary(64, frequencies=given)
