@@ -213,6 +213,7 @@ class CacheBatch:
         self.page_table = torch.tensor(rows, dtype=torch.int32, device=device)
         self.lengths = torch.tensor(lengths, dtype=torch.int32, device=device)
         self.counts = torch.tensor(list(tokens), dtype=torch.int32, device=device)
+        self._kept = F._Kept(torch, self.page_table, self.lengths, self.counts)
 
     def _check_tokens(self, k) -> None:
         if k.dim() == 4 and k.shape[2] < self._most:  # (their places would keep what the pages held)
@@ -221,6 +222,7 @@ class CacheBatch:
     def write(self, layer: int, k, v) -> None:
         """k: [B,Hkv,T,D], v: [B,Hkv,T,Dv]; the first tokens[i] rows of each sequence."""
         self._check_tokens(k)
+        self._kept.used(None)
         F.cache_write(k, v, self.cache.k_pages[layer], self.cache.v_pages[layer], self.page_table, self.lengths,
                       counts=self.counts)
         self._renew_bounds(layer)
@@ -234,6 +236,7 @@ class CacheBatch:
         """`write` with K turned by `rotary` (a Rotary) on the way. Returns q
         [B,H,T,D], the queries of the same tokens, turned too (None without)."""
         self._check_tokens(k)
+        self._kept.used(None)
         q = F.cache_append(k, v, self.cache.k_pages[layer], self.cache.v_pages[layer], self.page_table, self.lengths,
                            rotary, q=q, counts=self.counts)
         self._renew_bounds(layer)
@@ -246,6 +249,7 @@ class CacheBatch:
         from the back (such batches go in parts of one T, or prompts through
         window_attention with the batch's lengths)."""
         self._check_queries(q)
+        self._kept.used(options.get("stream"))
         return F.paged_attention(q, self.cache.k_pages[layer], self.cache.v_pages[layer], self.page_table,
                                  self.lengths, **options)
 
@@ -276,6 +280,7 @@ class CacheBatch:
     def attend_shared(self, layer: int, q, **options):
         """`attend`, with the pages that forks share read once for all of them."""
         self._check_queries(q)
+        self._kept.used(options.get("stream"))
         return F.shared_prefix_attention(q, self.cache.k_pages[layer], self.cache.v_pages[layer], self.page_table,
                                          self.lengths, groups=self.groups, **options)
 
@@ -287,6 +292,7 @@ class CacheBatch:
             raise ValueError("the cache has no bounds (PagedCache(bounds=True))")
         if q.dim() != 4:
             raise ValueError("q must be a rank-4 tensor")
+        self._kept.used(stream)
         attend = F.SelectedAttention(self.cache.k_pages[layer], self.cache.v_pages[layer], self.cache.k_bounds[layer],
                                      self.page_table, self.lengths, heads=q.shape[1], query_tokens=q.shape[2], pages=pages,
                                      **options)

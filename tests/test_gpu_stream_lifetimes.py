@@ -127,3 +127,34 @@ def test_frequencies_from_a_device_are_there(ofh, monkeypatch):
     given[3] = float("nan")
     with pytest.raises(ValueError, match="finite"):
         ofh.Rotary(64, frequencies=given)
+
+
+@pytest.mark.parametrize("method", ["attend", "attend_shared", "attend_selected", "write", "append"])
+def test_tables_of_a_dropped_batch(ofh, monkeypatch, method):
+    """A cache's batch is dropped with the next step's, and its tables with it."""
+    from onednn_flash_cache import PagedCache
+    cache = PagedCache(layers=1, num_pages=40, page_size=16, kv_heads=2, head_dim=64, bounds=True)
+    seqs = [cache.add() for _ in range(4)]
+    k, q = (torch.randn(4, h, 40, 64, device="cuda", dtype=torch.bfloat16) for h in (2, 8))
+    cache.extend(seqs, [40] * 4).write(0, k, k)
+    rotary = ofh.Rotary(64)
+    ptrs = spy(monkeypatch, ofh)
+    batch = cache.extend(seqs, [1] * 4)
+    k, q = k[:, :, :1].contiguous(), q[:, :, :1].contiguous()
+    batch.write(0, k, k)
+    call = {"attend": lambda **o: batch.attend(0, q, **o), "attend_shared": lambda **o: batch.attend_shared(0, q, **o),
+            "attend_selected": lambda **o: batch.attend_selected(0, q, pages=3, first_pages=0, **o),
+            "write": lambda: batch.write(0, k, k), "append": lambda: batch.append(0, k, k, rotary, q)}[method]
+    want = call()  # (also makes the batch's groups)
+    pages = cache.k_pages.clone()
+    for current in (True, False) if method.startswith("attend") else (True,):
+        busy = busy_stream()
+        if current:
+            with torch.cuda.stream(busy):
+                out = call()
+        else:
+            out = call(stream=busy)
+    del batch, call
+    assert len(ptrs) == (5 if method == "attend_shared" else 3) and not reused(ptrs, 64) and not busy.query()
+    busy.synchronize()
+    assert torch.equal(cache.k_pages, pages) and (want is None or torch.equal(out, want))

@@ -85,3 +85,19 @@ def test_groups_of_a_list_are_made_on_the_calls_stream(monkeypatch):
 def test_on_stream_of_the_cpu():
     with F._on_stream(torch, torch.device("cpu"), 7):
         pass
+
+
+def test_batches_tell_their_tables(monkeypatch):
+    import onednn_flash_cache as C
+    cache = C.PagedCache(layers=1, num_pages=8, page_size=16, kv_heads=2, head_dim=8, device="cpu", bounds=True)
+    batch = cache.extend([cache.add()], [1])
+    assert [id(t) for t in batch._kept.tensors] == [id(t) for t in (batch.page_table, batch.lengths, batch.counts)]
+    told = []
+    monkeypatch.setattr(batch._kept, "used", told.append)
+    side, q, k = Stream(3), torch.zeros(1, 4, 1, 8), torch.zeros(1, 2, 1, 8)
+    for call in (lambda: batch.write(0, k, k), lambda: batch.append(0, k, k, None), lambda: batch.attend(0, q),
+                 lambda: batch.attend(0, q, stream=side), lambda: batch.attend_shared(0, q, stream=side),
+                 lambda: batch.attend_selected(0, q, pages=4, stream=side)):
+        with pytest.raises(ValueError, match="GPU"):  # (past what a cache on the CPU can do)
+            call()
+    assert told == [None, None, None, side, side, side]
