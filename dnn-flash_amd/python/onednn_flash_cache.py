@@ -284,9 +284,10 @@ class CacheBatch:
         return F.shared_prefix_attention(q, self.cache.k_pages[layer], self.cache.v_pages[layer], self.page_table,
                                          self.lengths, groups=self.groups, **options)
 
-    def attend_selected(self, layer: int, q, *, pages: int, selected=None, out=None, stream=None, **options):
+    def attend_selected(self, layer: int, q, *, pages: int, selected=None, out=None, workspace=None, stream=None,
+                        **options):
         """`attend` over `pages` of each sequence's pages, of a cache with bounds;
-        options as SelectedAttention."""
+        options as SelectedAttention, which the other arguments are passed to."""
         self._check_queries(q)
         if self.cache.k_bounds is None:
             raise ValueError("the cache has no bounds (PagedCache(bounds=True))")
@@ -296,4 +297,4 @@ class CacheBatch:
         attend = F.SelectedAttention(self.cache.k_pages[layer], self.cache.v_pages[layer], self.cache.k_bounds[layer],
                                      self.page_table, self.lengths, heads=q.shape[1], query_tokens=q.shape[2], pages=pages,
                                      **options)
-        return attend(q, selected=selected, out=out, stream=stream)
+        return attend(q, selected=selected, out=out, workspace=workspace, stream=stream)

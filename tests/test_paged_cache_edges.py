@@ -49,3 +49,22 @@ def test_page_sizes_that_no_kernel_takes(size):
     with pytest.raises(ValueError, match="power of two, 16 or more"):
         cache(page_size=size)
     assert cache(page_size=64).pool.page_size == 64
+
+
+def test_arguments_of_selected_attention(monkeypatch):
+    """A batch passes a call's tensors on: the workspace among them."""
+    made, called = [], []
+
+    class Attention:
+        def __init__(self, *args, **options):
+            made.append(options)
+
+        def __call__(self, q, **options):
+            called.append(options)
+
+    monkeypatch.setattr(C.F, "SelectedAttention", Attention)
+    c = cache(bounds=True)
+    batch = c.extend([c.add()], [1])
+    call = dict(selected=1, out=2, workspace=3, stream=None)
+    batch.attend_selected(0, torch.zeros(1, 4, 1, 8), pages=4, recent_pages=1, **call)
+    assert made == [dict(heads=4, query_tokens=1, pages=4, recent_pages=1)] and called == [call]
