@@ -865,14 +865,15 @@ class _Kept:
         self._torch, self.tensors, self._index = torch, tensors, tensors[0].device.index
         self._told = set()
         if self._index is not None:  # (None: on the CPU)
-            self._told.add(torch._C._cuda_getCurrentRawStream(self._index))
+            self._current = torch._C._cuda_getCurrentRawStream
+            self._told.add(self._current(self._index))
 
     def used(self, stream) -> None:
         """A call on `stream` (as _launch takes it) reads the tensors."""
         if self._index is None:
             return
         if stream is None:
-            if self._torch._C._cuda_getCurrentRawStream(self._index) in self._told:
+            if self._current(self._index) in self._told:
                 return
             stream = self._torch.cuda.current_stream(self._index)
         elif not isinstance(stream, self._torch.cuda.Stream):
