@@ -155,6 +155,9 @@ class PagedCache:
         if page_size < 16 or page_size & (page_size - 1):  # (what the kernels read and write)
             raise ValueError("page_size must be a power of two, 16 or more")
         dtype = torch.bfloat16 if dtype is None else dtype
+        step = 16 // dtype.itemsize
+        if bounds and (head_dim % step or not 0 < head_dim <= 256):  # (refused later, a batch would have written its rows)
+            raise ValueError(f"a cache with bounds needs a head_dim that is a multiple of {step} up to 256")
         shape = (layers, num_pages, kv_heads, page_size)
         # (zeros: what a page holds past its tokens is never seen, but a program may look)
         self.k_pages = torch.zeros((*shape, head_dim), dtype=dtype, device=device)

@@ -68,3 +68,16 @@ def test_arguments_of_selected_attention(monkeypatch):
     call = dict(selected=1, out=2, workspace=3, stream=None)
     batch.attend_selected(0, torch.zeros(1, 4, 1, 8), pages=4, recent_pages=1, **call)
     assert made == [dict(heads=4, query_tokens=1, pages=4, recent_pages=1)] and called == [call]
+
+
+@pytest.mark.parametrize("dtype,good,bad", [(torch.float32, (4, 20, 256), (2, 66, 260)), (torch.bfloat16, (8, 24, 256), (4, 20, 264)),
+                                            (torch.float16, (8, 136), (12, 260))])
+def test_head_dims_of_a_cache_with_bounds(dtype, good, bad):
+    """The bounds' kernels take rows of 16-byte words up to 256 columns: others are refused
+    when the cache is made, not by a write whose rows are then in their pages."""
+    for D in good:
+        assert cache(head_dim=D, dtype=dtype, bounds=True).k_bounds.shape == (1, 8, 2, 2, D)
+    for D in bad:
+        with pytest.raises(ValueError, match="a cache with bounds needs"):
+            cache(head_dim=D, dtype=dtype, bounds=True)
+        assert cache(head_dim=D, dtype=dtype).k_bounds is None
