@@ -5,7 +5,12 @@
 // page's keys k when q is a head of its group:
 //     max over the group's heads of sum_d q_d (q_d > 0 ? hi_d : lo_d),
 // hi and lo the columns' largest and smallest values in the page. The sum is
-// formed in 64 bits and rounded to fp32: its order then decides no rank.
+// formed in 64 bits and rounded to fp32. Products of 16-bit numbers are exact there
+// (bf16 16 bits, fp16 22), and so are sums of up to 256 while the products' exponents
+// lie within 29 (bf16) or 23 (fp16) of each other: their order then decides nothing.
+// Otherwise, and in fp32, another order moves the last of the sum's 64-bit digits, and
+// a score, a tie or a rank only where the sum is that near to the middle between two
+// fp32 numbers.
 
 #include <algorithm>
 #include <type_traits>
@@ -157,10 +162,10 @@ constexpr int kScoreQuery = 4096;   // numbers of Q that a workgroup keeps at mo
 // for a word. Tokens that see no more pages than they may take need no scores.
 //
 // What bounds it (bf16, 32 sequences of 2000-32768 tokens, pages of 32, H32/8 D128: 71 MB
-// of bounds, 22.5 us): half the sums, half the reading of 512 bytes here and there
-// (without the sums 17); the same sums in fp32 save nothing. Workgroups are
-// numbered chunk by chunk, since row by row the late chunks, which only long
-// sequences have, fall on the same XCDs: 26.6.
+// of bounds, 23.9 us in a trace): the reading of 512 bytes here and there, and beside it
+// the sums (without them 19.8; in fp32 22.8). Workgroups are numbered chunk by chunk,
+// since row by row the late chunks, which only long sequences have, fall on the same
+// XCDs: 29.0.
 template <typename T>
 __global__ __launch_bounds__(kSelectThreads) void page_score_kernel(SelectArgs a, int per, int lanes, int heads_kept) {
     using X = Words<T>;

@@ -4,9 +4,10 @@
 // Pair (x, y) at position p becomes m (x cos a - y sin a, y cos a + x sin a),
 // a = p f_i, or with -a in the transposed form (the gradient of the other).
 // The angle is formed in 64 bits in turns and brought within half a turn
-// there, so that far positions keep their digits: p f_i / 2 pi is off by 2^-52 of
-// itself, 2^-31 turns at p = 2^21, where 32 bits would be off by a sixteenth of
-// a turn. Sine and cosine are then fp32, with what the angle's rounding to fp32 takes
+// there, so that far positions keep their digits: p f_i / 2 pi takes three roundings
+// (of 1 / 2 pi, times f_i, times p), each 2^-53 of it at most. At p = 2^21 and f_i = 1, 2^18.3
+// turns, they are 2^-33 turns together, where each of 32 bits could be 2^-5.7,
+// a fiftieth of a turn. Sine and cosine are then fp32, with what the angle's rounding to fp32 takes
 // off put back to first order, and so are the products; the result is rounded once.
 //
 // Both kernels are bound by reading and writing each row once. A wavefront (or,

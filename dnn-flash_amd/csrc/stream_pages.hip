@@ -7,6 +7,12 @@
 //  * selected pages (kSelected): a tile per token and key-value head, whose
 //    16-key blocks are those of the pages on its list.
 //
+// Probabilities are rounded to the inputs' type for their product with V, and alike in
+// the row's sum, as in all of the library's 16-bit attention: half a step each, averaged
+// over the keys, is about what the rounding of the result is (rms of normal rows: bf16
+// 1.6e-3 and 1.7e-3, both 2.3e-3; fp16 2.0e-4, 2.1e-4, both 2.9e-4). In 32 bits each
+// product with V would be two, of P's upper and lower half. fp32 keeps its own.
+//
 // Measured (us) and what bounds it: few rows are latency, launch, table, K, V and the
 // join's launch in turn (bf16 4 sequences, H32/8 D128, 1024 shared 12.6, of which the
 // join 4.2; fp32 D64 3 groups of 5 with 3 tokens, H8, 4000 shared 24.5, 60 MB, matrix

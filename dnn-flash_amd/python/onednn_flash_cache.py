@@ -144,8 +144,9 @@ class PagePool:
 class PagedCache:
     """The K and V pools of `layers` layers, [layers, P, Hkv, S, D], and the
     sequences in them; with `bounds` also the bounds of the pages' keys, [layers, P,
-    Hkv, 2, D], which batches keep up to date and attend_selected reads. Copies run on the current stream; a program that uses the
-    cache from several streams orders them itself."""
+    Hkv, 2, D], which batches keep up to date and attend_selected reads. Copies run on
+    the current stream; a program that uses the cache from several streams orders them
+    itself."""
 
     def __init__(self, *, layers: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int,
                  value_dim: int | None = None, dtype=None, device="cuda", bounds: bool = False):

@@ -1482,7 +1482,7 @@ class Rotary:
         is at position offset + t; or positions[t] or positions[b, t] (int32
         device [T] or [B,T]); or lengths[b] - T + t (int32 device [B]: the last
         T of lengths[b] tokens). `transpose` turns back: the gradient of x from
-        that of the result. out: x itself, or a tensor like it. Returns out."""
+        that of the result. out: x itself, or a tensor like it elsewhere. Returns out."""
         torch, dev = self._torch, self._device
         layout = (x.shape, x.stride(), x.dtype, x.device) if isinstance(x, torch.Tensor) else None
         held = self._held
