@@ -858,8 +858,9 @@ class _Kept:
     """Device tensors of the library's own that kernels read, on whichever stream an
     object is called. When nothing holds them their memory goes to the next tensor of
     the stream that they were made on, so a call on another torch stream tells the
-    allocator, which then waits for it. (Not for a stream given by its handle, which
-    may be gone by then: such a call's object is kept until it has run.)"""
+    allocator, which then waits for it. (Not for a stream given by its handle or as an
+    ExternalStream, which may be gone by then and is nothing to wait for: such a call's
+    object is kept until it has run.)"""
 
     def __init__(self, torch, *tensors):
         self._torch, self.tensors, self._index = torch, tensors, tensors[0].device.index
@@ -876,7 +877,7 @@ class _Kept:
             if self._current(self._index) in self._told:
                 return
             stream = self._torch.cuda.current_stream(self._index)
-        elif not isinstance(stream, self._torch.cuda.Stream):
+        elif not isinstance(stream, self._torch.cuda.Stream) or isinstance(stream, self._torch.cuda.ExternalStream):
             return
         if stream.cuda_stream not in self._told:
             for t in self.tensors:

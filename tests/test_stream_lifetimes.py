@@ -19,6 +19,10 @@ class Stream:
         self.cuda_stream = handle
 
 
+class ExternalStream(Stream):
+    pass
+
+
 class Tensor:
     def __init__(self, index=0):
         self.device = types.SimpleNamespace(index=index)
@@ -34,7 +38,7 @@ class Torch:
     def __init__(self):
         self.current = Stream(0)
         self._C = types.SimpleNamespace(_cuda_getCurrentRawStream=lambda index: self.current.cuda_stream)
-        self.cuda = types.SimpleNamespace(Stream=Stream, current_stream=lambda index: self.current)
+        self.cuda = types.SimpleNamespace(Stream=Stream, ExternalStream=ExternalStream, current_stream=lambda index: self.current)
 
 
 def test_kept_tensors_know_their_streams():
@@ -44,6 +48,7 @@ def test_kept_tensors_know_their_streams():
     kept.used(None)         # the stream that they were made on
     kept.used(Stream(0))
     kept.used(7)            # a handle: the caller keeps the object
+    kept.used(ExternalStream(9))
     assert all(x.recorded == [] for x in tensors)
     kept.used(Stream(3))
     kept.used(Stream(3))    # (known by now)
